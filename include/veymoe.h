@@ -347,6 +347,90 @@ typedef struct VmGroupedArgs {
   uint32_t act_dtype, combine_mode;
 } VmGroupedArgs;
 
+/* MX rows: e4m3 values with one e8m0 scale per group of VM_MX_GROUP along the
+ * row.  A group's scale is the least 2^e, e >= -127, with max|v| <= 448 * 2^e,
+ * stored as e + 127; a value is v * 2^-e rounded to the nearest e4m3, ties to
+ * even.  A group with an infinity or a NaN has scale 0xff and NaN values. */
+#define VM_MX_GROUP 32
+
+/* vm_rms_norm: per row, fp32 throughout and rounded once where it is stored,
+ *   h   = x + residual                        (residual NULL: h = x)
+ *   out = h / sqrt(mean(h^2) + eps) * gain    gain = weight (one_centered) or 1 + weight
+ * as `out` [rows, width] in act_dtype, or as MX rows `values` [rows, width] and
+ * `scales` [rows, width / 32], contiguous (width a multiple of 32, values
+ * 8-byte aligned).  `sum_out` optionally receives h in act_dtype; it may be x
+ * or residual, and out may be x.  Strides count elements between rows.
+ * width up to VM_NORM_MAX_WIDTH.  No counterpart in the reference's surface
+ * beyond its norm (patch_rmsnorm.py:108-135). */
+#define VM_NORM_MAX_WIDTH 16384
+typedef struct VmNormArgs {
+  const void* x;                 /* [rows, width] act_dtype */
+  const void* residual;          /* optional [rows, width] act_dtype */
+  const void* weight;            /* [width] weight_dtype */
+  void* out;                     /* either out, */
+  void* sum_out;                 /* optional [rows, width] act_dtype */
+  uint8_t* values;               /* or values and scales */
+  uint8_t* scales;
+  uint64_t x_stride, residual_stride, out_stride, sum_stride;
+  uint32_t rows, width, act_dtype, weight_dtype, one_centered;
+  float eps;
+} VmNormArgs;
+
+/* Element formats of vm_grouped_matmul's operands. */
+#define VM_FORMAT_BF16 0u
+#define VM_FORMAT_MX 1u
+#define VM_ACTIVATION_NONE 0u
+#define VM_ACTIVATION_SWIGLU 1u
+
+/* vm_grouped_matmul: routed rows times their expert's matrix, fp32 sums:
+ *   out[i] = x[i / x_div] . weight[ids[i]]^T            i < rows
+ * VM_ACTIVATION_SWIGLU: the matrix has 2 n rows, gate then up, and
+ * out = silu(gate) * up in fp32.  bf16 or MX operands (both the same), output
+ * in bf16 or, with swiglu and n a multiple of 32, as MX rows.  An id outside
+ * 0..experts-1 gives a row of zeros.
+ * k: a multiple of 8 (bf16) or 32 (MX); rows of x and weight 16-byte aligned,
+ * `out` 8-byte and `out_values` 4-byte aligned; out, out_values and out_scales
+ * contiguous.  experts up to VM_PRODUCT_MAX_EXPERTS.  Strides count elements
+ * (of an MX scale array: scales).  The workspace needs no initialisation. */
+#define VM_PRODUCT_MAX_EXPERTS 1024
+typedef struct VmProductArgs {
+  const void* x;                 /* [ceil(rows / x_div), k] */
+  const uint8_t* x_scales;       /* MX: [ceil(rows / x_div), k / 32] */
+  const void* weight;            /* [experts, n or 2 n, k] */
+  const uint8_t* weight_scales;  /* MX: [experts, n or 2 n, k / 32] */
+  const int32_t* ids;            /* [rows] */
+  void* out;                     /* [rows, n] bf16, or */
+  uint8_t* out_values;           /* [rows, n] and */
+  uint8_t* out_scales;           /* [rows, n / 32] */
+  void* workspace;
+  uint64_t workspace_bytes;
+  uint64_t x_stride, x_scale_stride;
+  uint64_t weight_stride, weight_expert_stride, weight_scale_stride, weight_scale_expert_stride;
+  uint32_t rows, x_div, k, n, experts, format, activation;
+} VmProductArgs;
+
+/* vm_add_adapters: low-rank adapters of many requests beside the projection
+ * they share, bf16 with fp32 sums:
+ *   out[t] = base[t] + scales[i] * b[i] (a[i] x[t]),  i = ids[t]
+ * and out[t] = base[t] for an id outside 0..adapters-1.  out may be base, and
+ * overlaps no other operand.  rank up to VM_ADAPTER_MAX_RANK, adapters up to
+ * VM_PRODUCT_MAX_EXPERTS.  Strides count elements.  The workspace needs no
+ * initialisation. */
+#define VM_ADAPTER_MAX_RANK 128
+typedef struct VmAdapterArgs {
+  const void* base;              /* [rows, n] */
+  const void* x;                 /* [rows, k] */
+  const void* a;                 /* [adapters, rank, k] */
+  const void* b;                 /* [adapters, n, rank] */
+  const float* scales;           /* optional [adapters], 1 without */
+  const int32_t* ids;            /* [rows] */
+  void* out;                     /* [rows, n] */
+  void* workspace;
+  uint64_t workspace_bytes;
+  uint64_t base_stride, x_stride, out_stride;
+  uint32_t rows, k, n, rank, adapters;
+} VmAdapterArgs;
+
 int vm_abi_version(void);
 /* 1 when a gfx950 device is usable by this library, else 0. */
 int vm_available(void);
@@ -391,6 +475,18 @@ uint64_t vm_moe_grouped_workspace(uint32_t tokens, uint32_t top_k, uint32_t hidd
                                   uint32_t inter_size, uint32_t expert_count, uint32_t act_dtype);
 int vm_moe_grouped(const VmGroupedArgs* args, void* stream);
 
+int vm_rms_norm(const VmNormArgs* args, void* stream);
+/* Rows of act_dtype, x_stride elements apart, as contiguous MX rows (the
+ * rules of VmNormArgs). */
+int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* scales, uint32_t rows, uint32_t width,
+                   uint32_t act_dtype, void* stream);
+
+uint64_t vm_grouped_matmul_workspace(uint32_t rows, uint32_t experts);
+int vm_grouped_matmul(const VmProductArgs* args, void* stream);
+
+uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t adapters);
+int vm_add_adapters(const VmAdapterArgs* args, void* stream);
+
 /* out[t, h] = sum_j expert_outputs[t, j, h] * scores[t, j] in fp32, written in
  * act_dtype; the normal form of weighted_combine (metal_runtime.py:145-191). */
 int vm_weighted_combine(const void* expert_outputs, const void* scores, void* out,
@@ -433,7 +529,8 @@ int vm_decode_pipeline(int mode);
  * enabled, every kernel the library launches is bracketed by hipEvents on its
  * stream; vm_timing_read returns the summed milliseconds and launch count of
  * the kernel family `name` ("router", "gateup", "down", "experts",
- * "grouped_gateup", "grouped_down", "sort", "combine"). */
+ * "grouped_gateup", "grouped_down", "sort", "combine", "norm", "products",
+ * "adapters"). */
 int vm_timing_enable(int enabled);
 int vm_timing_read(const char* name, double* total_ms, uint64_t* launches);
 int vm_timing_reset(void);

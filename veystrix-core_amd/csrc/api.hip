@@ -1492,6 +1492,279 @@ int vm_weighted_combine(const void* expert_outputs, const void* scores, void* ou
   return VM_OK;
 }
 
+// --------------------------------------------------------------- norm ---
+
+// Blocks of a launch: the grid's threads are counted in 32 bits.
+constexpr uint64_t kMaxBlocks = (1ull << 24) - 1;
+
+static bool rows_aligned(const void* p, uint64_t stride_bytes, uint32_t unit) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % unit == 0 && stride_bytes % unit == 0);
+}
+
+static int check_mx_rows(const uint8_t* values, const uint8_t* scales, uint32_t width) {
+  if (values == nullptr || scales == nullptr) return fail(VM_EINVAL, "MX rows need both values and scales");
+  if (width % VM_MX_GROUP) return fail(VM_EINVAL, "MX rows need a width that is a multiple of %d", VM_MX_GROUP);
+  if (reinterpret_cast<uintptr_t>(values) % 8) return fail(VM_EINVAL, "MX values must be 8-byte aligned");
+  return VM_OK;
+}
+
+static int run_norm(vm::NormLaunch& p, void* stream) {
+  const uint64_t bytes = p.act_dtype == static_cast<int>(VM_F32) ? 4 : 2;
+  p.vector = p.width % 8 == 0 && rows_aligned(p.x, p.x_stride * bytes, 16) &&
+             rows_aligned(p.residual, p.residual_stride * bytes, 16) &&
+             rows_aligned(p.out, p.out_stride * bytes, 16) && rows_aligned(p.sum_out, p.sum_stride * bytes, 16) &&
+             rows_aligned(p.weight, 0, 16);
+  const hipError_t e = vm::launch_norm(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "norm launch");
+  return VM_OK;
+}
+
+int vm_rms_norm(const VmNormArgs* a, void* stream) {
+  if (a == nullptr) return fail(VM_EINVAL, "null arguments");
+  if (a->act_dtype > VM_F32 || a->weight_dtype > VM_F32) return fail(VM_EINVAL, "dtypes must be bf16 or f32");
+  if (a->width == 0 || a->width > VM_NORM_MAX_WIDTH)
+    return fail(VM_EUNSUPPORTED, "width must be 1..%d", VM_NORM_MAX_WIDTH);
+  if (a->rows > kMaxBlocks) return fail(VM_EUNSUPPORTED, "at most %llu rows per call", (unsigned long long)kMaxBlocks);
+  if (a->rows == 0) return VM_OK;
+  if (a->x == nullptr || a->weight == nullptr) return fail(VM_EINVAL, "x and weight are required");
+  const bool mx = a->values != nullptr || a->scales != nullptr;
+  if (mx == (a->out != nullptr)) return fail(VM_EINVAL, "either out or MX values and scales are required");
+  if (mx) {
+    const int rc = check_mx_rows(a->values, a->scales, a->width);
+    if (rc != VM_OK) return rc;
+  }
+  const uint64_t w = a->width;
+  if (a->rows > 1 && ((a->out != nullptr && a->out_stride < w) || (a->sum_out != nullptr && a->sum_stride < w)))
+    return fail(VM_EINVAL, "the row strides of outputs must be at least the width");
+  vm::NormLaunch p{};
+  p.x = a->x;
+  p.residual = a->residual;
+  p.weight = a->weight;
+  p.out = a->out;
+  p.sum_out = a->sum_out;
+  p.values = a->values;
+  p.scales = a->scales;
+  p.x_stride = a->x_stride;
+  p.residual_stride = a->residual_stride;
+  p.out_stride = a->out_stride;
+  p.sum_stride = a->sum_stride;
+  p.rows = a->rows;
+  p.width = a->width;
+  p.one_centered = a->one_centered ? 1u : 0u;
+  p.eps = a->eps;
+  p.act_dtype = static_cast<int>(a->act_dtype);
+  p.weight_dtype = static_cast<int>(a->weight_dtype);
+  return run_norm(p, stream);
+}
+
+int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* scales, uint32_t rows, uint32_t width,
+                   uint32_t act_dtype, void* stream) {
+  if (act_dtype > VM_F32) return fail(VM_EINVAL, "act_dtype must be bf16 or f32");
+  if (width == 0 || width > VM_NORM_MAX_WIDTH) return fail(VM_EUNSUPPORTED, "width must be 1..%d", VM_NORM_MAX_WIDTH);
+  if (rows > kMaxBlocks) return fail(VM_EUNSUPPORTED, "at most %llu rows per call", (unsigned long long)kMaxBlocks);
+  if (rows == 0) return VM_OK;
+  if (x == nullptr) return fail(VM_EINVAL, "x is required");
+  const int rc = check_mx_rows(values, scales, width);
+  if (rc != VM_OK) return rc;
+  vm::NormLaunch p{};
+  p.x = x;
+  p.x_stride = x_stride;
+  p.values = values;
+  p.scales = scales;
+  p.rows = rows;
+  p.width = width;
+  p.act_dtype = static_cast<int>(act_dtype);
+  return run_norm(p, stream);
+}
+
+// ----------------------------------------------------- sorted row calls ---
+
+// Workspace of a sort of `rows` ids into `groups` groups, laid out for tiles
+// of `tile_rows` rows.
+struct RowSortWs {
+  uint64_t row_off, tiles, tiles_dn, tile_count, counts, row_token, row_pair, total;
+};
+
+static RowSortWs row_sort_ws(uint32_t rows, uint32_t groups, uint32_t tile_rows) {
+  RowSortWs w{};
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t r = at;
+    at += align_up(bytes);
+    return r;
+  };
+  const uint64_t tiles = uint64_t(vm::grouped_max_tiles(rows, groups, tile_rows)) * sizeof(uint2);
+  w.row_off = take((uint64_t(groups) + 1) * 4);
+  w.tile_count = take(2 * 4);
+  w.counts = take(2 * 1024 * 4);
+  w.tiles = take(tiles);
+  w.tiles_dn = take(tiles);
+  w.row_token = take(uint64_t(rows) * 4);
+  w.row_pair = take(uint64_t(rows) * 4);
+  w.total = at;
+  return w;
+}
+
+static hipError_t sort_rows(const int32_t* ids, uint32_t rows, uint32_t groups, uint32_t tile_rows, const RowSortWs& w,
+                            char* ws, hipStream_t stream) {
+  vm::SortLaunch s{};
+  s.inds = ids;
+  s.row_off = reinterpret_cast<uint32_t*>(ws + w.row_off);
+  s.tiles = reinterpret_cast<uint2*>(ws + w.tiles);
+  s.tiles_dn = reinterpret_cast<uint2*>(ws + w.tiles_dn);
+  s.tile_count = reinterpret_cast<uint32_t*>(ws + w.tile_count);
+  s.tile_count_dn = s.tile_count + 1;
+  s.counts = reinterpret_cast<uint32_t*>(ws + w.counts);
+  s.cursors = s.counts + 1024;
+  s.row_token = reinterpret_cast<uint32_t*>(ws + w.row_token);
+  s.pair_row = reinterpret_cast<uint32_t*>(ws + w.row_pair);
+  s.tokens = rows;
+  s.slots = 1;
+  s.experts = groups;
+  s.tile_rows = s.tile_rows_dn = tile_rows;
+  s.by_row = true;
+  return vm::launch_sort(s, stream);
+}
+
+// ----------------------------------------------------- grouped products ---
+
+uint64_t vm_grouped_matmul_workspace(uint32_t rows, uint32_t experts) {
+  const uint32_t tile = experts == 0 ? 0 : vm::product_tile_rows(rows, experts);
+  return tile == 0 ? 0 : row_sort_ws(rows, experts, tile).total;
+}
+
+int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
+  if (a == nullptr) return fail(VM_EINVAL, "null arguments");
+  const hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  if (a->format > VM_FORMAT_MX) return fail(VM_EINVAL, "format must be bf16 or MX");
+  if (a->activation > VM_ACTIVATION_SWIGLU) return fail(VM_EINVAL, "unknown activation");
+  const bool mx = a->format == VM_FORMAT_MX, swiglu = a->activation == VM_ACTIVATION_SWIGLU;
+  if (a->k == 0 || a->n == 0) return fail(VM_EINVAL, "k and n must be positive");
+  if (a->experts == 0 || a->experts > VM_PRODUCT_MAX_EXPERTS)
+    return fail(VM_EUNSUPPORTED, "experts must be 1..%d", VM_PRODUCT_MAX_EXPERTS);
+  if (a->x_div == 0) return fail(VM_EINVAL, "x_div must be positive");
+  const uint32_t size = mx ? 1 : 2, unit = mx ? VM_MX_GROUP : 8;
+  if (a->k % unit) return fail(VM_EUNSUPPORTED, "k must be a multiple of %u", unit);
+  if (a->k > (1u << 24) || a->n > (1u << 24) || a->rows > (1u << 28))
+    return fail(VM_EUNSUPPORTED, "k and n of at most 2^24 and rows of at most 2^28");
+  if (a->rows == 0) return VM_OK;
+  if (a->x == nullptr || a->weight == nullptr || a->ids == nullptr) return fail(VM_EINVAL, "x, weight and ids are required");
+  if (mx && (a->x_scales == nullptr || a->weight_scales == nullptr))
+    return fail(VM_EINVAL, "MX operands need x_scales and weight_scales");
+  const bool mx_out = a->out_values != nullptr || a->out_scales != nullptr;
+  if (mx_out == (a->out != nullptr)) return fail(VM_EINVAL, "either out or out_values and out_scales are required");
+  if (mx_out) {
+    if (!swiglu) return fail(VM_EUNSUPPORTED, "MX output is written by the swiglu activation");
+    const int rc = check_mx_rows(a->out_values, a->out_scales, a->n);
+    if (rc != VM_OK) return rc;
+  } else if (reinterpret_cast<uintptr_t>(a->out) % 8) {
+    return fail(VM_EINVAL, "out must be 8-byte aligned");
+  }
+  if (!rows_aligned(a->x, a->x_stride * size, 16) || !rows_aligned(a->weight, a->weight_stride * size, 16) ||
+      a->weight_expert_stride * size % 16)
+    return fail(VM_EINVAL, "rows of x and weight must be 16-byte aligned");
+  const uint32_t tile = vm::product_tile_rows(a->rows, a->experts);
+  if (vm::product_blocks(a->rows, a->experts, a->n, tile, swiglu) > kMaxBlocks)
+    return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
+  vm::ProductLaunch p{};
+  if (tile != 0) {
+    const RowSortWs w = row_sort_ws(a->rows, a->experts, tile);
+    if (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace))
+      return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
+    char* ws = static_cast<char*>(a->workspace);
+    const hipError_t e = sort_rows(a->ids, a->rows, a->experts, tile, w, ws, stream);
+    if (e != hipSuccess) return hip_fail(e, "sort launch");
+    p.row_off = reinterpret_cast<const uint32_t*>(ws + w.row_off);
+    p.tiles = reinterpret_cast<const uint2*>(ws + w.tiles);
+    p.tile_count = reinterpret_cast<const uint32_t*>(ws + w.tile_count);
+    p.row_pair = reinterpret_cast<const uint32_t*>(ws + w.row_pair);
+  }
+  p.x = static_cast<const uint8_t*>(a->x);
+  p.x_scales = a->x_scales;
+  p.w = static_cast<const uint8_t*>(a->weight);
+  p.w_scales = a->weight_scales;
+  p.x_stride = a->x_stride * size;
+  p.x_scale_stride = a->x_scale_stride;
+  p.w_stride = a->weight_stride * size;
+  p.w_expert = a->weight_expert_stride * size;
+  p.w_scale_stride = a->weight_scale_stride;
+  p.w_scale_expert = a->weight_scale_expert_stride;
+  p.ids = a->ids;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.values = a->out_values;
+  p.scales = a->out_scales;
+  p.rows = a->rows;
+  p.x_div = a->x_div;
+  p.k_bytes = a->k * size;
+  p.n = a->n;
+  p.experts = a->experts;
+  p.mx = mx;
+  p.swiglu = swiglu;
+  const hipError_t e = vm::launch_products(p, tile, stream);
+  if (e != hipSuccess) return hip_fail(e, "products launch");
+  return VM_OK;
+}
+
+// ----------------------------------------------------------- adapters ---
+
+uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t adapters) {
+  return rows <= vm::kAdapterRows ? 0 : row_sort_ws(rows, adapters, vm::kAdapterTile).total;
+}
+
+int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
+  if (a == nullptr) return fail(VM_EINVAL, "null arguments");
+  const hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+  if (a->k == 0 || a->n == 0 || a->k > (1u << 24) || a->n > (1u << 24))
+    return fail(VM_EINVAL, "k and n must be 1..2^24");
+  if (a->rank == 0 || a->rank > VM_ADAPTER_MAX_RANK)
+    return fail(VM_EUNSUPPORTED, "rank must be 1..%d", VM_ADAPTER_MAX_RANK);
+  if (a->adapters == 0 || a->adapters > VM_PRODUCT_MAX_EXPERTS)
+    return fail(VM_EUNSUPPORTED, "adapters must be 1..%d", VM_PRODUCT_MAX_EXPERTS);
+  if (a->rows == 0) return VM_OK;
+  if (a->base == nullptr || a->x == nullptr || a->a == nullptr || a->b == nullptr || a->ids == nullptr || a->out == nullptr)
+    return fail(VM_EINVAL, "base, x, a, b, ids and out are required");
+  if (a->rows > 1 && a->out_stride < a->n) return fail(VM_EINVAL, "the row stride of out must be at least n");
+  if (a->out == a->base && a->out_stride != a->base_stride && a->rows > 1)
+    return fail(VM_EINVAL, "in place, base and out must have one stride");
+  const bool tiled = a->rows > vm::kAdapterRows;
+  vm::AdapterLaunch p{};
+  p.base = static_cast<const uint16_t*>(a->base);
+  p.x = static_cast<const uint16_t*>(a->x);
+  p.a = static_cast<const uint16_t*>(a->a);
+  p.b = static_cast<const uint16_t*>(a->b);
+  p.scales = a->scales;
+  p.ids = a->ids;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.base_stride = a->base_stride;
+  p.x_stride = a->x_stride;
+  p.out_stride = a->out_stride;
+  p.rows = a->rows;
+  p.k = a->k;
+  p.n = a->n;
+  p.rank = a->rank;
+  p.adapters = a->adapters;
+  p.vector_k = a->k % 8 == 0 && rows_aligned(a->x, a->x_stride * 2, 16) && aligned16(a->a);
+  p.vector_rank = a->rank % 8 == 0 && aligned16(a->b);
+  p.quads = a->n % 4 == 0 && rows_aligned(a->base, a->base_stride * 2, 8) && rows_aligned(a->out, a->out_stride * 2, 8);
+  if (vm::adapter_blocks(a->rows, a->adapters, a->n, tiled) > kMaxBlocks)
+    return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
+  if (tiled) {
+    const RowSortWs w = row_sort_ws(a->rows, a->adapters, vm::kAdapterTile);
+    if (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace))
+      return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
+    char* ws = static_cast<char*>(a->workspace);
+    const hipError_t e = sort_rows(a->ids, a->rows, a->adapters, vm::kAdapterTile, w, ws, stream);
+    if (e != hipSuccess) return hip_fail(e, "sort launch");
+    p.row_off = reinterpret_cast<const uint32_t*>(ws + w.row_off);
+    p.tiles = reinterpret_cast<const uint2*>(ws + w.tiles);
+    p.tile_count = reinterpret_cast<const uint32_t*>(ws + w.tile_count);
+    p.row_pair = reinterpret_cast<const uint32_t*>(ws + w.row_pair);
+  }
+  const hipError_t e = vm::launch_adapters(p, tiled, stream);
+  if (e != hipSuccess) return hip_fail(e, "adapters launch");
+  return VM_OK;
+}
+
 // -------------------------------------------------------------- stage ---
 
 int vm_pool_stage(void* pool_base, uint64_t header_size, uint64_t record_stride, uint64_t pool_records,

@@ -1,0 +1,197 @@
+// Root-mean-square norm of rows with the residual's addition in front of it, and rows in MX (vm_mx.h).
+//
+//   h = x + residual                       fp32; stored rounded to the input's type where sum_out is given
+//   y = h * (1 / sqrt(mean(h^2) + eps)) * gain, gain = weight or 1 + weight
+//
+// The norm reads the unrounded h: the sum is rounded once, where it is stored.  y is rounded once, to the input's
+// type or to e4m3 under the scale of its group of 32.  Without a weight the rows are only converted to MX.
+//
+// A row is read once and stays in registers, eight consecutive values per thread and step, so that four lanes hold a
+// scale's group and its maximum takes two DPP steps.  Calls are bound by HBM (two rows in, one and a half out, five
+// operations a value) or, with few rows, by one row's latency:
+//   * many rows: one wave per row, no barrier, four rows per block;
+//   * few rows, or rows wider than a wave's registers: one block of 256 threads per row, so that a row's loads are one
+//     round trip.
+// Rows that are not 16-byte aligned, or whose width is not a multiple of eight, take the same code with element loads
+// and stores.
+
+#include <hip/hip_ext.h>
+#include <hip/hip_runtime.h>
+
+#include "vm_internal.h"
+#include "vm_mx.h"
+
+namespace vm {
+
+namespace {
+
+constexpr int kNormThreads = 256;
+
+// Eight consecutive values from element `at` of a row; those at `width` and behind it are zero.
+template <class A, bool VEC>
+__device__ __forceinline__ void load8(const void* row, uint32_t at, uint32_t width, float v[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+  if constexpr (VEC) {
+    if (at >= width) return;
+    const uint8_t* src = static_cast<const uint8_t*>(row) + static_cast<size_t>(at) * A::kBytes;
+    const uint4 a = ldg16(src);
+    if constexpr (A::kBytes == 2) {
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+      const uint4 b = ldg16(src + 16);
+      v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+      v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at + j < width) v[j] = A::load(row, at + j);
+  }
+}
+
+template <class A, bool VEC>
+__device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t width, const float v[8]) {
+  if constexpr (VEC) {
+    if (at >= width) return;
+    if constexpr (A::kBytes == 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(v[2 * j]) | (f32_to_bf16(v[2 * j + 1]) << 16);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(row) + at);
+      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (at + j < width) A::store(row, at + j, v[j]);
+  }
+}
+
+// TPR threads per row (64 or 256), up to NV steps of eight values per thread.
+template <class A, int TPR, int NV, bool VEC>
+__global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
+  const uint32_t t = threadIdx.x % TPR;
+  const uint32_t row = blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR;
+  if (row >= p.rows) return;  // TPR 64: whole waves; TPR 256: never
+  const auto row_of = [&](const void* base, uint64_t stride) {
+    return static_cast<const uint8_t*>(base) + static_cast<uint64_t>(row) * stride * A::kBytes;
+  };
+  float h[NV][8];
+  const uint8_t* x = row_of(p.x, p.x_stride);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) load8<A, VEC>(x, (i * TPR + t) * 8u, p.width, h[i]);
+  if (p.residual != nullptr) {
+    const uint8_t* r = row_of(p.residual, p.residual_stride);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float v[8];
+      load8<A, VEC>(r, (i * TPR + t) * 8u, p.width, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] += v[j];
+    }
+  }
+  float scale = 1.0f;
+  if (p.weight != nullptr) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+    ss = wave_sum_all(ss);
+    if constexpr (TPR > 64) {
+      __shared__ float s_part[TPR / 64];
+      if (t % 64 == 0) s_part[t / 64] = ss;
+      __syncthreads();
+      ss = 0.0f;
+#pragma unroll
+      for (int w = 0; w < TPR / 64; ++w) ss += s_part[w];
+    }
+    scale = 1.0f / sqrtf(ss / static_cast<float>(p.width) + p.eps);
+  }
+  if (p.sum_out != nullptr) {
+    uint8_t* s = const_cast<uint8_t*>(row_of(p.sum_out, p.sum_stride));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store8<A, VEC>(s, (i * TPR + t) * 8u, p.width, h[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t at = (i * TPR + t) * 8u;
+    if (p.weight != nullptr) {
+      float g[8];
+      if (p.weight_dtype == 0) load8<ActBF16, VEC>(p.weight, at, p.width, g);
+      else load8<ActF32, VEC>(p.weight, at, p.width, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * scale * (p.one_centered ? g[j] : 1.0f + g[j]);
+    }
+    if (p.values == nullptr) {
+      store8<A, VEC>(const_cast<uint8_t*>(row_of(p.out, p.out_stride)), at, p.width, h[i]);
+      continue;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(h[i][j]));
+    m = max(m, dpp_u<kDppQuadXor1>(m));
+    m = max(m, dpp_u<kDppQuadXor2>(m));
+    const uint32_t e = mx_scale(m);
+    if (at < p.width) {  // the width is whole groups, so a lane's eight values are all in it
+      const uint64_t first = static_cast<uint64_t>(row) * p.width + at;
+      *reinterpret_cast<uint2*>(p.values + first) =
+          make_uint2(mx_pack4(h[i][0], h[i][1], h[i][2], h[i][3], e), mx_pack4(h[i][4], h[i][5], h[i][6], h[i][7], e));
+      if (t % 4 == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e);
+    }
+  }
+}
+
+template <class A, int TPR, int NV>
+hipError_t norm_go(const NormLaunch& p, hipStream_t stream) {
+  const uint32_t per = kNormThreads / TPR;
+  const dim3 grid((p.rows + per - 1) / per);
+  auto kernel = p.vector ? &k_norm<A, TPR, NV, true> : &k_norm<A, TPR, NV, false>;
+  hipEvent_t start = nullptr, stop = nullptr;
+  if (timing_events("norm", &start, &stop))
+    hipExtLaunchKernelGGL(kernel, grid, dim3(kNormThreads), 0, stream, start, stop, 0, p);
+  else
+    hipLaunchKernelGGL(kernel, grid, dim3(kNormThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+// Rows from which one wave per row fills the chip (256 CUs of four-row blocks).
+constexpr uint32_t kNormWaveRows = 1024;
+
+template <class A>
+hipError_t norm_dispatch(const NormLaunch& p, hipStream_t stream) {
+  const uint32_t steps = (p.width + 511) / 512;  // of one wave
+  if (p.rows >= kNormWaveRows && steps <= 8) {
+    switch (steps) {
+      case 1: return norm_go<A, 64, 1>(p, stream);
+      case 2: return norm_go<A, 64, 2>(p, stream);
+      case 3: return norm_go<A, 64, 3>(p, stream);
+      case 4: return norm_go<A, 64, 4>(p, stream);
+      case 5: return norm_go<A, 64, 5>(p, stream);
+      case 6: return norm_go<A, 64, 6>(p, stream);
+      default: return norm_go<A, 64, 8>(p, stream);
+    }
+  }
+  if (steps <= 4) return norm_go<A, 256, 1>(p, stream);
+  if (steps <= 8) return norm_go<A, 256, 2>(p, stream);
+  if (steps <= 16) return norm_go<A, 256, 4>(p, stream);
+  return norm_go<A, 256, 8>(p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_norm(const NormLaunch& p, hipStream_t stream) {
+  if (p.rows == 0 || p.width == 0 || p.width > kNormMaxWidth) return hipErrorInvalidValue;
+  return p.act_dtype == 0 ? norm_dispatch<ActBF16>(p, stream) : norm_dispatch<ActF32>(p, stream);
+}
+
+}  // namespace vm

@@ -419,4 +419,85 @@ uint64_t hyper_tile_bytes(uint32_t tokens, uint32_t n, uint32_t rows);
 
 hipError_t launch_hyper_mix(const HcLaunch& p, hipStream_t stream);
 
+// ------------------------------------------------------------------ norm --
+constexpr uint32_t kNormMaxWidth = 16384;
+
+// Rows normalised, or only converted to MX (norm.hip).  Strides in elements.
+struct NormLaunch {
+  const void* x;               // [rows, width]
+  const void* residual;        // optional [rows, width]
+  const void* weight;          // [width], or null: no norm
+  void* out;                   // [rows, width] in the input's type (values null)
+  void* sum_out;               // optional [rows, width]: x + residual
+  uint8_t* values;             // MX: [rows, width] e4m3
+  uint8_t* scales;             // MX: [rows, width / 32] e8m0
+  uint64_t x_stride, residual_stride, out_stride, sum_stride;
+  uint32_t rows, width, one_centered;
+  float eps;
+  int act_dtype, weight_dtype;
+  bool vector;                 // every row and the weight 16-byte aligned, width a multiple of 8
+};
+
+hipError_t launch_norm(const NormLaunch& p, hipStream_t stream);
+
+// -------------------------------------------------------------- products --
+// Products of routed rows with their expert's matrix (products.hip).  Routed
+// row i reads x row i / x_div and writes output row i.  Byte strides.
+struct ProductLaunch {
+  const uint8_t* x;            // rows of k_bytes
+  const uint8_t* x_scales;     // MX: k_bytes / 32 bytes per row
+  const uint8_t* w;            // [experts, n (2 n with swiglu)] rows of k_bytes
+  const uint8_t* w_scales;
+  uint64_t x_stride, x_scale_stride, w_stride, w_expert, w_scale_stride, w_scale_expert;
+  const int32_t* ids;          // [rows] expert of every routed row; others' output rows are zeroed
+  const uint32_t* row_off;     // sorted calls: [experts + 1] first sorted row of every expert
+  const uint2* tiles;          // (expert, first row in it)
+  const uint32_t* tile_count;
+  const uint32_t* row_pair;    // routed row of every sorted row
+  uint16_t* out;               // [rows, n] bf16, or
+  uint8_t* values;             // MX [rows, n] and
+  uint8_t* scales;             // [rows, n / 32]
+  uint32_t rows, x_div, k_bytes, n, experts;
+  uint32_t tile_blocks;        // blocks of the grid that serve tiles (set by launch_products)
+  bool mx, swiglu;
+};
+
+// How a call of this many routed rows runs: 0 its rows one by one, or rows per
+// tile (kStreamRows, 64 or 128) after a sort by expert.
+constexpr uint32_t kStreamRows = 16;
+uint32_t product_tile_rows(uint32_t rows, uint32_t experts);
+// An upper bound of a call's blocks.
+uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu);
+hipError_t launch_products(const ProductLaunch& p, uint32_t tile_rows, hipStream_t stream);
+
+// -------------------------------------------------------------- adapters --
+// Low-rank adapters added to a projection's output (adapters.hip).  Strides in
+// elements.
+constexpr uint32_t kAdapterMaxRank = 128;
+constexpr uint32_t kAdapterTile = 16;     // rows per tile of a sorted call
+struct AdapterLaunch {
+  const uint16_t* base;        // [rows, n]
+  const uint16_t* x;           // [rows, k]
+  const uint16_t* a;           // [adapters, rank, k]
+  const uint16_t* b;           // [adapters, n, rank]
+  const float* scales;         // optional [adapters]
+  const int32_t* ids;          // [rows]
+  uint16_t* out;               // [rows, n], may be base
+  uint64_t base_stride, x_stride, out_stride;
+  const uint32_t* row_off;     // tiled calls: [adapters + 1] first sorted row of every adapter
+  const uint2* tiles;          // (adapter, first row in it)
+  const uint32_t* tile_count;
+  const uint32_t* row_pair;    // row of every sorted row
+  uint32_t rows, k, n, rank, adapters;
+  uint32_t splits, split_cols, tile_blocks;  // set by launch_adapters
+  bool vector_k, vector_rank;  // x and A, B: rows of whole aligned 16-byte units
+  bool quads;                  // base and out: rows of whole aligned 8-byte units
+};
+
+// Rows up to which a call runs one block per row and column split, without a sort.
+constexpr uint32_t kAdapterRows = 128;
+// An upper bound of a call's blocks.
+uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled);
+hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream);
+
 }  // namespace vm

@@ -176,6 +176,49 @@ class VmGroupedArgs(ctypes.Structure):
     ]
 
 
+VM_FORMAT_BF16 = 0
+VM_FORMAT_MX = 1
+VM_ACTIVATION_NONE = 0
+VM_ACTIVATION_SWIGLU = 1
+VM_MX_GROUP = 32
+VM_NORM_MAX_WIDTH = 16384
+VM_PRODUCT_MAX_EXPERTS = 1024
+VM_ADAPTER_MAX_RANK = 128
+
+
+class VmNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("weight", _vp), ("out", _vp), ("sum_out", _vp), ("values", _vp),
+        ("scales", _vp),
+        ("x_stride", _c_u64), ("residual_stride", _c_u64), ("out_stride", _c_u64), ("sum_stride", _c_u64),
+        ("rows", _c_u32), ("width", _c_u32), ("act_dtype", _c_u32), ("weight_dtype", _c_u32),
+        ("one_centered", _c_u32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class VmProductArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("x_scales", _vp), ("weight", _vp), ("weight_scales", _vp), ("ids", _vp),
+        ("out", _vp), ("out_values", _vp), ("out_scales", _vp),
+        ("workspace", _vp), ("workspace_bytes", _c_u64),
+        ("x_stride", _c_u64), ("x_scale_stride", _c_u64),
+        ("weight_stride", _c_u64), ("weight_expert_stride", _c_u64),
+        ("weight_scale_stride", _c_u64), ("weight_scale_expert_stride", _c_u64),
+        ("rows", _c_u32), ("x_div", _c_u32), ("k", _c_u32), ("n", _c_u32), ("experts", _c_u32),
+        ("format", _c_u32), ("activation", _c_u32),
+    ]
+
+
+class VmAdapterArgs(ctypes.Structure):
+    _fields_ = [
+        ("base", _vp), ("x", _vp), ("a", _vp), ("b", _vp), ("scales", _vp), ("ids", _vp), ("out", _vp),
+        ("workspace", _vp), ("workspace_bytes", _c_u64),
+        ("base_stride", _c_u64), ("x_stride", _c_u64), ("out_stride", _c_u64),
+        ("rows", _c_u32), ("k", _c_u32), ("n", _c_u32), ("rank", _c_u32), ("adapters", _c_u32),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "vm_abi_version": (ctypes.c_int, []),
@@ -194,6 +237,12 @@ SIGNATURES = {
     "vm_moe_grouped_workspace": (_c_u64, [_c_u32, _c_u32, _c_u32, _c_u32, _c_u32, _c_u32]),
     "vm_moe_grouped": (ctypes.c_int, [ctypes.POINTER(VmGroupedArgs), _vp]),
     "vm_weighted_combine": (ctypes.c_int, [_vp, _vp, _vp, _c_u32, _c_u32, _c_u32, _c_u32, _c_u32, _vp]),
+    "vm_rms_norm": (ctypes.c_int, [ctypes.POINTER(VmNormArgs), _vp]),
+    "vm_mx_quantize": (ctypes.c_int, [_vp, _c_u64, _vp, _vp, _c_u32, _c_u32, _c_u32, _vp]),
+    "vm_grouped_matmul_workspace": (_c_u64, [_c_u32, _c_u32]),
+    "vm_grouped_matmul": (ctypes.c_int, [ctypes.POINTER(VmProductArgs), _vp]),
+    "vm_add_adapters_workspace": (_c_u64, [_c_u32, _c_u32]),
+    "vm_add_adapters": (ctypes.c_int, [ctypes.POINTER(VmAdapterArgs), _vp]),
     "vm_pool_stage": (ctypes.c_int, [_vp, _c_u64, _c_u64, _c_u64, _vp, _c_u64, _c_u64, _c_u64,
                                      ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),
                                      _c_u32, _vp]),
