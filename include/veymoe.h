@@ -389,8 +389,7 @@ typedef struct VmNormArgs {
  * in bf16 or, with swiglu and n a multiple of 32, as MX rows.  An id outside
  * 0..experts-1 gives a row of zeros.
  * k: a multiple of 8 (bf16) or 32 (MX); rows of x and weight 16-byte aligned,
- * `out` 8-byte and `out_values` 4-byte aligned; out, out_values and out_scales
- * contiguous.  experts up to VM_PRODUCT_MAX_EXPERTS.  Strides count elements
+ * `out_values` 8-byte aligned; out, out_values and out_scales contiguous.  experts up to VM_PRODUCT_MAX_EXPERTS.  Strides count elements
  * (of an MX scale array: scales).  The workspace needs no initialisation. */
 #define VM_PRODUCT_MAX_EXPERTS 1024
 typedef struct VmProductArgs {

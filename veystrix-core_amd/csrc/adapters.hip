@@ -6,7 +6,7 @@
 //   k_adapter_rows   a block per row and column split: decode, where every row has an adapter of its own.  Each block
 //                    computes the row's rank sums itself (A_i comes from the L2 for all but the first) rather than
 //                    wait for another launch.
-//   k_adapter_tiles  tiles of 16 rows sorted by adapter: the rank sums by MFMA with k split over the block's four
+//   k_adapter_tiles  tiles of 16 rows sorted by adapter: the rank sums by MFMA with k split over the block's eight
 //                    waves, joined in LDS, then B_i's product strip by strip, added to base.  The rank sums are split
 //                    into a bf16 value and the bf16 rest, two MFMAs, so they lose no more than 2^-16 of themselves;
 //                    the second product is bound by base and out, so this is free.
@@ -14,6 +14,7 @@
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 
+#include "vm_dma.h"
 #include "vm_internal.h"
 
 namespace vm {
@@ -23,10 +24,12 @@ namespace {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = 256;  // of the rows' kernel
 constexpr uint32_t kWaves = kThreads / 64;
 
-__device__ uint4 g_adapter_zeros[8];   // units at and behind the end of a row load from here
+constexpr uint32_t kCopyRows = 4;  // rows checked per wave of the blocks for rows without an adapter
+
+__device__ uint4 g_adapter_zeros[kChunk / 16];  // units at and behind the end of a row load from here
 
 // Eight values of a bf16 row from element `at`, those at `width` and behind it zero.
 template <bool VEC>
@@ -56,7 +59,11 @@ __device__ __forceinline__ void copy_row(const AdapterLaunch& p, uint32_t row, u
   const uint16_t* b = p.base + static_cast<uint64_t>(row) * p.base_stride;
   uint16_t* o = p.out + static_cast<uint64_t>(row) * p.out_stride;
   if (b == o) return;
-  for (uint32_t n = lo + t; n < hi; n += threads) o[n] = b[n];
+  if (p.vector_n) {  // the columns of a split are whole units of eight
+    for (uint32_t n = lo + 8 * t; n < hi; n += 8 * threads) *reinterpret_cast<uint4*>(o + n) = ldg16(b + n);
+  } else {
+    for (uint32_t n = lo + t; n < hi; n += threads) o[n] = b[n];
+  }
 }
 
 // ------------------------------------------------------------------ rows ---
@@ -114,26 +121,115 @@ __global__ __launch_bounds__(kThreads) void k_adapter_rows(AdapterLaunch p) {
 
 // ----------------------------------------------------------------- tiles ---
 
+constexpr uint32_t kTileWaves = 4;
+constexpr uint32_t kTileThreads = kTileWaves * 64;
+constexpr uint32_t kTileCols = 64;   // columns of a wave's strip
+
 __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t acc) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc,
                                                  0, 0, 0);
 }
 
-// RF 16-row fragments of A (rank up to 16 RF).
-template <int RF, bool VEC_K, bool VEC_R>
-__global__ __launch_bounds__(kThreads) void k_adapter_tiles(AdapterLaunch p) {
-  constexpr uint32_t kRankPad = (RF + 1) / 2 * 32;          // rank in whole MFMA steps
-  constexpr uint32_t kPitch = kRankPad * 2 + 16;            // bytes of a row of rank sums in LDS
-  constexpr int kDepth = 2;
-  __shared__ f32x4_t s_part[kWaves][RF][64];
-  __shared__ uint4 s_v[2][kAdapterTile * kPitch / 16];      // the rank sums' bf16 values and rests
+// Stage J of every wave's own ring: first 16 rows of x and 16 RF rows of A, 128 bytes each, then strips of B (at most
+// 2 RF KB).
+template <int RF>
+constexpr uint32_t stage_bytes() {
+  return (kAdapterTile + 16 * RF) * kChunk;
+}
+// Byte `at` of it; whole offsets in one step, past a few of which the compiler no longer tells the stages apart and
+// waits for every load in flight before it reads one.
+template <int J, int RF>
+__device__ __forceinline__ uint8_t* wave_stage(uint32_t at) {
+  __shared__ uint4 buf[kTileWaves * stage_bytes<RF>() / 16];
+  return reinterpret_cast<uint8_t*>(buf) + at;
+}
+
+// Rank sums of the tile, this wave's chunks w, w + 4, .. of 64 inputs.  Operands by DMA, a chunk ahead.
+template <int RF>
+__device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t id, uint32_t first_row, uint32_t rows,
+                                              uint32_t wave, uint32_t lane, f32x4_t acc[RF]) {
+  constexpr int kLoads = (kAdapterTile + 16 * RF) / 8;
+  const uint32_t lm = lane & 15u, kb = lane >> 4, sub = lane / 8u, mine = wave * stage_bytes<RF>();
+  const uint8_t* src[kLoads];
+  const uint32_t unit = ((lane % 8u) ^ tile_swz(sub)) * 16u;   // byte of the lane's unit in a chunk of rows sub, 8 + sub, ..
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const uint32_t r = i * 8u + sub;
+    if (i < 2) {
+      const uint32_t row = p.row_pair[first_row + min(r, rows - 1)];
+      src[i] = reinterpret_cast<const uint8_t*>(p.x + static_cast<uint64_t>(row) * p.x_stride) + unit;
+    } else {
+      const uint32_t j = min(r - kAdapterTile, p.rank - 1);
+      src[i] = reinterpret_cast<const uint8_t*>(p.a + (static_cast<uint64_t>(id) * p.rank + j) * p.k) + unit;
+    }
+  }
+  const uint32_t k_bytes = p.k * 2, chunks = (k_bytes + kChunk - 1) / kChunk;
+  auto issue = [&](auto J, uint32_t c) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      load_to_lds(c * kChunk + unit < k_bytes ? src[i] + c * kChunk : reinterpret_cast<const uint8_t*>(g_adapter_zeros),
+                  wave_stage<decltype(J)::value, RF>(mine + i * 1024u));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const uint32_t s = tile_swz(lm);
+  const uint32_t u[2] = {mine + lm * kChunk + (kb ^ s) * 16u, mine + lm * kChunk + ((4u | kb) ^ s) * 16u};
+  // a wave without a chunk, and the steps behind a wave's last one, load zeros: every step issues the same loads
+  using J0 = std::integral_constant<int, 0>;
+  issue(J0{}, wave);
+  for (uint32_t c = wave; c < chunks; c += 2 * kTileWaves) {
+    unroll<0, 2>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      issue(std::integral_constant<int, 1 - j>{}, c + (j + 1) * kTileWaves);
+      wait_vm<kLoads>();   // this step's loads have landed; the next one's are in flight
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 x = *reinterpret_cast<const uint4*>(wave_stage<j, RF>(u[h]));
+#pragma unroll
+        for (uint32_t f = 0; f < RF; ++f)
+          acc[f] = mfma(*reinterpret_cast<const uint4*>(wave_stage<j, RF>(u[h] + (f + 1) * 16 * kChunk)), x, acc[f]);
+      }
+      wait_lgkm0();        // the stage has been read before it is filled again
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+  wait_vm<0>();
+}
+
+// The same with every lane fetching its own operands: rows off the 16-byte units.
+template <int RF>
+__device__ __forceinline__ void rank_sums_direct(const AdapterLaunch& p, uint32_t id, uint32_t first_row, uint32_t rows,
+                                                 uint32_t wave, uint32_t lane, f32x4_t acc[RF]) {
+  const uint32_t lm = lane & 15u, kb = lane >> 4;
+  const uint16_t* x = p.x + static_cast<uint64_t>(p.row_pair[first_row + min(lm, rows - 1)]) * p.x_stride;
+  for (uint32_t c = wave * 64u; c < p.k; c += kTileWaves * 64u) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t at = c + 32u * h + kb * 8u;
+      const uint4 xv = unit_of<false>(x, at, p.k);
+#pragma unroll
+      for (int f = 0; f < RF; ++f) {
+        const uint32_t j = min(f * 16u + lm, p.rank - 1);
+        acc[f] = mfma(unit_of<false>(p.a + (static_cast<uint64_t>(id) * p.rank + j) * p.k, at, p.k), xv, acc[f]);
+      }
+    }
+  }
+}
+
+// RF 16-row fragments of A (rank up to 16 RF).  VEC_K: x and A, and VEC_R: B move as 16-byte units; VEC_N: base and out.
+template <int RF, bool VEC_K, bool VEC_R, bool VEC_N>
+__global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p) {
+  constexpr int kSteps = (RF + 1) / 2;                      // MFMA steps over the rank
+  constexpr uint32_t kPitch = kSteps * 64 + 16;             // bytes of a row of rank sums in LDS
+  // first the rank sums' bf16 values and rests, then every wave's 16 x 64 products in fp32
+  __shared__ uint4 s_y[kTileWaves * 16 * 64 * 4 / 16];
+  static_assert(2 * kAdapterTile * kPitch <= sizeof(s_y), "the rank sums fit");
   const uint32_t tid = threadIdx.x, lane = tid & 63u, lm = lane & 15u, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lin = blockIdx.x;
   if (lin >= p.tile_blocks) {  // rows without an adapter
-    const uint32_t first = ((lin - p.tile_blocks) * kWaves + wave) * 64u;
+    const uint32_t first = ((lin - p.tile_blocks) * kTileWaves + wave) * kCopyRows;
     const uint32_t i = first + lane;
-    uint64_t left = __ballot(i < p.rows && static_cast<uint32_t>(p.ids[i]) >= p.adapters);
+    uint64_t left = __ballot(lane < kCopyRows && i < p.rows && static_cast<uint32_t>(p.ids[i]) >= p.adapters);
     while (left != 0) {
       const uint32_t j = static_cast<uint32_t>(__builtin_ctzll(left));
       left &= left - 1;
@@ -146,58 +242,77 @@ __global__ __launch_bounds__(kThreads) void k_adapter_tiles(AdapterLaunch p) {
   const uint32_t count = *p.tile_count, run = (count + 7) / 8;
   const uint32_t tile = (lin & 7u) * run + local;
   if (local >= run || tile >= count) return;
-  const uint2 td = p.tiles[tile];
-  const uint32_t id = td.x, row0 = p.row_off[id] + td.y;
-  const uint32_t rows = min(p.row_off[id + 1] - row0, kAdapterTile);
-  const uint32_t row = p.row_pair[row0 + min(lm, rows - 1)];
-  const uint16_t* x = p.x + static_cast<uint64_t>(row) * p.x_stride;
-  const uint16_t* a_row[RF];
-#pragma unroll
-  for (int f = 0; f < RF; ++f)
-    a_row[f] = p.a + (static_cast<uint64_t>(id) * p.rank + min(f * 16u + lm, p.rank - 1)) * p.k;
+  const RowTile td = p.tiles[tile];
+  const uint32_t id = td.group, rows = td.rows;
+  const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
 
-  // rank sums: wave w takes the chunks w, w + 4, .. of 64 inputs; those behind the last one load zeros
-  const uint32_t chunks = (p.k + 63) / 64;
-  const uint32_t mine = chunks > wave ? (chunks - wave + kWaves - 1) / kWaves : 0u;
-  struct Chunk {
-    uint4 a[RF][2], x[2];
-  } buf[kDepth];
-  auto load = [&](Chunk& c, uint32_t i) {
-    const uint32_t at = (wave + i * kWaves) * 64u + kb * 8u;
-#pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-      c.x[h] = unit_of<VEC_K>(x, at + 32u * h, p.k);
-#pragma unroll
-      for (int f = 0; f < RF; ++f) c.a[f][h] = unit_of<VEC_K>(a_row[f], at + 32u * h, p.k);
-    }
-  };
   f32x4_t acc[RF];
 #pragma unroll
   for (int f = 0; f < RF; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (VEC_K) rank_sums_dma<RF>(p, id, td.row, rows, wave, lane, acc);
+  else rank_sums_direct<RF>(p, id, td.row, rows, wave, lane, acc);
+
+  // Strips of 64 columns.  B's rows of a strip lie side by side: one copy of 64 rank values to LDS, whose units are
+  // swizzled within their rows where a row is a power of two of them; base goes to registers as the rows' own units,
+  // lane j holding unit j % 8 of row j / 8 (and of row 8 + j / 8).  Both are fetched a strip ahead.
+  const uint32_t first = split * p.split_cols, end = min(first + p.split_cols, p.n);
+  const uint8_t* b = reinterpret_cast<const uint8_t*>(p.b + static_cast<uint64_t>(id) * p.n * p.rank);
+  const uint32_t units = p.rank / 8, b_units = p.n * units;   // of a row, of the matrix (VEC_R)
+  const uint32_t mask = (units & (units - 1)) == 0 ? units - 1 : 0u, shift = mask == 0 ? 0u : 4u - __builtin_ctz(units);
+  constexpr int kB = 2 * RF;
+  uint32_t b_unit[kB];   // unit of the strip that the lane copies with load i
+  if constexpr (VEC_R) {
 #pragma unroll
-  for (int j = 0; j < kDepth; ++j) load(buf[j], j);
-  for (uint32_t i = 0; i < mine; i += kDepth) {
-#pragma unroll
-    for (int j = 0; j < kDepth; ++j) {
-#pragma unroll
-      for (int f = 0; f < RF; ++f) {
-        acc[f] = mfma(buf[j].a[f][0], buf[j].x[0], acc[f]);
-        acc[f] = mfma(buf[j].a[f][1], buf[j].x[1], acc[f]);
-      }
-      load(buf[j], i + j + kDepth);
+    for (uint32_t i = 0; i < kB; ++i) {
+      const uint32_t v = i * 64u + lane, r = v / units;
+      b_unit[i] = r * units + ((v - r * units) ^ ((r >> shift) & mask));
     }
   }
+  auto copy_b = [&](auto J, uint32_t col) {
+    if constexpr (VEC_R) {
 #pragma unroll
-  for (int f = 0; f < RF; ++f) s_part[wave][f][lane] = acc[f];
-  __syncthreads();
+      for (uint32_t i = 0; i < kB; ++i)
+        load_to_lds(b + static_cast<uint64_t>(min(col * units + b_unit[i], b_units - 1)) * 16u,
+                    wave_stage<decltype(J)::value, RF>(wave * stage_bytes<RF>() + i * 1024u));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  uint64_t base_at[2], out_at[2];
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h) {
+    const uint32_t row = p.row_pair[td.row + min(lane / 8u + 8u * h, rows - 1)];
+    base_at[h] = static_cast<uint64_t>(row) * p.base_stride;
+    out_at[h] = static_cast<uint64_t>(row) * p.out_stride;
+  }
+  const uint32_t sub = 8u * (lane & 7u);
+  uint4 base[2][2];
+  auto load_base = [&](int j, uint32_t col) {
+    if constexpr (VEC_N) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) base[j][h] = unit_of<true>(p.base + base_at[h], col + sub, p.n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // the waves' rank sums join: in stage 0, which is free
+  f32x4_t* part = reinterpret_cast<f32x4_t*>(wave_stage<0, RF>(0));
+  constexpr uint32_t kWavePart = stage_bytes<RF>() / 16;
+  static_assert(RF * 1024 <= stage_bytes<RF>(), "the partial sums fit");
+#pragma unroll
+  for (int f = 0; f < RF; ++f) part[wave * kWavePart + f * 64 + lane] = acc[f];
+  uint32_t col = first + wave * kTileCols;
+  load_base(0, col);
+  lds_barrier();
   // lane holds rank sums 16 f + 4 kb .. +3 of its row; ranks at and behind `rank` are zero
-  const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
-  uint8_t* v_hi = reinterpret_cast<uint8_t*>(s_v[0]);
-  uint8_t* v_lo = reinterpret_cast<uint8_t*>(s_v[1]);
-  for (uint32_t f = wave; f < kRankPad / 16; f += kWaves) {
+  uint8_t* v_hi = reinterpret_cast<uint8_t*>(s_y);
+  uint8_t* v_lo = v_hi + kAdapterTile * kPitch;
+  for (uint32_t f = wave; f < kSteps * 2; f += kTileWaves) {
     uint32_t hi[4], lo[4];
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (f < RF) v = s_part[0][f][lane] + s_part[1][f][lane] + s_part[2][f][lane] + s_part[3][f][lane];
+    if (f < RF) {
+#pragma unroll
+      for (uint32_t w = 0; w < kTileWaves; ++w) v += part[w * kWavePart + f * 64 + lane];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float r = f * 16u + kb * 4u + i < p.rank ? v[i] * scale : 0.0f;
@@ -209,94 +324,143 @@ __global__ __launch_bounds__(kThreads) void k_adapter_tiles(AdapterLaunch p) {
     *reinterpret_cast<uint2*>(v_hi + at) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
     *reinterpret_cast<uint2*>(v_lo + at) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
   }
-  __syncthreads();
-  constexpr int kSteps = kRankPad / 32;
+  lds_barrier();
+  copy_b(std::integral_constant<int, 0>{}, col);
   uint4 hi[kSteps], lo[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     hi[s] = *reinterpret_cast<const uint4*>(v_hi + lm * kPitch + s * 64 + kb * 16);
     lo[s] = *reinterpret_cast<const uint4*>(v_lo + lm * kPitch + s * 64 + kb * 16);
   }
+  lds_barrier();  // the rank sums have been read before the products take their place
+  float* y_wave = reinterpret_cast<float*>(s_y) + wave * 16 * 64;
 
-  const uint32_t first = split * p.split_cols, end = min(first + p.split_cols, p.n);
-  const uint16_t* b = p.b + static_cast<uint64_t>(id) * p.n * p.rank;
-  const uint16_t* base = p.base + static_cast<uint64_t>(row) * p.base_stride;
-  uint16_t* out = p.out + static_cast<uint64_t>(row) * p.out_stride;
-  for (uint32_t col = first + wave * 64u; col < end; col += kWaves * 64u) {
+  auto strip = [&](auto J) {
+    constexpr int j = decltype(J)::value;
+    const uint32_t next = col + kTileWaves * kTileCols;
+    copy_b(std::integral_constant<int, 1 - j>{}, min(next, p.n - 1));
+    load_base(1 - j, next);
     f32x4_t y[4];
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      y[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      const uint16_t* b_row = b + static_cast<uint64_t>(min(col + f * 16u + lm, p.n - 1)) * p.rank;
+    for (int f = 0; f < 4; ++f) y[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    // this strip's copies have landed: behind them only the next strip's and the stores of the one before
+    if constexpr (VEC_R) wait_vm<kB + (VEC_N ? 2 : 0)>();
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint4 w = unit_of<VEC_R>(b_row, s * 32u + kb * 8u, p.rank);
+    for (uint32_t f = 0; f < 4; ++f) {
+      const uint32_t r = 16u * f + lm;
+#pragma unroll
+      for (uint32_t s = 0; s < kSteps; ++s) {
+        const uint32_t unit = s * 4u + kb;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if constexpr (VEC_R) {
+          if (unit < units) w = *reinterpret_cast<const uint4*>(
+                wave_stage<j, RF>(wave * stage_bytes<RF>() + (r * units + (unit ^ ((r >> shift) & mask))) * 16u));
+        } else {
+          const uint16_t* row = p.b + (static_cast<uint64_t>(id) * p.n + min(col + r, p.n - 1)) * p.rank;
+          w = unit_of<false>(row, unit * 8u, p.rank);
+        }
         y[f] = mfma(w, hi[s], y[f]);
         y[f] = mfma(w, lo[s], y[f]);
       }
     }
-    if (lm >= rows) continue;
+    // lane holds columns 16 f + 4 kb .. +3 of row lm: unit 4 f + kb of 16, stored at that ^ lm
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      const uint32_t at = col + f * 16u + kb * 4u;
-      if (p.quads) {
-        if (at >= p.n) continue;
-        const uint2 v = *reinterpret_cast<const uint2*>(base + at);
-        const float o[4] = {__uint_as_float(v.x << 16) + y[f][0], __uint_as_float(v.x & 0xffff0000u) + y[f][1],
-                            __uint_as_float(v.y << 16) + y[f][2], __uint_as_float(v.y & 0xffff0000u) + y[f][3]};
-        *reinterpret_cast<uint2*>(out + at) =
-            make_uint2(f32_to_bf16(o[0]) | (f32_to_bf16(o[1]) << 16), f32_to_bf16(o[2]) | (f32_to_bf16(o[3]) << 16));
-      } else {
+    for (uint32_t f = 0; f < 4; ++f)
+      *reinterpret_cast<f32x4_t*>(y_wave + lm * 64u + ((4u * f + kb) ^ lm) * 4u) = y[f];
+    wait_lgkm0();  // the wave's own stores, in order
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t r = lane / 8u + 8u * h;
+      float o[8];
+#pragma unroll
+      for (uint32_t q = 0; q < 2; ++q) {
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(y_wave + r * 64u + ((2u * (lane & 7u) + q) ^ r) * 4u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[4 * q + i] = v[i];
+      }
+      if (r >= rows) continue;
+      const uint32_t at = col + sub;
+      if constexpr (VEC_N) {
+        const uint32_t v[4] = {base[j][h].x, base[j][h].y, base[j][h].z, base[j][h].w};
+        uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (at + i < p.n) out[at + i] = static_cast<uint16_t>(f32_to_bf16(bf16_to_f32(base[at + i]) + y[f][i]));
+          w[i] = f32_to_bf16(__uint_as_float(v[i] << 16) + o[2 * i]) |
+                 (f32_to_bf16(__uint_as_float(v[i] & 0xffff0000u) + o[2 * i + 1]) << 16);
+        if (at < p.n) *reinterpret_cast<uint4*>(p.out + out_at[h] + at) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (at + i < p.n)
+            p.out[out_at[h] + at + i] = static_cast<uint16_t>(f32_to_bf16(bf16_to_f32(p.base[base_at[h] + at + i]) + o[i]));
       }
     }
+    wait_lgkm0();  // stage and products have been read before they are written again
+    __builtin_amdgcn_sched_barrier(0);
+    col = next;
+  };
+  while (col < end) {
+    strip(std::integral_constant<int, 0>{});
+    if (col >= end) break;
+    strip(std::integral_constant<int, 1>{});
   }
+  wait_vm<0>();  // no load into LDS outlives the block
 }
 
 template <class Kernel>
-hipError_t go(Kernel kernel, uint32_t blocks, const AdapterLaunch& p, hipStream_t stream) {
+hipError_t go(Kernel kernel, uint32_t blocks, uint32_t threads, const AdapterLaunch& p, hipStream_t stream) {
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("adapters", &start, &stop))
-    hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, stream, start, stop, 0, p);
+    hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, start, stop, 0, p);
   else
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, p);
   return hipGetLastError();
 }
 
+// Operands off the vector units share one instance per rank.
 template <int RF>
 hipError_t tiles_go(const AdapterLaunch& p, uint32_t blocks, hipStream_t stream) {
-  if (p.vector_k && p.vector_rank) return go(&k_adapter_tiles<RF, true, true>, blocks, p, stream);
-  if (p.vector_k) return go(&k_adapter_tiles<RF, true, false>, blocks, p, stream);
-  return go(&k_adapter_tiles<RF, false, false>, blocks, p, stream);
+  if (p.vector_k && p.vector_rank)
+    return p.vector_n ? go(&k_adapter_tiles<RF, true, true, true>, blocks, kTileThreads, p, stream)
+                      : go(&k_adapter_tiles<RF, true, true, false>, blocks, kTileThreads, p, stream);
+  if (p.vector_k)
+    return p.vector_n ? go(&k_adapter_tiles<RF, true, false, true>, blocks, kTileThreads, p, stream)
+                      : go(&k_adapter_tiles<RF, true, false, false>, blocks, kTileThreads, p, stream);
+  return go(&k_adapter_tiles<RF, false, false, false>, blocks, kTileThreads, p, stream);
+}
+
+// Columns per block: all of them once the units (rows or tiles) fill the chip twice, at least `least` and whole strips
+// of a block.
+uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least) {
+  const uint32_t parts = (n + least - 1) / least;
+  const uint32_t want = units >= 512 ? 1u : min(parts, (512 + units - 1) / units);
+  return (parts + want - 1) / want * least;
 }
 
 }  // namespace
 
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled) {
-  const uint64_t passes = (uint64_t(n) + kThreads - 1) / kThreads;
-  const uint64_t units = tiled ? (uint64_t(rows) + kAdapterTile - 1) / kAdapterTile + adapters + 7 : rows;
-  return (units >= 512 ? units : units * passes) + rows / (64 * kWaves) + 1;
+  const uint64_t parts = (uint64_t(n) + kThreads - 1) / kThreads;
+  const uint64_t units = tiled ? uint64_t(rows) / kAdapterTile + adapters + 7 : rows;
+  return (units >= 512 ? units : units * parts) + rows / (kCopyRows * kTileWaves) + 1;
 }
 
 hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
   if (p.rows == 0 || p.rank == 0 || p.rank > kAdapterMaxRank) return hipErrorInvalidValue;
   if (!p.vector_k) p.vector_rank = false;
-  const uint32_t units = tiled ? grouped_max_tiles(p.rows, p.adapters, kAdapterTile) : p.rows;
-  // columns per block: all of them once the rows fill the chip twice, at least one pass of the block
-  const uint32_t passes = (p.n + kThreads - 1) / kThreads;
-  const uint32_t want = units >= 512 ? 1u : min(passes, (512 + units - 1) / units);
-  p.split_cols = (passes + want - 1) / want * kThreads;
-  p.splits = (p.n + p.split_cols - 1) / p.split_cols;
   if (!tiled) {
+    p.split_cols = split_columns(p.n, p.rows, kThreads);
+    p.splits = (p.n + p.split_cols - 1) / p.split_cols;
     const uint32_t blocks = p.rows * p.splits;
-    if (p.vector_k && p.vector_rank) return go(&k_adapter_rows<true, true>, blocks, p, stream);
-    if (p.vector_k) return go(&k_adapter_rows<true, false>, blocks, p, stream);
-    return go(&k_adapter_rows<false, false>, blocks, p, stream);
+    if (p.vector_k && p.vector_rank) return go(&k_adapter_rows<true, true>, blocks, kThreads, p, stream);
+    if (p.vector_k) return go(&k_adapter_rows<true, false>, blocks, kThreads, p, stream);
+    return go(&k_adapter_rows<false, false>, blocks, kThreads, p, stream);
   }
+  const uint32_t units = row_max_tiles(p.rows, p.adapters, kAdapterTile);
+  p.split_cols = split_columns(p.n, units, kTileWaves * kTileCols);
+  p.splits = (p.n + p.split_cols - 1) / p.split_cols;
   p.tile_blocks = (units + 7) / 8 * 8 * p.splits;
-  const uint32_t blocks = p.tile_blocks + (p.rows + 64 * kWaves - 1) / (64 * kWaves);
+  const uint32_t blocks = p.tile_blocks + (p.rows + kCopyRows * kTileWaves - 1) / (kCopyRows * kTileWaves);
   if (p.rank <= 16) return tiles_go<1>(p, blocks, stream);
   if (p.rank <= 32) return tiles_go<2>(p, blocks, stream);
   if (p.rank <= 64) return tiles_go<4>(p, blocks, stream);

@@ -1582,7 +1582,7 @@ int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* s
 // Workspace of a sort of `rows` ids into `groups` groups, laid out for tiles
 // of `tile_rows` rows.
 struct RowSortWs {
-  uint64_t row_off, tiles, tiles_dn, tile_count, counts, row_token, row_pair, total;
+  uint64_t tiles, tile_count, block_counts, row_pair, total;
 };
 
 static RowSortWs row_sort_ws(uint32_t rows, uint32_t groups, uint32_t tile_rows) {
@@ -1593,37 +1593,27 @@ static RowSortWs row_sort_ws(uint32_t rows, uint32_t groups, uint32_t tile_rows)
     at += align_up(bytes);
     return r;
   };
-  const uint64_t tiles = uint64_t(vm::grouped_max_tiles(rows, groups, tile_rows)) * sizeof(uint2);
-  w.row_off = take((uint64_t(groups) + 1) * 4);
-  w.tile_count = take(2 * 4);
-  w.counts = take(2 * 1024 * 4);
-  w.tiles = take(tiles);
-  w.tiles_dn = take(tiles);
-  w.row_token = take(uint64_t(rows) * 4);
+  w.tiles = take(uint64_t(vm::row_max_tiles(rows, groups, tile_rows)) * sizeof(vm::RowTile));
+  w.tile_count = take(4);
+  w.block_counts = take(rows <= vm::kOneLaunchRows ? 0 : uint64_t(vm::row_sort_blocks(rows)) * groups * 4);
   w.row_pair = take(uint64_t(rows) * 4);
   w.total = at;
   return w;
 }
 
+// Sorts into the workspace; the lists are in `s` afterwards.
 static hipError_t sort_rows(const int32_t* ids, uint32_t rows, uint32_t groups, uint32_t tile_rows, const RowSortWs& w,
-                            char* ws, hipStream_t stream) {
-  vm::SortLaunch s{};
-  s.inds = ids;
-  s.row_off = reinterpret_cast<uint32_t*>(ws + w.row_off);
-  s.tiles = reinterpret_cast<uint2*>(ws + w.tiles);
-  s.tiles_dn = reinterpret_cast<uint2*>(ws + w.tiles_dn);
+                            void* workspace, hipStream_t stream, vm::RowSortLaunch& s) {
+  char* ws = static_cast<char*>(workspace);
+  s.ids = ids;
+  s.tiles = reinterpret_cast<vm::RowTile*>(ws + w.tiles);
   s.tile_count = reinterpret_cast<uint32_t*>(ws + w.tile_count);
-  s.tile_count_dn = s.tile_count + 1;
-  s.counts = reinterpret_cast<uint32_t*>(ws + w.counts);
-  s.cursors = s.counts + 1024;
-  s.row_token = reinterpret_cast<uint32_t*>(ws + w.row_token);
-  s.pair_row = reinterpret_cast<uint32_t*>(ws + w.row_pair);
-  s.tokens = rows;
-  s.slots = 1;
-  s.experts = groups;
-  s.tile_rows = s.tile_rows_dn = tile_rows;
-  s.by_row = true;
-  return vm::launch_sort(s, stream);
+  s.block_counts = reinterpret_cast<uint32_t*>(ws + w.block_counts);
+  s.row_pair = reinterpret_cast<uint32_t*>(ws + w.row_pair);
+  s.rows = rows;
+  s.groups = groups;
+  s.tile_rows = tile_rows;
+  return vm::launch_row_sort(s, stream);
 }
 
 // ----------------------------------------------------- grouped products ---
@@ -1657,8 +1647,6 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
     if (!swiglu) return fail(VM_EUNSUPPORTED, "MX output is written by the swiglu activation");
     const int rc = check_mx_rows(a->out_values, a->out_scales, a->n);
     if (rc != VM_OK) return rc;
-  } else if (reinterpret_cast<uintptr_t>(a->out) % 8) {
-    return fail(VM_EINVAL, "out must be 8-byte aligned");
   }
   if (!rows_aligned(a->x, a->x_stride * size, 16) || !rows_aligned(a->weight, a->weight_stride * size, 16) ||
       a->weight_expert_stride * size % 16)
@@ -1671,13 +1659,12 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
     const RowSortWs w = row_sort_ws(a->rows, a->experts, tile);
     if (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace))
       return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
-    char* ws = static_cast<char*>(a->workspace);
-    const hipError_t e = sort_rows(a->ids, a->rows, a->experts, tile, w, ws, stream);
+    vm::RowSortLaunch s{};
+    const hipError_t e = sort_rows(a->ids, a->rows, a->experts, tile, w, a->workspace, stream, s);
     if (e != hipSuccess) return hip_fail(e, "sort launch");
-    p.row_off = reinterpret_cast<const uint32_t*>(ws + w.row_off);
-    p.tiles = reinterpret_cast<const uint2*>(ws + w.tiles);
-    p.tile_count = reinterpret_cast<const uint32_t*>(ws + w.tile_count);
-    p.row_pair = reinterpret_cast<const uint32_t*>(ws + w.row_pair);
+    p.tiles = s.tiles;
+    p.tile_count = s.tile_count;
+    p.row_pair = s.row_pair;
   }
   p.x = static_cast<const uint8_t*>(a->x);
   p.x_scales = a->x_scales;
@@ -1700,6 +1687,7 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   p.experts = a->experts;
   p.mx = mx;
   p.swiglu = swiglu;
+  p.out_aligned = aligned16(a->out);
   const hipError_t e = vm::launch_products(p, tile, stream);
   if (e != hipSuccess) return hip_fail(e, "products launch");
   return VM_OK;
@@ -1745,20 +1733,19 @@ int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
   p.adapters = a->adapters;
   p.vector_k = a->k % 8 == 0 && rows_aligned(a->x, a->x_stride * 2, 16) && aligned16(a->a);
   p.vector_rank = a->rank % 8 == 0 && aligned16(a->b);
-  p.quads = a->n % 4 == 0 && rows_aligned(a->base, a->base_stride * 2, 8) && rows_aligned(a->out, a->out_stride * 2, 8);
+  p.vector_n = a->n % 8 == 0 && rows_aligned(a->base, a->base_stride * 2, 16) && rows_aligned(a->out, a->out_stride * 2, 16);
   if (vm::adapter_blocks(a->rows, a->adapters, a->n, tiled) > kMaxBlocks)
     return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
   if (tiled) {
     const RowSortWs w = row_sort_ws(a->rows, a->adapters, vm::kAdapterTile);
     if (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace))
       return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
-    char* ws = static_cast<char*>(a->workspace);
-    const hipError_t e = sort_rows(a->ids, a->rows, a->adapters, vm::kAdapterTile, w, ws, stream);
+    vm::RowSortLaunch s{};
+    const hipError_t e = sort_rows(a->ids, a->rows, a->adapters, vm::kAdapterTile, w, a->workspace, stream, s);
     if (e != hipSuccess) return hip_fail(e, "sort launch");
-    p.row_off = reinterpret_cast<const uint32_t*>(ws + w.row_off);
-    p.tiles = reinterpret_cast<const uint2*>(ws + w.tiles);
-    p.tile_count = reinterpret_cast<const uint32_t*>(ws + w.tile_count);
-    p.row_pair = reinterpret_cast<const uint32_t*>(ws + w.row_pair);
+    p.tiles = s.tiles;
+    p.tile_count = s.tile_count;
+    p.row_pair = s.row_pair;
   }
   const hipError_t e = vm::launch_adapters(p, tiled, stream);
   if (e != hipSuccess) return hip_fail(e, "adapters launch");

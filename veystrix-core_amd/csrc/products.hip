@@ -9,15 +9,14 @@
 // cancelled terms survive to 2^-24 of the largest).  The scaled 8-bit MFMA, at twice the rate, lost those below 2^-16
 // of its group's largest product and put 2e-5 of the terms' magnitude on a sum (measured), which an MX output shows as
 // flipped values; these products read hundreds of matrices for a few rows each and wait for HBM, not for the MFMA.
-// The matrix is the first operand, the rows the second, so a lane receives outputs 4 kb .. +3 of row lane % 16: four
-// neighbouring outputs to store.
+// The matrix is the first operand, the rows the second, so a lane receives outputs of row lane % 16.
 //
-// With hundreds of experts the weights are most of the bytes, each read for a few to a few hundred rows.  Three forms:
-//   k_stream, rows one by one   calls of few routed rows: no sort, one launch; a block per routed row and 64 matrix
-//                               rows, the matrix streamed from HBM into the operand registers.
-//   k_stream, tiles of 16       few rows per expert: the same over rows sorted by expert, so each matrix is read once
-//                               per 16 rows.
-//   k_tiles                     tiles of 64 or 128 sorted rows by 128 matrix rows, both staged through LDS by DMA.
+// With hundreds of experts the weights are most of the bytes, each read for a few to a few hundred rows.  Two forms:
+//   k_rows    calls of few routed rows: no sort, one launch; a block per routed row and a few dozen matrix rows, each
+//             read a kilobyte at a time by one wave and multiplied by v_dot2.
+//   k_tiles   tiles of up to 32 or 64 rows sorted by expert by 128 or 256 matrix rows, both staged in LDS by DMA.
+// MFMA operands loaded straight from memory (16 rows of 64 bytes per load) are limited to 16 bytes per clock and CU,
+// the L1's rate for lanes of different rows; the DMA's eight rows of 128 bytes reach 55 (measured).
 // Rows whose id names no expert are written as zeros by blocks behind the tiles'.
 
 #include <hip/hip_ext.h>
@@ -25,9 +24,19 @@
 
 #include <type_traits>
 
+#include "vm_dma.h"
 #include "vm_internal.h"
 #include "vm_mx.h"
 
+#ifndef VM_ROWS
+#define VM_ROWS 160
+#endif
+#ifndef VM_MEAN
+#define VM_MEAN 16
+#endif
+#ifndef VM_WIDEK
+#define VM_WIDEK 20
+#endif
 namespace vm {
 
 namespace {
@@ -35,9 +44,8 @@ namespace {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kChunk = 128;          // bytes of a row per step
 constexpr int kStrip = 4;                 // 16-row fragments of the matrix per wave
-constexpr uint32_t kZeroRows = 64;        // routed rows checked per wave of the zeroing blocks
+constexpr uint32_t kZeroRows = 8;         // routed rows checked per wave of the zeroing blocks
 
 enum : int { kOutBf16 = 0, kOutMx = 1 };
 
@@ -91,12 +99,14 @@ __device__ __forceinline__ uint32_t chunk_scales(const uint8_t* row, uint32_t c,
   return v;
 }
 
-// Matrix row behind row `r` (0..63) of a wave's strip that starts at output column `col`: with SwiGLU fragments
-// alternate between 16 gate rows and the 16 up rows of the same outputs.
+// Matrix row behind row `r` (0..63) of a wave's strip that starts at output column `col`.  Row 4 q + i of fragment f
+// becomes output i of lane group q, so the fragments are dealt to give a lane neighbouring outputs over all of them:
+// 16 of the strip's 64, or with SwiGLU 8 of its 32, where fragments alternate between gate rows and up rows.
 template <bool SWIGLU>
 __device__ __forceinline__ uint32_t matrix_row(uint32_t col, uint32_t r, uint32_t n) {
-  if constexpr (SWIGLU) return min(col + (r >> 5) * 16u + (r & 15u), n - 1u) + ((r >> 4) & 1u) * n;
-  else return min(col + r, n - 1u);
+  const uint32_t f = r >> 4, q = (r >> 2) & 3u, i = r & 3u;
+  if constexpr (SWIGLU) return min(col + 8u * q + 4u * (f >> 1) + i, n - 1u) + (f & 1u) * n;
+  else return min(col + 16u * q + 4u * f + i, n - 1u);
 }
 
 // Outputs per strip.
@@ -111,47 +121,43 @@ __device__ __forceinline__ float swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f)) * u;
 }
 
-// Stores one strip of one 16-row fragment: lane holds outputs 4 kb .. +3 of each fragment for its routed row.
+// Stores one strip of one 16-row fragment: a lane holds 16 (SwiGLU: 8) neighbouring outputs of its routed row.
 template <bool SWIGLU, int OUT>
 __device__ __forceinline__ void store_strip(const ProductLaunch& p, const f32x4_t acc[kStrip], uint32_t col,
                                             uint32_t pair, bool live, uint32_t kb) {
-  constexpr int kFrags = SWIGLU ? kStrip / 2 : kStrip;
-  float y[kFrags][4];
+  constexpr uint32_t kOut = SWIGLU ? 8 : 16;
+  float y[kOut];
 #pragma unroll
-  for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[f][i] = SWIGLU ? swiglu(acc[2 * f][i], acc[2 * f + 1][i]) : acc[f][i];
+  for (uint32_t j = 0; j < kOut; ++j)
+    y[j] = SWIGLU ? swiglu(acc[2 * (j / 4)][j % 4], acc[2 * (j / 4) + 1][j % 4]) : acc[j / 4][j % 4];
+  const uint32_t at = col + kOut * kb;
+  const uint64_t row = static_cast<uint64_t>(pair) * p.n;
   if constexpr (OUT == kOutMx) {
     static_assert(SWIGLU || OUT == kOutBf16, "a strip of SwiGLU outputs is one group");
     uint32_t m = 0;
 #pragma unroll
-    for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = max(m, mx_magnitude(y[f][i]));
+    for (uint32_t j = 0; j < kOut; ++j) m = max(m, mx_magnitude(y[j]));
     m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16)));
     m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32)));
     const uint32_t e = mx_scale(m);
     if (!live) return;
-    const uint64_t first = static_cast<uint64_t>(pair) * p.n + col;
-#pragma unroll
-    for (int f = 0; f < kFrags; ++f)
-      *reinterpret_cast<uint32_t*>(p.values + first + f * 16 + kb * 4) = mx_pack4(y[f][0], y[f][1], y[f][2], y[f][3], e);
-    if (kb == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e);
+    *reinterpret_cast<uint2*>(p.values + row + at) =
+        make_uint2(mx_pack4(y[0], y[1], y[2], y[3], e), mx_pack4(y[4], y[5], y[6], y[7], e));
+    if (kb == 0) p.scales[(row + col) / kMxGroup] = static_cast<uint8_t>(e);
   } else {
     if (!live) return;
-    uint16_t* row = p.out + static_cast<uint64_t>(pair) * p.n;
+    if (p.n % 8 == 0 && p.out_aligned) {
 #pragma unroll
-    for (int f = 0; f < kFrags; ++f) {
-      const uint32_t at = col + f * 16 + kb * 4;
-      if (p.n % 4 == 0) {
-        if (at < p.n)
-          *reinterpret_cast<uint2*>(row + at) = make_uint2(f32_to_bf16(y[f][0]) | (f32_to_bf16(y[f][1]) << 16),
-                                                           f32_to_bf16(y[f][2]) | (f32_to_bf16(y[f][3]) << 16));
-      } else {
+      for (uint32_t j = 0; j < kOut; j += 8) {
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (at + i < p.n) row[at + i] = static_cast<uint16_t>(f32_to_bf16(y[f][i]));
+        for (uint32_t i = 0; i < 4; ++i) w[i] = f32_to_bf16(y[j + 2 * i]) | (f32_to_bf16(y[j + 2 * i + 1]) << 16);
+        if (at + j < p.n) *reinterpret_cast<uint4*>(p.out + row + at + j) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < kOut; ++j)
+        if (at + j < p.n) p.out[row + at + j] = static_cast<uint16_t>(f32_to_bf16(y[j]));
     }
   }
 }
@@ -172,7 +178,7 @@ __device__ __forceinline__ void zero_row(const ProductLaunch& p, uint32_t pair, 
 template <int OUT>
 __device__ void zero_rows(const ProductLaunch& p, uint32_t first, uint32_t lane) {
   const uint32_t i = first + lane;
-  const bool none = i < p.rows && static_cast<uint32_t>(p.ids[i]) >= p.experts;
+  const bool none = lane < kZeroRows && i < p.rows && static_cast<uint32_t>(p.ids[i]) >= p.experts;
   uint64_t left = __ballot(none);
   while (left != 0) {
     const uint32_t j = static_cast<uint32_t>(__builtin_ctzll(left));
@@ -181,170 +187,129 @@ __device__ void zero_rows(const ProductLaunch& p, uint32_t first, uint32_t lane)
   }
 }
 
-// ---------------------------------------------------------------- stream ---
+// ------------------------------------------------------------------ rows ---
 
-// One row of 16 lanes' addresses: unit `u` of chunk `c`, or zeros at and behind the row's end.
-__device__ __forceinline__ const uint8_t* unit_at(const uint8_t* row, uint32_t c, uint32_t u, uint32_t k_bytes) {
-  const uint32_t at = c * kChunk + u * 16u;
-  return at < k_bytes ? row + at : reinterpret_cast<const uint8_t*>(g_product_zeros);
+constexpr int kRowBatch = 8;              // matrix rows a wave sums at once
+constexpr uint32_t kRowStep = 64 * 16;    // bytes of a row per step of a wave
+
+// Eight (bf16) or sixteen (MX) products of a lane's unit, fp32 sums.
+template <bool MX>
+__device__ __forceinline__ float unit_dot(const Operand<MX>& w, const Operand<MX>& x, float acc) {
+#pragma unroll
+  for (int i = 0; i < (MX ? 2 : 1); ++i) {
+    const uint32_t a[4] = {w.part[i].x, w.part[i].y, w.part[i].z, w.part[i].w};
+    const uint32_t b[4] = {x.part[i].x, x.part[i].y, x.part[i].z, x.part[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a[j]), __builtin_bit_cast(bf16x2, b[j]), acc, false);
+  }
+  return acc;
 }
 
-// The operands of one chunk and strip.
-template <bool MX, bool WHOLE>
-struct StreamChunk {
-  uint4 w[kStrip][2], x[2];
-  uint32_t ws[kStrip], xs;
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-  __device__ __forceinline__ void load(const uint8_t* const w_row[kStrip], const uint8_t* const ws_row[kStrip],
-                                       const uint8_t* x_row, const uint8_t* xs_row, uint32_t c, uint32_t kb,
-                                       uint32_t k_bytes) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      x[h] = ldg16(unit_at(x_row, c, 4 * h + kb, k_bytes));
-#pragma unroll
-      for (int f = 0; f < kStrip; ++f) w[f][h] = ldg16(unit_at(w_row[f], c, 4 * h + kb, k_bytes));
-    }
-    if constexpr (MX) {
-      // chunks behind the last one have zero values under any scale
-      const uint32_t groups = k_bytes / kMxGroup, at = WHOLE ? min(c, groups / 4u - 1u) : c;
-      xs = chunk_scales<WHOLE>(xs_row, at, groups);
-#pragma unroll
-      for (int f = 0; f < kStrip; ++f) ws[f] = chunk_scales<WHOLE>(ws_row[f], at, groups);
-    }
-  }
-  __device__ __forceinline__ void mfma(f32x4_t acc[kStrip], uint32_t kb) const {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const Operand<MX> xo(x[h], MX ? unit_scale(xs, kb, h) : 1.0f);
-#pragma unroll
-      for (int f = 0; f < kStrip; ++f)
-        acc[f] = unit_mfma(Operand<MX>(w[f][h], MX ? unit_scale(ws[f], kb, h) : 1.0f), xo, acc[f]);
-    }
-  }
-};
-
-// KS waves of a block split a strip's chunks between them and add up in LDS (4), or each wave has a strip of its own
-// (1).  SORTED: tiles of up to 16 sorted rows; else one routed row per block.  WHOLE: K is whole chunks and scales are
-// aligned to their four bytes.
-template <bool MX, bool SWIGLU, int OUT, int KS, bool SORTED, bool WHOLE>
-__global__ __launch_bounds__(256) void k_stream(ProductLaunch p) {
-  constexpr int kWaves = 4, kDepth = 2;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, lm = lane & 15u, kb = lane >> 4;
+// One routed row per block and 8 WAVES matrix rows, eight per wave: a wave reads a kilobyte of one matrix row at a
+// time, the row's unit of the lane stays in registers for all eight.
+template <bool MX, bool SWIGLU, int OUT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_rows(ProductLaunch p) {
+  constexpr uint32_t kMatrix = kRowBatch * WAVES, kCols = SWIGLU ? kMatrix / 2 : kMatrix;
+  static_assert(OUT == kOutBf16 || kCols == kMxGroup, "a block's outputs are one group");
+  __shared__ float s_y[kMatrix];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  constexpr uint32_t kCols = strip_cols<SWIGLU>() * (kWaves / KS);
   const uint32_t slices = (p.n + kCols - 1) / kCols;
-  uint32_t expert, pair, rows = 1, slice;
-  if constexpr (SORTED) {
-    // each XCD takes a contiguous run of the tiles with all their slices: its L2 serves a tile's rows to every slice
-    const uint32_t lin = blockIdx.x, local = (lin >> 3) / slices;
-    slice = (lin >> 3) % slices;
-    const uint32_t count = *p.tile_count, chunk = (count + 7) / 8;
-    const uint32_t tile = (lin & 7u) * chunk + local;
-    if (lin >= p.tile_blocks) {
-      zero_rows<OUT>(p, ((lin - p.tile_blocks) * kWaves + wave) * kZeroRows, lane);
-      return;
-    }
-    if (local >= chunk || tile >= count) return;
-    const uint2 td = p.tiles[tile];
-    expert = td.x;
-    const uint32_t row0 = p.row_off[expert] + td.y;
-    rows = min(p.row_off[expert + 1] - row0, kStreamRows);
-    pair = p.row_pair[row0 + min(lm, rows - 1)];
-  } else {
-    pair = blockIdx.x / slices;
-    slice = blockIdx.x % slices;
-    expert = static_cast<uint32_t>(p.ids[pair]);
-    if (expert >= p.experts) {
-      if (slice == 0 && wave == 0) zero_row<OUT>(p, pair, lane);
-      return;
-    }
+  const uint32_t pair = blockIdx.x / slices, col0 = blockIdx.x % slices * kCols;
+  const uint32_t expert = static_cast<uint32_t>(p.ids[pair]);
+  if (expert >= p.experts) {
+    if (col0 == 0 && wave == 0) zero_row<OUT>(p, pair, lane);
+    return;
   }
-  const uint32_t col = slice * kCols + (KS == 1 ? wave * strip_cols<SWIGLU>() : 0u);
-  const uint32_t x_row_id = pair / p.x_div;
-  const uint8_t* x_row = p.x + static_cast<uint64_t>(x_row_id) * p.x_stride;
-  const uint8_t* xs_row = MX ? p.x_scales + static_cast<uint64_t>(x_row_id) * p.x_scale_stride : nullptr;
-  const uint8_t* w_row[kStrip];
-  const uint8_t* ws_row[kStrip];
+  const uint8_t* x_row = p.x + static_cast<uint64_t>(pair / p.x_div) * p.x_stride;
+  const uint8_t* xs_row = MX ? p.x_scales + static_cast<uint64_t>(pair / p.x_div) * p.x_scale_stride : nullptr;
+  const uint8_t *w_row[kRowBatch], *ws_row[kRowBatch];
 #pragma unroll
-  for (int f = 0; f < kStrip; ++f) {
-    const uint64_t r = matrix_row<SWIGLU>(col, f * 16u + lm, p.n);
-    w_row[f] = p.w + expert * p.w_expert + r * p.w_stride;
-    ws_row[f] = MX ? p.w_scales + expert * p.w_scale_expert + r * p.w_scale_stride : nullptr;
+  for (int j = 0; j < kRowBatch; ++j) {
+    // with SwiGLU rows 2 j and 2 j + 1 of the block are gate and up of its output j
+    const uint32_t r = wave * kRowBatch + j;
+    const uint64_t m = SWIGLU ? min(col0 + r / 2, p.n - 1) + (r & 1u) * p.n : min(col0 + r, p.n - 1);
+    w_row[j] = p.w + expert * p.w_expert + m * p.w_stride;
+    ws_row[j] = MX ? p.w_scales + expert * p.w_scale_expert + m * p.w_scale_stride : nullptr;
   }
-  const uint32_t chunks = (p.k_bytes + kChunk - 1) / kChunk;
-  const uint32_t first = KS == 1 ? 0u : wave;
-  const uint32_t count = chunks > first ? (chunks - first + KS - 1) / KS : 0u;
-  f32x4_t acc[kStrip];
+  float acc[kRowBatch] = {};
+  uint4 xv, wv[kRowBatch];
+  uint32_t xs = 0, ws[kRowBatch] = {};
+  auto load = [&](uint32_t at) {
+    const bool in = at < p.k_bytes;
+    xv = ldg16(in ? x_row + at : reinterpret_cast<const uint8_t*>(g_product_zeros));
 #pragma unroll
-  for (int f = 0; f < kStrip; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  // chunks behind the last one load zeros, so no load of the pipeline is conditional
-  StreamChunk<MX, WHOLE> buf[kDepth];
+    for (int j = 0; j < kRowBatch; ++j) wv[j] = ldg16(in ? w_row[j] + at : reinterpret_cast<const uint8_t*>(g_product_zeros));
+    if constexpr (MX) {
+      const uint32_t g = min(at, p.k_bytes - 1) / kMxGroup;
+      xs = xs_row[g];
 #pragma unroll
-  for (int j = 0; j < kDepth; ++j) buf[j].load(w_row, ws_row, x_row, xs_row, first + j * KS, kb, p.k_bytes);
-  for (uint32_t i = 0; i < count; i += kDepth) {
-#pragma unroll
-    for (int j = 0; j < kDepth; ++j) {
-      buf[j].mfma(acc, kb);
-      buf[j].load(w_row, ws_row, x_row, xs_row, first + (i + j + kDepth) * KS, kb, p.k_bytes);
+      for (int j = 0; j < kRowBatch; ++j) ws[j] = ws_row[j][g];
     }
-  }
-  if constexpr (KS > 1) {
-    __shared__ f32x4_t s_acc[KS - 1][kStrip][64];
-    if (wave != 0) {
+  };
+  load(lane * 16u);
+  for (uint32_t at = lane * 16u; at - lane * 16u < p.k_bytes; at += kRowStep) {
+    const Operand<MX> x(xv, scale_of(xs));
+    uint4 now[kRowBatch];
+    uint32_t scale[kRowBatch];
 #pragma unroll
-      for (int f = 0; f < kStrip; ++f) s_acc[wave - 1][f][lane] = acc[f];
+    for (int j = 0; j < kRowBatch; ++j) {
+      now[j] = wv[j];
+      scale[j] = ws[j];
     }
-    __syncthreads();
-    if (wave != 0) return;
+    load(at + kRowStep);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int w = 0; w < KS - 1; ++w)
-#pragma unroll
-      for (int f = 0; f < kStrip; ++f) acc[f] += s_acc[w][f][lane];
+    for (int j = 0; j < kRowBatch; ++j) acc[j] = unit_dot(Operand<MX>(now[j], scale_of(scale[j])), x, acc[j]);
   }
-  if (col >= p.n) return;
-  store_strip<SWIGLU, OUT>(p, acc, col, pair, lm < rows, kb);
+#pragma unroll
+  for (int j = 0; j < kRowBatch; ++j) {
+    const float y = group_sum<64>(acc[j]);
+    if (lane == 63) s_y[wave * kRowBatch + j] = y;
+  }
+  __syncthreads();
+  if (tid >= kCols) return;
+  const float y = SWIGLU ? swiglu(s_y[2 * tid], s_y[2 * tid + 1]) : s_y[tid];
+  const uint64_t at = static_cast<uint64_t>(pair) * p.n + col0 + tid;
+  if constexpr (OUT == kOutMx) {
+    uint32_t m = mx_magnitude(y);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), d)));
+    const uint32_t e = mx_scale(m);
+    p.values[at] = static_cast<uint8_t>(mx_pack4(y, y, y, y, e));
+    if (tid == 0) p.scales[at / kMxGroup] = static_cast<uint8_t>(e);
+  } else if (col0 + tid < p.n) {
+    p.out[at] = static_cast<uint16_t>(f32_to_bf16(y));
+  }
 }
 
 // ----------------------------------------------------------------- tiles ---
 
-constexpr uint32_t kTileCols = 128;       // matrix rows per block
-
-// Unit u of row r lies at unit u ^ swz(r) of its 128 bytes: an operand read (lane: row lane % 16, unit lane / 16 or
-// 4 + lane / 16) then spreads over all 64 banks in every lane grouping of the read.
-__device__ __forceinline__ uint32_t tile_swz(uint32_t r) { return ((r >> 1) & 2u) | ((r << 1) & 4u); }
-
 // Stage J: the tile's rows, then the matrix rows, 128 bytes each; and the four scale bytes of each.  One LDS object
-// per stage, so that the compiler can tell the stage being read from the one being filled.
-template <int J, int BM>
+// per stage, so that the compiler can tell the stage being read from the ones being filled.
+template <int J, int ROWS>
 __device__ __forceinline__ uint8_t* tile_stage() {
-  __shared__ uint4 buf[(BM + kTileCols) * kChunk / 16];
+  __shared__ uint4 buf[ROWS * kChunk / 16];
   return reinterpret_cast<uint8_t*>(buf);
 }
-template <int J, int BM>
+template <int J, int ROWS>
 __device__ __forceinline__ uint32_t* tile_scales() {
-  __shared__ uint32_t buf[BM + kTileCols];
+  __shared__ uint32_t buf[ROWS];
   return buf;
 }
 
-// s_waitcnt for the vector memory count or the LDS count at zero, the others left alone
-__device__ __forceinline__ void wait_vm0() { __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); }
-__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4)); }
-
-// A block barrier that no memory access is moved across and that waits for none by itself.
-__device__ __forceinline__ void bare_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-// BM rows by 128 matrix rows; four waves of BM / 2 rows by 64 matrix rows each.  WHOLE: K is whole chunks.
-template <bool MX, bool SWIGLU, int OUT, int BM, bool WHOLE>
-__global__ __launch_bounds__(256) void k_tiles(ProductLaunch p) {
-  constexpr int kWaves = 4;
-  constexpr int kRowFrags = BM / 32;               // 16-row fragments per wave
-  constexpr int kDmaX = BM / 8 / kWaves;           // 1 KB loads (eight rows) per wave and chunk
-  constexpr int kDmaW = kTileCols / 8 / kWaves;
-  constexpr uint32_t kCols = strip_cols<SWIGLU>() * (kTileCols / 64);
+// WM x WN waves of 16 RF rows by 64 matrix rows each, S stages.  WHOLE: K is whole chunks and scales are aligned.
+template <bool MX, bool SWIGLU, int OUT, int RF, int WM, int WN, int S, bool WHOLE>
+__global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
+  constexpr int kWaves = WM * WN;
+  constexpr uint32_t kRows = 16 * RF * WM, kMatrix = 64 * WN;
+  constexpr int kDmaX = kRows / 8 / kWaves;           // 1 KB loads (eight rows) per wave and chunk
+  constexpr int kDmaW = kMatrix / 8 / kWaves;
+  static_assert(kDmaX * 8 * kWaves == kRows && kDmaW * 8 * kWaves == kMatrix, "whole 1 KB loads per wave");
+  constexpr uint32_t kCols = strip_cols<SWIGLU>() * WN;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, lm = lane & 15u, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t slices = (p.n + kCols - 1) / kCols;
@@ -356,12 +321,13 @@ __global__ __launch_bounds__(256) void k_tiles(ProductLaunch p) {
     return;
   }
   if (local >= run || tile >= count) return;
-  const uint2 td = p.tiles[tile];
-  const uint32_t expert = td.x;
-  const uint32_t row0 = p.row_off[expert] + td.y;
-  const uint32_t rows = min(p.row_off[expert + 1] - row0, static_cast<uint32_t>(BM));
+  const RowTile td = p.tiles[tile];
+  const uint32_t expert = td.group, row0 = td.row, rows = td.rows;
   const uint32_t col0 = slice * kCols;
   const uint8_t* w = p.w + expert * p.w_expert;
+  const auto matrix_at = [&](uint32_t r) {   // matrix row of the block's row r
+    return matrix_row<SWIGLU>(col0 + (r >> 6) * strip_cols<SWIGLU>(), r & 63u, p.n);
+  };
 
   // DMA: load i of a wave fills eight rows; lane j loads unit (j % 8) ^ swz(row) of row j / 8 into bytes 16 j, so the
   // swizzle costs nothing.  Rows behind the tile's last one load it again.
@@ -378,107 +344,121 @@ __global__ __launch_bounds__(256) void k_tiles(ProductLaunch p) {
 #pragma unroll
   for (int i = 0; i < kDmaW; ++i) {
     const uint32_t r = (wave * kDmaW + i) * 8u + sub;
-    const uint32_t n = matrix_row<SWIGLU>(col0 + (r >> 6) * strip_cols<SWIGLU>(), r & 63u, p.n);
     at[kDmaX + i] = (unit ^ tile_swz(r)) * 16u;
-    src[kDmaX + i] = w + n * p.w_stride + at[kDmaX + i];
+    src[kDmaX + i] = w + matrix_at(r) * p.w_stride + at[kDmaX + i];
   }
-  // scales: thread t serves row t of the stage
-  const uint8_t* scale_row = nullptr;
+  // scales: thread t serves rows t, t + threads, .. of the stage
+  constexpr uint32_t kThreads = 64 * kWaves, kScaleRows = MX ? (kRows + kMatrix + kThreads - 1) / kThreads : 1;
+  const uint8_t* scale_row[kScaleRows];
   if constexpr (MX) {
-    if (tid < BM) {
-      const uint32_t pair = p.row_pair[row0 + min(tid, rows - 1)];
-      scale_row = p.x_scales + static_cast<uint64_t>(pair / p.x_div) * p.x_scale_stride;
-    } else if (tid < BM + kTileCols) {
-      const uint32_t r = tid - BM;
-      const uint32_t n = matrix_row<SWIGLU>(col0 + (r >> 6) * strip_cols<SWIGLU>(), r & 63u, p.n);
-      scale_row = p.w_scales + expert * p.w_scale_expert + n * p.w_scale_stride;
+#pragma unroll
+    for (uint32_t i = 0; i < kScaleRows; ++i) {
+      const uint32_t r = min(i * kThreads + tid, kRows + kMatrix - 1);
+      const bool is_x = r < kRows;
+      const uint32_t pair = p.row_pair[row0 + min(r, rows - 1)];
+      scale_row[i] = is_x ? p.x_scales + static_cast<uint64_t>(pair / p.x_div) * p.x_scale_stride
+                          : p.w_scales + expert * p.w_scale_expert + matrix_at(r - kRows) * p.w_scale_stride;
     }
   }
   const uint32_t chunks = (p.k_bytes + kChunk - 1) / kChunk, groups = p.k_bytes / kMxGroup;
   auto issue = [&](auto J, uint32_t c) {
-    uint8_t* st = tile_stage<decltype(J)::value, BM>();
+    uint8_t* st = tile_stage<decltype(J)::value, kRows + kMatrix>();
 #pragma unroll
     for (int i = 0; i < kDmaX + kDmaW; ++i) {
-      const uint32_t g = i < kDmaX ? wave * kDmaX + i : BM / 8 + wave * kDmaW + (i - kDmaX);
+      const uint32_t g = i < kDmaX ? wave * kDmaX + i : kRows / 8 + wave * kDmaW + (i - kDmaX);
       const uint8_t* s = src[i] + c * kChunk;
       if constexpr (!WHOLE)
         if (c * kChunk + at[i] >= p.k_bytes) s = reinterpret_cast<const uint8_t*>(g_product_zeros);
-      __builtin_amdgcn_global_load_lds(s, (__attribute__((address_space(3))) void*)(st + g * 1024u), 16, 0, 0);
+      load_to_lds(s, st + g * 1024u);
     }
   };
-  auto scales_of = [&](uint32_t c) -> uint32_t {
-    return scale_row != nullptr ? chunk_scales<WHOLE>(scale_row, c, groups) : 0u;
-  };
-  auto keep_scales = [&](auto J, uint32_t v) {
-    if (tid < BM + kTileCols) tile_scales<decltype(J)::value, BM>()[tid] = v;
-  };
 
-  const uint32_t wm = wave & 1u, wn = wave >> 1;
+  const uint32_t wm = wave % WM, wn = wave / WM;
   const uint32_t s = tile_swz(lm);
   const uint32_t u0 = (kb ^ s) * 16u, u1 = ((4u | kb) ^ s) * 16u;
-  const uint32_t x_base = (wm * (BM / 2) + lm) * kChunk, w_base = (BM + wn * 64u + lm) * kChunk;
-  f32x4_t acc[kRowFrags][kStrip];
+  const uint32_t x_base = (wm * (16 * RF) + lm) * kChunk, w_base = (kRows + wn * 64u + lm) * kChunk;
+  // 16-row fragments of this wave that hold rows of the tile
+  const uint32_t live = rows > wm * (16 * RF) ? min((rows - wm * (16 * RF) + 15u) / 16u, static_cast<uint32_t>(RF)) : 0u;
+  f32x4_t acc[RF][kStrip];
 #pragma unroll
-  for (int i = 0; i < kRowFrags; ++i)
+  for (int i = 0; i < RF; ++i)
 #pragma unroll
     for (int f = 0; f < kStrip; ++f) acc[i][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto compute = [&](auto J) {
-    const uint8_t* st = tile_stage<decltype(J)::value, BM>();
-    uint32_t xs[kRowFrags], ws[kStrip];
+  // F fragments of stage J: all reads first, so that the second half's are under way while the first is multiplied
+  auto compute = [&](auto J, auto frags) {
+    constexpr int F = decltype(frags)::value;
+    const uint8_t* st = tile_stage<decltype(J)::value, kRows + kMatrix>();
+    uint32_t xs[F], ws[kStrip];
+    uint4 xv[2][F], wv[2][kStrip];
     if constexpr (MX) {
-      const uint32_t* sc = tile_scales<decltype(J)::value, BM>();
+      const uint32_t* sc = tile_scales<decltype(J)::value, kRows + kMatrix>();
 #pragma unroll
-      for (int f = 0; f < kStrip; ++f) ws[f] = sc[BM + wn * 64 + f * 16 + lm];
+      for (int f = 0; f < kStrip; ++f) ws[f] = sc[kRows + wn * 64 + f * 16 + lm];
 #pragma unroll
-      for (int i = 0; i < kRowFrags; ++i) xs[i] = sc[wm * (BM / 2) + i * 16 + lm];
+      for (int i = 0; i < F; ++i) xs[i] = sc[wm * (16 * RF) + i * 16 + lm];
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t u = h ? u1 : u0;
-      uint4 xv[kRowFrags], wv[kStrip];
 #pragma unroll
-      for (int f = 0; f < kStrip; ++f) wv[f] = *reinterpret_cast<const uint4*>(st + w_base + f * 16 * kChunk + u);
+      for (int f = 0; f < kStrip; ++f) wv[h][f] = *reinterpret_cast<const uint4*>(st + w_base + f * 16 * kChunk + u);
 #pragma unroll
-      for (int i = 0; i < kRowFrags; ++i) xv[i] = *reinterpret_cast<const uint4*>(st + x_base + i * 16 * kChunk + u);
+      for (int i = 0; i < F; ++i) xv[h][i] = *reinterpret_cast<const uint4*>(st + x_base + i * 16 * kChunk + u);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int f = 0; f < kStrip; ++f) {
-        const Operand<MX> wo(wv[f], MX ? unit_scale(ws[f], kb, h) : 1.0f);
+        const Operand<MX> wo(wv[h][f], MX ? unit_scale(ws[f], kb, h) : 1.0f);
 #pragma unroll
-        for (int i = 0; i < kRowFrags; ++i)
-          acc[i][f] = unit_mfma(wo, Operand<MX>(xv[i], MX ? unit_scale(xs[i], kb, h) : 1.0f), acc[i][f]);
+        for (int i = 0; i < F; ++i)
+          acc[i][f] = unit_mfma(wo, Operand<MX>(xv[h][i], MX ? unit_scale(xs[i], kb, h) : 1.0f), acc[i][f]);
       }
-    }
   };
 
-  using J0 = std::integral_constant<int, 0>;
-  using J1 = std::integral_constant<int, 1>;
-  auto step = [&](auto J, auto JN, uint32_t c) {
-    uint32_t v = 0;
-    if (c + 1 < chunks) {
-      issue(JN, c + 1);
-      if constexpr (MX) v = scales_of(c + 1);
+  // Ring of S stages: stage c % S is multiplied while the next S - 1 chunks are in flight.  Chunks behind the last one
+  // are loaded from its place again (their stages are never read), so that every step issues the same DMA loads and
+  // waits for all but the last S - 2 steps' of them; the scale loads stand before them and only add to what is in
+  // flight.
+  constexpr int kLoads = kDmaX + kDmaW;
+  uint32_t held[S][kScaleRows];   // the scale bytes on their way to a stage
+  auto begin = [&](auto J, uint32_t c) {
+    if constexpr (MX) {
+#pragma unroll
+      for (uint32_t i = 0; i < kScaleRows; ++i) held[decltype(J)::value][i] = chunk_scales<WHOLE>(scale_row[i], c, groups);
     }
-    compute(J);
-    wait_vm0();    // the next stage has landed; it was loaded for as long as this one was multiplied
-    if constexpr (MX) keep_scales(JN, v);
-    wait_lgkm0();  // this wave's reads and writes are done before the barrier
-    bare_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    issue(J, c);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  issue(J0{}, 0);
-  if constexpr (MX) keep_scales(J0{}, scales_of(0));
-  wait_vm0();
-  wait_lgkm0();
-  bare_barrier();
-  for (uint32_t c = 0; c < chunks; c += 2) {
-    step(J0{}, J1{}, c);
-    if (c + 1 < chunks) step(J1{}, J0{}, c + 1);
+  unroll<0, S - 1>([&](auto J) { begin(J, min(static_cast<uint32_t>(decltype(J)::value), chunks - 1)); });
+  for (uint32_t c = 0; c < chunks; c += S) {
+    unroll<0, S>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      if (c + j >= chunks) return;
+      wait_vm<(S - 2) * kLoads>();   // this wave's loads of stage j have landed
+      if constexpr (MX) {
+#pragma unroll
+        for (uint32_t i = 0; i < kScaleRows; ++i)
+          if (i * kThreads + tid < kRows + kMatrix) tile_scales<j, kRows + kMatrix>()[i * kThreads + tid] = held[j][i];
+      }
+      wait_lgkm0();                  // its reads of the stage before and its scales are done
+      bare_barrier();
+      begin(std::integral_constant<int, (j + S - 1) % S>{}, min(c + j + S - 1, chunks - 1));
+      if (live > RF / 2) compute(J, std::integral_constant<int, RF>{});
+      else if (live > RF / 4) compute(J, std::integral_constant<int, (RF + 1) / 2>{});
+      else if (live > 0) compute(J, std::integral_constant<int, (RF + 3) / 4>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
   }
+  wait_vm<0>();  // no load into LDS outlives the block
 
   const uint32_t col = col0 + wn * strip_cols<SWIGLU>();
   if (col >= p.n) return;
 #pragma unroll
-  for (int i = 0; i < kRowFrags; ++i) {
-    const uint32_t r = wm * (BM / 2) + i * 16u + lm;
+  for (int i = 0; i < RF; ++i) {
+    const uint32_t r = wm * (16 * RF) + i * 16u + lm;
     const uint32_t pair = p.row_pair[row0 + min(r, rows - 1)];
     store_strip<SWIGLU, OUT>(p, acc[i], col, pair, r < rows, kb);
   }
@@ -487,12 +467,12 @@ __global__ __launch_bounds__(256) void k_tiles(ProductLaunch p) {
 // -------------------------------------------------------------- dispatch ---
 
 template <class Kernel>
-hipError_t go(Kernel kernel, uint32_t blocks, const ProductLaunch& p, hipStream_t stream) {
+hipError_t go(Kernel kernel, uint32_t blocks, uint32_t threads, const ProductLaunch& p, hipStream_t stream) {
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("products", &start, &stop))
-    hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, start, stop, 0, p);
+    hipExtLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, start, stop, 0, p);
   else
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -504,46 +484,43 @@ bool scales_aligned(const ProductLaunch& p) {
 
 template <bool MX, bool SWIGLU, int OUT>
 hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) {
-  const uint32_t chunks = (p.k_bytes + kChunk - 1) / kChunk;
-  const bool split = chunks >= 16;  // a wave of a split strip then has at least four chunks
+  if (tile_rows == 0) {
+    constexpr int kWaves = OUT == kOutMx ? 8 : 4;
+    constexpr uint32_t cols = kRowBatch * kWaves / (SWIGLU ? 2 : 1);
+    return go(&k_rows<MX, SWIGLU, OUT, kWaves>, (p.n + cols - 1) / cols * p.rows, 64 * kWaves, p, stream);
+  }
+  const uint32_t tiles = (row_max_tiles(p.rows, p.experts, tile_rows) + 7) / 8 * 8;
   const bool whole = p.k_bytes % kChunk == 0 && (!MX || scales_aligned(p));
-  const auto stream_go = [&](auto sorted, uint32_t units, uint32_t more) {
-    constexpr bool kSorted = decltype(sorted)::value;
-    const uint32_t cols = strip_cols<SWIGLU>() * (split ? 1u : 4u);
-    p.tile_blocks = (p.n + cols - 1) / cols * units;
-    const uint32_t blocks = p.tile_blocks + more;
-    // bf16 loads check the row's end in either case
-    if (MX && whole)
-      return split ? go(&k_stream<MX, SWIGLU, OUT, 4, kSorted, MX>, blocks, p, stream)
-                   : go(&k_stream<MX, SWIGLU, OUT, 1, kSorted, MX>, blocks, p, stream);
-    return split ? go(&k_stream<MX, SWIGLU, OUT, 4, kSorted, false>, blocks, p, stream)
-                 : go(&k_stream<MX, SWIGLU, OUT, 1, kSorted, false>, blocks, p, stream);
+  const auto tiles_go = [&](auto rf, auto wm, auto wn) {
+    constexpr int RF = decltype(rf)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+    constexpr uint32_t kWaves = WM * WN, cols = strip_cols<SWIGLU>() * WN;
+    p.tile_blocks = (p.n + cols - 1) / cols * tiles;
+    const uint32_t blocks = p.tile_blocks + (p.rows + kWaves * kZeroRows - 1) / (kWaves * kZeroRows);
+    return whole ? go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, 2, true>, blocks, 64 * kWaves, p, stream)
+                 : go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, 2, false>, blocks, 64 * kWaves, p, stream);
   };
-  if (tile_rows == 0) return stream_go(std::false_type{}, p.rows, 0);
-  const uint32_t tiles = (grouped_max_tiles(p.rows, p.experts, tile_rows) + 7) / 8 * 8;
-  const uint32_t zero = (p.rows + 4 * kZeroRows - 1) / (4 * kZeroRows);
-  if (tile_rows == kStreamRows) return stream_go(std::true_type{}, tiles, zero);
-  const uint32_t cols = strip_cols<SWIGLU>() * 2u;
-  p.tile_blocks = (p.n + cols - 1) / cols * tiles;
-  if (tile_rows == 64)
-    return whole ? go(&k_tiles<MX, SWIGLU, OUT, 64, true>, p.tile_blocks + zero, p, stream)
-                 : go(&k_tiles<MX, SWIGLU, OUT, 64, false>, p.tile_blocks + zero, p, stream);
-  return whole ? go(&k_tiles<MX, SWIGLU, OUT, 128, true>, p.tile_blocks + zero, p, stream)
-               : go(&k_tiles<MX, SWIGLU, OUT, 128, false>, p.tile_blocks + zero, p, stream);
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I4 = std::integral_constant<int, 4>;
+  // 256 matrix rows per block read a tile's rows half as often as 128, but fewer such blocks fit a CU: for enough
+  // blocks of a long K
+  const uint32_t slices = (p.n + 4 * strip_cols<SWIGLU>() - 1) / (4 * strip_cols<SWIGLU>());
+  const bool wide = uint64_t(tiles) * slices >= 512 && (p.k_bytes + kChunk - 1) / kChunk >= VM_WIDEK;
+  if (tile_rows == 32) return wide ? tiles_go(I2{}, I1{}, I4{}) : tiles_go(I2{}, I1{}, I2{});
+  return wide ? tiles_go(I4{}, I1{}, I4{}) : tiles_go(I2{}, I2{}, I2{});
 }
 
 }  // namespace
 
 uint32_t product_tile_rows(uint32_t rows, uint32_t experts) {
-  if (rows <= 32) return 0;
-  const uint32_t mean = rows / experts;
-  return mean < 12 ? kStreamRows : mean < 96 ? 64u : 128u;
+  if (rows <= VM_ROWS) return 0;
+  return rows / experts < VM_MEAN ? 32u : 64u;
 }
 
 uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu) {
-  const uint64_t strips = (uint64_t(n) + (swiglu ? 31 : 63)) / (swiglu ? 32 : 64);
-  const uint64_t units = tile_rows == 0 ? rows : (uint64_t(rows) + tile_rows - 1) / tile_rows + experts + 7;
-  return units * strips + rows / (4 * kZeroRows) + 1;
+  const uint64_t strips = (uint64_t(n) + (swiglu ? 15 : 31)) / (swiglu ? 16 : 32);  // the narrowest blocks
+  const uint64_t units = tile_rows == 0 ? rows : uint64_t(rows) / tile_rows + experts + 7;
+  return units * strips + rows / (2 * kZeroRows) + 1;
 }
 
 hipError_t launch_products(const ProductLaunch& p, uint32_t tile_rows, hipStream_t stream) {

@@ -440,6 +440,27 @@ struct NormLaunch {
 
 hipError_t launch_norm(const NormLaunch& p, hipStream_t stream);
 
+// -------------------------------------------------------------- row sort --
+// Rows sorted by group (row_sort.hip).
+struct RowTile {
+  uint32_t group, row, rows, pad;  // first sorted row and how many
+};
+struct RowSortLaunch {
+  const int32_t* ids;          // [rows]
+  uint32_t* row_pair;          // out: row of every sorted row
+  RowTile* tiles;              // out: row_max_tiles entries of room
+  uint32_t* tile_count;        // out
+  uint32_t* block_counts;      // scratch of larger calls: [row_sort_blocks, groups]
+  uint32_t rows, groups, tile_rows;
+};
+constexpr uint32_t kOneLaunchRows = 16384;
+uint32_t row_sort_blocks(uint32_t rows);
+// Tiles of `rows` rows over `groups` groups: no group begins more than one that is not full.
+inline uint32_t row_max_tiles(uint32_t rows, uint32_t groups, uint32_t tile_rows) {
+  return rows / tile_rows + (groups < rows ? groups : rows);
+}
+hipError_t launch_row_sort(const RowSortLaunch& p, hipStream_t stream);
+
 // -------------------------------------------------------------- products --
 // Products of routed rows with their expert's matrix (products.hip).  Routed
 // row i reads x row i / x_div and writes output row i.  Byte strides.
@@ -450,8 +471,7 @@ struct ProductLaunch {
   const uint8_t* w_scales;
   uint64_t x_stride, x_scale_stride, w_stride, w_expert, w_scale_stride, w_scale_expert;
   const int32_t* ids;          // [rows] expert of every routed row; others' output rows are zeroed
-  const uint32_t* row_off;     // sorted calls: [experts + 1] first sorted row of every expert
-  const uint2* tiles;          // (expert, first row in it)
+  const RowTile* tiles;        // sorted calls
   const uint32_t* tile_count;
   const uint32_t* row_pair;    // routed row of every sorted row
   uint16_t* out;               // [rows, n] bf16, or
@@ -460,11 +480,11 @@ struct ProductLaunch {
   uint32_t rows, x_div, k_bytes, n, experts;
   uint32_t tile_blocks;        // blocks of the grid that serve tiles (set by launch_products)
   bool mx, swiglu;
+  bool out_aligned;            // out is 16-byte aligned
 };
 
 // How a call of this many routed rows runs: 0 its rows one by one, or rows per
-// tile (kStreamRows, 64 or 128) after a sort by expert.
-constexpr uint32_t kStreamRows = 16;
+// tile (32 or 64) after a sort by expert.
 uint32_t product_tile_rows(uint32_t rows, uint32_t experts);
 // An upper bound of a call's blocks.
 uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu);
@@ -484,14 +504,13 @@ struct AdapterLaunch {
   const int32_t* ids;          // [rows]
   uint16_t* out;               // [rows, n], may be base
   uint64_t base_stride, x_stride, out_stride;
-  const uint32_t* row_off;     // tiled calls: [adapters + 1] first sorted row of every adapter
-  const uint2* tiles;          // (adapter, first row in it)
+  const RowTile* tiles;        // tiled calls
   const uint32_t* tile_count;
   const uint32_t* row_pair;    // row of every sorted row
   uint32_t rows, k, n, rank, adapters;
   uint32_t splits, split_cols, tile_blocks;  // set by launch_adapters
   bool vector_k, vector_rank;  // x and A, B: rows of whole aligned 16-byte units
-  bool quads;                  // base and out: rows of whole aligned 8-byte units
+  bool vector_n;               // base and out: rows of whole aligned 16-byte units
 };
 
 // Rows up to which a call runs one block per row and column split, without a sort.

@@ -11,16 +11,17 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import device_call, require_same_device, route_ids, row_stride, rows_view
+from .device import device_call, route_ids, row_span
 
-_BF16 = (torch.bfloat16,)
+_BF16 = torch.bfloat16
 
 
-def _bank(name, t, shape):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16:
-        raise TypeError(f"{name} must be a bfloat16 tensor")
+def _bank(name, t, index):
+    if not isinstance(t, torch.Tensor) or t.dtype != _BF16 or not t.is_cuda or t.get_device() != index:
+        raise TypeError(f"{name} must be a bfloat16 tensor on GPU {index}")
     if t.dim() != 3 or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous of shape {shape}")
+        raise ValueError(f"{name} must be a contiguous bank of matrices")
+    return t.data_ptr()
 
 
 def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor, *,
@@ -32,44 +33,40 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     (1 without).  Up to 1024 adapters of rank up to 128.  The rank sums stay in fp32, and the result is rounded once.
     ``out`` may be base.
     """
-    x_rows, base_rows = rows_view("x", x, _BF16), rows_view("base", base, _BF16)
-    _bank("a", a, "(adapters, rank, k)")
-    _bank("b", b, "(adapters, n, rank)")
+    index = x.get_device() if isinstance(x, torch.Tensor) else None
+    x_at, x_stride = row_span("x", x, _BF16, index)
+    base_at, base_stride = row_span("base", base, _BF16, index)
+    a_at, b_at = _bank("a", a, index), _bank("b", b, index)
     adapters, rank, k = a.shape
-    n = base_rows.shape[1]
-    if x_rows.shape[1] != k or tuple(b.shape) != (adapters, n, rank) or x.shape[:-1] != base.shape[:-1]:
-        raise ValueError(f"base {tuple(base.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)} and b {tuple(b.shape)} "
+    lead, shape = x.shape[:-1], base.shape
+    n = shape[-1]
+    if x.shape[-1] != k or b.shape != (adapters, n, rank) or lead != shape[:-1]:
+        raise ValueError(f"base {tuple(shape)}, x {tuple(x.shape)}, a {tuple(a.shape)} and b {tuple(b.shape)} "
                          "do not fit together")
-    ids = route_ids("ids", ids, adapters)
-    if ids.shape != x.shape[:-1]:
-        raise ValueError(f"ids must have shape {tuple(x.shape[:-1])}")
-    if scales is not None and (scales.dtype != torch.float32 or scales.shape != (adapters,)
-                               or not scales.is_contiguous()):
-        raise ValueError(f"scales must be contiguous float32 of shape ({adapters},)")
-    device = x.device
-    if out is None:
-        out = torch.empty(base.shape, dtype=base.dtype, device=device)
-    elif out.shape != base.shape:
-        raise ValueError("out must have base's shape")
-    require_same_device(device, base=base, a=a, b=b, ids=ids, scales=scales, out=out)
-    out_rows = rows_view("out", out, _BF16)
-    if out.numel() == 0:
-        return out
-    p = _lib.VmAdapterArgs()
-    p.base, p.base_stride = base_rows.data_ptr(), row_stride(base_rows)
-    p.x, p.x_stride = x_rows.data_ptr(), row_stride(x_rows)
-    p.out, p.out_stride = out_rows.data_ptr(), row_stride(out_rows)
-    p.a, p.b, p.ids = a.data_ptr(), b.data_ptr(), ids.data_ptr()
+    ids = route_ids("ids", ids, adapters, index)
+    if ids.shape != lead:
+        raise ValueError(f"ids must have shape {tuple(lead)}")
+    scales_at = None
     if scales is not None:
-        p.scales = scales.data_ptr()
-    rows = x_rows.shape[0]
-    p.rows, p.k, p.n, p.rank, p.adapters = rows, k, n, rank, adapters
+        if scales.dtype != torch.float32 or scales.shape != (adapters,) or not scales.is_contiguous() \
+                or scales.device != x.device:
+            raise ValueError(f"scales must be contiguous float32 of shape ({adapters},) on {x.device}")
+        scales_at = scales.data_ptr()
+    if out is None:
+        out = base.new_empty(shape)
+    elif out.shape != shape:
+        raise ValueError("out must have base's shape")
+    out_at, out_stride = row_span("out", out, _BF16, index)
+    rows = ids.numel()
+    if rows == 0 or n == 0:
+        return out
     lib = _lib.lib()
     nbytes = lib.vm_add_adapters_workspace(rows, adapters)
-    if nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.check(device_call(device, lib.vm_add_adapters, ctypes.byref(p)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    p = _lib.VmAdapterArgs(base_at, x_at, a_at, b_at, scales_at, ids.data_ptr(), out_at,
+                           ws.data_ptr() if nbytes else None, nbytes, base_stride, x_stride, out_stride, rows, k, n,
+                           rank, adapters)
+    _lib.check(device_call(index, lib.vm_add_adapters, ctypes.byref(p)))
     return out
 
 

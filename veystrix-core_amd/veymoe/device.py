@@ -57,53 +57,56 @@ def stream_handle(stream=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream.cuda_stream)
 
 
-def device_call(device, call, *args) -> int:
-    """``call(*args, stream)`` on ``device``'s current stream, with ``device`` current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return call(*args, stream_handle())
-    with torch.cuda.device(device):
-        return call(*args, stream_handle())
+_current_device = torch._C._cuda_getDevice
 
 
-def rows_view(name: str, tensor, dtypes):
-    """``tensor`` [.., width] on the GPU as [rows, width], element stride 1 within a row and one stride between rows;
-    a tensor whose rows have no single stride is refused rather than copied."""
-    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
-        raise TypeError(f"{name} must be a tensor on the GPU")
-    if tensor.dtype not in dtypes:
-        raise TypeError(f"{name} has dtype {tensor.dtype}; expected one of {dtypes}")
-    if tensor.dim() == 0:
+def device_call(index, call, *args) -> int:
+    """``call(*args, stream)`` on the current stream of GPU ``index``, with that GPU current."""
+    if index == _current_device():
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def row_span(name: str, tensor, dtype, index):
+    """(address, elements between rows) of the rows of ``tensor`` [.., width], which must be contiguous in themselves,
+    lie at one stride (refused rather than copied otherwise), be of ``dtype`` and lie on GPU ``index``."""
+    try:
+        if tensor.dtype != dtype:
+            raise TypeError(f"{name} has dtype {tensor.dtype}; expected {dtype}")
+        if not tensor.is_cuda or tensor.get_device() != index:
+            raise TypeError(f"{name} must live on GPU {index} (got {tensor.device})")
+        strides = tensor.stride()
+    except AttributeError:
+        raise TypeError(f"{name} must be a torch tensor on the GPU, got {type(tensor).__name__}") from None
+    if len(strides) == 2 and strides[1] == 1:
+        return tensor.data_ptr(), strides[0]
+    shape = tensor.shape
+    if not shape:
         raise ValueError(f"{name} must have at least one dimension")
-    if tensor.dim() != 2:
-        try:
-            tensor = tensor.view(-1, tensor.shape[-1]) if tensor.numel() else tensor.reshape(-1, tensor.shape[-1])
-        except RuntimeError:
-            raise ValueError(f"the rows of {name} must have one stride") from None
-    if tensor.shape[1] > 1 and tensor.stride(1) != 1:
+    if shape[-1] > 1 and strides[-1] != 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    return tensor
+    step, span = None, 1        # the leading dimensions as one: each stride the inner one's extent
+    for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if size == 1:
+            continue
+        if step is None:
+            step = stride
+        elif stride != step * span:
+            raise ValueError(f"the rows of {name} must have one stride")
+        span *= size
+    return tensor.data_ptr(), shape[-1] if step is None else step
 
 
-def row_stride(rows) -> int:
-    """Elements between the rows of a [rows, width] view (a single row: its width)."""
-    return rows.stride(0) if rows.shape[0] > 1 else max(rows.shape[1], 1)
-
-
-def require_same_device(device, **tensors):
-    for name, tensor in tensors.items():
-        if tensor is not None and tensor.device != device:
-            raise ValueError(f"{name} is on {tensor.device}, not on {device}")
-
-
-def route_ids(name: str, ids, count: int):
-    """Contiguous int32 group ids on the GPU; 64-bit ids outside 0..count-1 stay outside."""
-    if not isinstance(ids, torch.Tensor) or not ids.is_cuda:
-        raise TypeError(f"{name} must be a tensor on the GPU")
+def route_ids(name: str, ids, count: int, index):
+    """Contiguous int32 group ids on GPU ``index``; 64-bit ids outside 0..count-1 stay outside."""
+    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.get_device() != index:
+        raise TypeError(f"{name} must be a tensor on GPU {index}")
     if ids.dtype == torch.int64:
         ids = ids.clamp(-1, count).to(torch.int32)
     elif ids.dtype != torch.int32:
         raise TypeError(f"{name} must be int32 or int64, got {ids.dtype}")
-    return ids.contiguous()
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def q4proj(weight=None, scales=None, biases=None) -> _lib.VmQ4Proj:

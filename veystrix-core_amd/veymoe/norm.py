@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .device import ACT_DTYPES, device_call, require_same_device, row_stride, rows_view
+from .device import ACT_DTYPES, device_call, row_span
 
 MX_GROUP = _lib.VM_MX_GROUP
 _SCALE_DTYPES = (torch.float8_e8m0fnu, torch.uint8)
@@ -44,13 +44,18 @@ def mx_empty(shape, device) -> MxTensor:
 def require_mx(name: str, t) -> MxTensor:
     if not isinstance(t, MxTensor):
         raise TypeError(f"{name} must be an MxTensor")
-    if not (t.values.is_cuda and t.scales.is_cuda) or t.values.device != t.scales.device:
-        raise TypeError(f"{name} must live on one GPU")
     if t.values.dtype != torch.float8_e4m3fn or t.scales.dtype not in _SCALE_DTYPES:
         raise TypeError(f"{name} must hold float8_e4m3fn values and float8_e8m0fnu (or uint8) scales")
     if t.values.shape[-1] % MX_GROUP or t.scales.shape != (*t.values.shape[:-1], t.values.shape[-1] // MX_GROUP):
         raise ValueError(f"{name} needs one scale per {MX_GROUP} values of a row")
     return t
+
+
+def _act_dtype(name, t) -> int:
+    try:
+        return ACT_DTYPES[t.dtype]
+    except (AttributeError, KeyError):
+        raise TypeError(f"{name} must be a bfloat16 or float32 tensor") from None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residual: torch.Tensor = None,
@@ -64,60 +69,58 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     (width a multiple of 32).  With a residual it returns ``(normed, h)``, h rounded to x's type; the norm itself reads
     the unrounded sum.  ``out`` may be x, ``residual_out`` may be x or residual.
     """
-    rows = rows_view("x", x, tuple(ACT_DTYPES))
-    width = rows.shape[1]
-    device = x.device
-    if not isinstance(weight, torch.Tensor) or weight.dtype not in ACT_DTYPES:
-        raise TypeError("weight must be a bfloat16 or float32 tensor")
+    act = _act_dtype("x", x)
+    dtype, shape, index = x.dtype, x.shape, x.get_device()
+    x_at, x_stride = row_span("x", x, dtype, index)
+    width = shape[-1]
+    weight_act = _act_dtype("weight", weight)
     if weight.shape != (width,) or not weight.is_contiguous():
         raise ValueError(f"weight must be contiguous of shape ({width},)")
-    if quantize and out is not None:
-        raise ValueError("out is not taken with quantize")
-    if residual_out is not None and residual is None:
-        raise ValueError("residual_out needs a residual")
-    require_same_device(device, weight=weight, residual=residual, out=out, residual_out=residual_out)
-    a = _lib.VmNormArgs()
-    a.x, a.x_stride = rows.data_ptr(), row_stride(rows)
-    a.weight = weight.data_ptr()
+    w_at, _ = row_span("weight", weight, weight.dtype, index)
+    r_at = r_stride = s_at = s_stride = y_at = y_stride = values_at = scales_at = 0
     if residual is not None:
-        if residual.shape != x.shape:
+        if residual.shape != shape:
             raise ValueError("residual must have x's shape")
-        r = rows_view("residual", residual, (x.dtype,))
+        r_at, r_stride = row_span("residual", residual, dtype, index)
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=device)
-        elif residual_out.shape != x.shape:
+            residual_out = x.new_empty(shape)
+        elif residual_out.shape != shape:
             raise ValueError("residual_out must have x's shape")
-        s = rows_view("residual_out", residual_out, (x.dtype,))
-        a.residual, a.residual_stride = r.data_ptr(), row_stride(r)
-        a.sum_out, a.sum_stride = s.data_ptr(), row_stride(s)
+        s_at, s_stride = row_span("residual_out", residual_out, dtype, index)
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
     if quantize:
+        if out is not None:
+            raise ValueError("out is not taken with quantize")
         if width % MX_GROUP:
             raise ValueError(f"quantize needs a width that is a multiple of {MX_GROUP}")
-        y = mx_empty(x.shape, device)
-        a.values, a.scales = y.values.data_ptr(), y.scales.data_ptr()
+        y = mx_empty(shape, x.device)
+        values_at, scales_at = y[0].data_ptr(), y[1].data_ptr()
     else:
-        y = torch.empty(x.shape, dtype=x.dtype, device=device) if out is None else out
-        if y.shape != x.shape:
+        y = x.new_empty(shape) if out is None else out
+        if y.shape != shape:
             raise ValueError("out must have x's shape")
-        o = rows_view("out", y, (x.dtype,))
-        a.out, a.out_stride = o.data_ptr(), row_stride(o)
-    a.rows, a.width = rows.shape
-    a.act_dtype, a.weight_dtype = ACT_DTYPES[x.dtype], ACT_DTYPES[weight.dtype]
-    a.one_centered = int(one_centered)
-    a.eps = eps
-    _lib.check(device_call(device, _lib.lib().vm_rms_norm, ctypes.byref(a)))
+        y_at, y_stride = row_span("out", y, dtype, index)
+    count = x.numel()
+    if count:
+        a = _lib.VmNormArgs(x_at, r_at or None, w_at, y_at or None, s_at or None, values_at or None, scales_at or None,
+                            x_stride, r_stride, y_stride, s_stride, count // width, width, act, weight_act,
+                            one_centered, eps)
+        _lib.check(device_call(index, _lib.lib().vm_rms_norm, ctypes.byref(a)))
     return y if residual is None else (y, residual_out)
 
 
 def mx_quantize(x: torch.Tensor) -> MxTensor:
     """x [.., width] bfloat16 or float32 (equally spaced rows, width a multiple of 32 up to 16384) as MX rows."""
-    rows = rows_view("x", x, tuple(ACT_DTYPES))
-    if rows.shape[1] % MX_GROUP:
+    act = _act_dtype("x", x)
+    at, stride = row_span("x", x, x.dtype, x.get_device())
+    width = x.shape[-1]
+    if width % MX_GROUP:
         raise ValueError(f"MX rows need a width that is a multiple of {MX_GROUP}")
     y = mx_empty(x.shape, x.device)
-    _lib.check(device_call(x.device, _lib.lib().vm_mx_quantize, rows.data_ptr(), row_stride(rows),
-                           y.values.data_ptr(), y.scales.data_ptr(), rows.shape[0], rows.shape[1],
-                           ACT_DTYPES[x.dtype]))
+    if x.numel():
+        _lib.check(device_call(x.get_device(), _lib.lib().vm_mx_quantize, at, stride, y.values.data_ptr(),
+                               y.scales.data_ptr(), x.numel() // width, width, act))
     return y
 
 

@@ -12,17 +12,22 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import device_call, require_same_device, route_ids, row_stride, rows_view
+from .device import device_call, route_ids, row_span
 from .norm import MX_GROUP, MxTensor, mx_empty, require_mx
 
 
-def _matrices(name, w):
-    """(row stride, expert stride) of weight [experts, n, k] with contiguous rows."""
+def _matrices(name, w, dtype, index):
+    """(address, row stride, expert stride) of a bank [experts, n, k] on GPU ``index`` with contiguous rows."""
+    if not isinstance(w, torch.Tensor) or w.dtype != dtype:
+        raise TypeError(f"{name} must be a tensor of {dtype}")
+    if not w.is_cuda or w.get_device() != index:
+        raise TypeError(f"{name} must live on GPU {index} (got {w.device})")
     if w.dim() != 3:
         raise ValueError(f"{name} must have shape (experts, outputs, inputs)")
-    if w.shape[2] > 1 and w.stride(2) != 1:
+    expert, row, one = w.stride()
+    if one != 1 and w.shape[2] > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    return (w.stride(1) if w.shape[1] > 1 else w.shape[2]), (w.stride(0) if w.shape[0] > 1 else 0)
+    return w.data_ptr(), row, expert
 
 
 def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, quantize: bool = False,
@@ -47,57 +52,54 @@ def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, qua
     if quantize and out is not None:
         raise ValueError("out is not taken with quantize")
     xv, wv = (require_mx("x", x).values, require_mx("weight", weight).values) if mx else (x, weight)
-    if not isinstance(wv, torch.Tensor) or not wv.is_cuda:
-        raise TypeError("weight must be a tensor on the GPU")
-    if not mx and wv.dtype != torch.bfloat16:
-        raise TypeError(f"weight has dtype {wv.dtype}; expected bfloat16 or an MxTensor")
-    rows = rows_view("x", xv, (torch.float8_e4m3fn if mx else torch.bfloat16,))
-    device = rows.device
-    a = _lib.VmProductArgs()
-    a.weight_stride, a.weight_expert_stride = _matrices("weight", wv)
-    experts, matrix, k = wv.shape
-    if swiglu and matrix % 2:
-        raise ValueError("swiglu needs an even number of matrix rows (gate, then up)")
-    n = matrix // 2 if swiglu else matrix
-    inds = route_ids("inds", inds, experts)
-    shape = tuple(inds.shape)
-    if tuple(xv.shape) == (*shape, k):
-        x_div = 1
-    elif shape and tuple(xv.shape) == (*shape[:-1], k):
-        x_div = shape[-1]
-    else:
-        raise ValueError(f"x of shape {tuple(xv.shape)} does not fit inds {shape} and weight {tuple(wv.shape)}")
-    require_same_device(device, weight=wv, inds=inds, out=out)
+    dtype = torch.float8_e4m3fn if mx else torch.bfloat16
+    index = xv.get_device() if isinstance(xv, torch.Tensor) else None
+    x_at, x_stride = row_span("x", xv, dtype, index)
+    w_at, w_stride, w_expert = _matrices("weight", wv, dtype, index)
+    experts, n, k = wv.shape
+    if swiglu:
+        if n % 2:
+            raise ValueError("swiglu needs an even number of matrix rows (gate, then up)")
+        n //= 2
+    inds = route_ids("inds", inds, experts, index)
+    lead, shape = xv.shape[:-1], inds.shape
+    x_div = 1
+    if lead != shape:
+        if not shape or lead != shape[:-1]:
+            raise ValueError(f"x {tuple(xv.shape)} does not fit inds {tuple(shape)} and weight {tuple(wv.shape)}")
+        x_div = max(shape[-1], 1)
+    if xv.shape[-1] != k:
+        raise ValueError(f"x {tuple(xv.shape)} does not fit weight {tuple(wv.shape)}")
+    y_at = values_at = scales_at = None
     if quantize:
         if n % MX_GROUP:
             raise ValueError(f"quantize needs a multiple of {MX_GROUP} outputs")
-        y = mx_empty((*shape, n), device)
-        a.out_values, a.out_scales = y.values.data_ptr(), y.scales.data_ptr()
+        y = mx_empty((*shape, n), xv.device)
+        values_at, scales_at = y[0].data_ptr(), y[1].data_ptr()
     else:
-        y = torch.empty((*shape, n), dtype=torch.bfloat16, device=device) if out is None else out
-        if y.shape != (*shape, n) or y.dtype != torch.bfloat16 or not y.is_contiguous():
-            raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {(*shape, n)}")
-        a.out = y.data_ptr()
-    count = inds.numel()
-    if count == 0 or n == 0:
+        if out is None:
+            y = torch.empty((*shape, n), dtype=torch.bfloat16, device=xv.device)
+        elif out.shape != (*shape, n) or out.dtype != torch.bfloat16 or not out.is_contiguous() \
+                or out.device != xv.device:
+            raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {(*shape, n)} on {xv.device}")
+        else:
+            y = out
+        y_at = y.data_ptr()
+    rows = inds.numel()
+    if rows == 0 or n == 0:
         return y
-    a.x, a.x_stride = rows.data_ptr(), row_stride(rows)
-    a.weight = wv.data_ptr()
+    xs_at = ws_at = None
+    xs_stride = ws_stride = ws_expert = 0
     if mx:
-        scales = rows_view("x scales", x.scales, (x.scales.dtype,))
-        a.x_scales, a.x_scale_stride = scales.data_ptr(), row_stride(scales)
-        a.weight_scales = weight.scales.data_ptr()
-        a.weight_scale_stride, a.weight_scale_expert_stride = _matrices("weight scales", weight.scales)
-        a.format = _lib.VM_FORMAT_MX
-    a.ids = inds.data_ptr()
-    a.rows, a.x_div, a.k, a.n, a.experts = count, x_div, k, n, experts
-    a.activation = int(swiglu)
+        xs_at, xs_stride = row_span("x scales", x.scales, x.scales.dtype, index)
+        ws_at, ws_stride, ws_expert = _matrices("weight scales", weight.scales, weight.scales.dtype, index)
     lib = _lib.lib()
-    nbytes = lib.vm_grouped_matmul_workspace(count, experts)
-    if nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.check(device_call(device, lib.vm_grouped_matmul, ctypes.byref(a)))
+    nbytes = lib.vm_grouped_matmul_workspace(rows, experts)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=xv.device) if nbytes else None
+    a = _lib.VmProductArgs(x_at, xs_at, w_at, ws_at, inds.data_ptr(), y_at, values_at, scales_at,
+                           ws.data_ptr() if nbytes else None, nbytes, x_stride, xs_stride, w_stride, w_expert,
+                           ws_stride, ws_expert, rows, x_div, k, n, experts, mx, swiglu)
+    _lib.check(device_call(index, lib.vm_grouped_matmul, ctypes.byref(a)))
     return y
 
 
