@@ -130,17 +130,23 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t acc) {
                                                  0, 0, 0);
 }
 
-// Stage J of every wave's own ring: first 16 rows of x and 16 RF rows of A, 128 bytes each, then strips of B (at most
-// 2 RF KB).
+// LDS of the waves, each its own part.  For the rank sums stage J is A's 16 RF rows of a chunk (main J) and the tile's 16
+// rows of x (side J).  After them main J holds a strip of B (64 rows of at most 16 RF ranks: as many bytes), and the two
+// sides the strip's products.  Four objects, and whole offsets in one step: past a few of those the compiler no longer
+// tells the objects apart and waits for every load in flight before it reads any.
 template <int RF>
-constexpr uint32_t stage_bytes() {
-  return (kAdapterTile + 16 * RF) * kChunk;
+constexpr uint32_t main_bytes() {
+  return 16 * RF * kChunk;
 }
-// Byte `at` of it; whole offsets in one step, past a few of which the compiler no longer tells the stages apart and
-// waits for every load in flight before it reads one.
+constexpr uint32_t kSideBytes = kAdapterTile * kChunk;
 template <int J, int RF>
-__device__ __forceinline__ uint8_t* wave_stage(uint32_t at) {
-  __shared__ uint4 buf[kTileWaves * stage_bytes<RF>() / 16];
+__device__ __forceinline__ uint8_t* lds_main(uint32_t at) {
+  __shared__ uint4 buf[kTileWaves * main_bytes<RF>() / 16];
+  return reinterpret_cast<uint8_t*>(buf) + at;
+}
+template <int J>
+__device__ __forceinline__ uint8_t* lds_side(uint32_t at) {
+  __shared__ uint4 buf[kTileWaves * kSideBytes / 16];
   return reinterpret_cast<uint8_t*>(buf) + at;
 }
 
@@ -149,7 +155,7 @@ template <int RF>
 __device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t id, uint32_t first_row, uint32_t rows,
                                               uint32_t wave, uint32_t lane, f32x4_t acc[RF]) {
   constexpr int kLoads = (kAdapterTile + 16 * RF) / 8;
-  const uint32_t lm = lane & 15u, kb = lane >> 4, sub = lane / 8u, mine = wave * stage_bytes<RF>();
+  const uint32_t lm = lane & 15u, kb = lane >> 4, sub = lane / 8u;
   const uint8_t* src[kLoads];
   const uint32_t unit = ((lane % 8u) ^ tile_swz(sub)) * 16u;   // byte of the lane's unit in a chunk of rows sub, 8 + sub, ..
 #pragma unroll
@@ -164,15 +170,18 @@ __device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t i
     }
   }
   const uint32_t k_bytes = p.k * 2, chunks = (k_bytes + kChunk - 1) / kChunk;
+  const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_adapter_zeros);
+  VM_KEEP(zeros);
   auto issue = [&](auto J, uint32_t c) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      load_to_lds(c * kChunk + unit < k_bytes ? src[i] + c * kChunk : reinterpret_cast<const uint8_t*>(g_adapter_zeros),
-                  wave_stage<decltype(J)::value, RF>(mine + i * 1024u));
+      load_to_lds(c * kChunk + unit < k_bytes ? src[i] + c * kChunk : zeros,
+                  i < 2 ? lds_side<decltype(J)::value>(wave * kSideBytes + i * 1024u)
+                        : lds_main<decltype(J)::value, RF>(wave * main_bytes<RF>() + (i - 2) * 1024u));
     __builtin_amdgcn_sched_barrier(0);
   };
   const uint32_t s = tile_swz(lm);
-  const uint32_t u[2] = {mine + lm * kChunk + (kb ^ s) * 16u, mine + lm * kChunk + ((4u | kb) ^ s) * 16u};
+  const uint32_t u[2] = {lm * kChunk + (kb ^ s) * 16u, lm * kChunk + ((4u | kb) ^ s) * 16u};
   // a wave without a chunk, and the steps behind a wave's last one, load zeros: every step issues the same loads
   using J0 = std::integral_constant<int, 0>;
   issue(J0{}, wave);
@@ -183,10 +192,11 @@ __device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t i
       wait_vm<kLoads>();   // this step's loads have landed; the next one's are in flight
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint4 x = *reinterpret_cast<const uint4*>(wave_stage<j, RF>(u[h]));
+        const uint4 x = *reinterpret_cast<const uint4*>(lds_side<j>(wave * kSideBytes + u[h]));
 #pragma unroll
         for (uint32_t f = 0; f < RF; ++f)
-          acc[f] = mfma(*reinterpret_cast<const uint4*>(wave_stage<j, RF>(u[h] + (f + 1) * 16 * kChunk)), x, acc[f]);
+          acc[f] = mfma(*reinterpret_cast<const uint4*>(lds_main<j, RF>(wave * main_bytes<RF>() + u[h] + f * 16 * kChunk)), x,
+                        acc[f]);
       }
       wait_lgkm0();        // the stage has been read before it is filled again
       __builtin_amdgcn_sched_barrier(0);
@@ -220,9 +230,7 @@ template <int RF, bool VEC_K, bool VEC_R, bool VEC_N>
 __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p) {
   constexpr int kSteps = (RF + 1) / 2;                      // MFMA steps over the rank
   constexpr uint32_t kPitch = kSteps * 64 + 16;             // bytes of a row of rank sums in LDS
-  // first the rank sums' bf16 values and rests, then every wave's 16 x 64 products in fp32
-  __shared__ uint4 s_y[kTileWaves * 16 * 64 * 4 / 16];
-  static_assert(2 * kAdapterTile * kPitch <= sizeof(s_y), "the rank sums fit");
+  static_assert(2 * kAdapterTile * kPitch <= kTileWaves * main_bytes<RF>(), "the rank sums fit");
   const uint32_t tid = threadIdx.x, lane = tid & 63u, lm = lane & 15u, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lin = blockIdx.x;
@@ -253,8 +261,8 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
   else rank_sums_direct<RF>(p, id, td.row, rows, wave, lane, acc);
 
   // Strips of 64 columns.  B's rows of a strip lie side by side: one copy of 64 rank values to LDS, whose units are
-  // swizzled within their rows where a row is a power of two of them; base goes to registers as the rows' own units,
-  // lane j holding unit j % 8 of row j / 8 (and of row 8 + j / 8).  Both are fetched a strip ahead.
+  // swizzled within their rows where a row is a power of two of them; base goes to registers.  Both are fetched a strip
+  // ahead.
   const uint32_t first = split * p.split_cols, end = min(first + p.split_cols, p.n);
   const uint8_t* b = reinterpret_cast<const uint8_t*>(p.b + static_cast<uint64_t>(id) * p.n * p.rank);
   const uint32_t units = p.rank / 8, b_units = p.n * units;   // of a row, of the matrix (VEC_R)
@@ -273,38 +281,35 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
 #pragma unroll
       for (uint32_t i = 0; i < kB; ++i)
         load_to_lds(b + static_cast<uint64_t>(min(col * units + b_unit[i], b_units - 1)) * 16u,
-                    wave_stage<decltype(J)::value, RF>(wave * stage_bytes<RF>() + i * 1024u));
+                    lds_main<decltype(J)::value, RF>(wave * main_bytes<RF>() + i * 1024u));
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  uint64_t base_at[2], out_at[2];
-#pragma unroll
-  for (uint32_t h = 0; h < 2; ++h) {
-    const uint32_t row = p.row_pair[td.row + min(lane / 8u + 8u * h, rows - 1)];
-    base_at[h] = static_cast<uint64_t>(row) * p.base_stride;
-    out_at[h] = static_cast<uint64_t>(row) * p.out_stride;
-  }
-  const uint32_t sub = 8u * (lane & 7u);
+  // lane j serves eight columns of row j / 4: 32 h + 8 (j % 4) of each half h of a strip
+  const uint32_t my_row = lane >> 2, sub = 8u * (lane & 3u);
+  const uint32_t out_row = p.row_pair[td.row + min(my_row, rows - 1)];
+  const uint16_t* base_row = p.base + static_cast<uint64_t>(out_row) * p.base_stride;
+  uint16_t* const out = p.out + static_cast<uint64_t>(out_row) * p.out_stride;
   uint4 base[2][2];
   auto load_base = [&](int j, uint32_t col) {
     if constexpr (VEC_N) {
+      // units behind the row's end load its last one, which is not stored
 #pragma unroll
-      for (int h = 0; h < 2; ++h) base[j][h] = unit_of<true>(p.base + base_at[h], col + sub, p.n);
+      for (uint32_t h = 0; h < 2; ++h) base[j][h] = ldg16(base_row + min(col + 32u * h + sub, p.n - 8u));
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // the waves' rank sums join: in stage 0, which is free
-  f32x4_t* part = reinterpret_cast<f32x4_t*>(wave_stage<0, RF>(0));
-  constexpr uint32_t kWavePart = stage_bytes<RF>() / 16;
-  static_assert(RF * 1024 <= stage_bytes<RF>(), "the partial sums fit");
+  // the waves' rank sums join: in main 0, and in main 1 their bf16 values and rests
+  f32x4_t* part = reinterpret_cast<f32x4_t*>(lds_main<0, RF>(0));
+  constexpr uint32_t kWavePart = main_bytes<RF>() / 16;
 #pragma unroll
   for (int f = 0; f < RF; ++f) part[wave * kWavePart + f * 64 + lane] = acc[f];
   uint32_t col = first + wave * kTileCols;
   load_base(0, col);
   lds_barrier();
   // lane holds rank sums 16 f + 4 kb .. +3 of its row; ranks at and behind `rank` are zero
-  uint8_t* v_hi = reinterpret_cast<uint8_t*>(s_y);
+  uint8_t* v_hi = lds_main<1, RF>(0);
   uint8_t* v_lo = v_hi + kAdapterTile * kPitch;
   for (uint32_t f = wave; f < kSteps * 2; f += kTileWaves) {
     uint32_t hi[4], lo[4];
@@ -332,8 +337,7 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
     hi[s] = *reinterpret_cast<const uint4*>(v_hi + lm * kPitch + s * 64 + kb * 16);
     lo[s] = *reinterpret_cast<const uint4*>(v_lo + lm * kPitch + s * 64 + kb * 16);
   }
-  lds_barrier();  // the rank sums have been read before the products take their place
-  float* y_wave = reinterpret_cast<float*>(s_y) + wave * 16 * 64;
+  lds_barrier();  // the rank sums have been read before a strip of B takes their place
 
   auto strip = [&](auto J) {
     constexpr int j = decltype(J)::value;
@@ -354,7 +358,7 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
         uint4 w = make_uint4(0, 0, 0, 0);
         if constexpr (VEC_R) {
           if (unit < units) w = *reinterpret_cast<const uint4*>(
-                wave_stage<j, RF>(wave * stage_bytes<RF>() + (r * units + (unit ^ ((r >> shift) & mask))) * 16u));
+                lds_main<j, RF>(wave * main_bytes<RF>() + (r * units + (unit ^ ((r >> shift) & mask))) * 16u));
         } else {
           const uint16_t* row = p.b + (static_cast<uint64_t>(id) * p.n + min(col + r, p.n - 1)) * p.rank;
           w = unit_of<false>(row, unit * 8u, p.rank);
@@ -363,23 +367,25 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
         y[f] = mfma(w, lo[s], y[f]);
       }
     }
-    // lane holds columns 16 f + 4 kb .. +3 of row lm: unit 4 f + kb of 16, stored at that ^ lm
+    // lane holds columns 16 f + 4 kb .. +3 of row lm, unit 4 (f % 2) + kb of half f / 2, stored at that ^ (lm % 8)
 #pragma unroll
-    for (uint32_t f = 0; f < 4; ++f)
-      *reinterpret_cast<f32x4_t*>(y_wave + lm * 64u + ((4u * f + kb) ^ lm) * 4u) = y[f];
+    for (uint32_t f = 0; f < 4; ++f) {
+      const uint32_t at = wave * kSideBytes + lm * 128u + ((4u * (f & 1u) + kb) ^ (lm & 7u)) * 16u;
+      *reinterpret_cast<f32x4_t*>(f < 2 ? lds_side<0>(at) : lds_side<1>(at)) = y[f];
+    }
     wait_lgkm0();  // the wave's own stores, in order
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
-      const uint32_t r = lane / 8u + 8u * h;
       float o[8];
 #pragma unroll
       for (uint32_t q = 0; q < 2; ++q) {
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(y_wave + r * 64u + ((2u * (lane & 7u) + q) ^ r) * 4u);
+        const uint32_t from = wave * kSideBytes + my_row * 128u + ((2u * (lane & 3u) + q) ^ (my_row & 7u)) * 16u;
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(h == 0 ? lds_side<0>(from) : lds_side<1>(from));
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[4 * q + i] = v[i];
       }
-      if (r >= rows) continue;
-      const uint32_t at = col + sub;
+      if (my_row >= rows) continue;
+      const uint32_t at = col + 32u * h + sub;
       if constexpr (VEC_N) {
         const uint32_t v[4] = {base[j][h].x, base[j][h].y, base[j][h].z, base[j][h].w};
         uint32_t w[4];
@@ -387,12 +393,11 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
         for (int i = 0; i < 4; ++i)
           w[i] = f32_to_bf16(__uint_as_float(v[i] << 16) + o[2 * i]) |
                  (f32_to_bf16(__uint_as_float(v[i] & 0xffff0000u) + o[2 * i + 1]) << 16);
-        if (at < p.n) *reinterpret_cast<uint4*>(p.out + out_at[h] + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (at < p.n) *reinterpret_cast<uint4*>(out + at) = make_uint4(w[0], w[1], w[2], w[3]);
       } else {
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
-          if (at + i < p.n)
-            p.out[out_at[h] + at + i] = static_cast<uint16_t>(f32_to_bf16(bf16_to_f32(p.base[base_at[h] + at + i]) + o[i]));
+          if (at + i < p.n) out[at + i] = static_cast<uint16_t>(f32_to_bf16(bf16_to_f32(base_row[at + i]) + o[i]));
       }
     }
     wait_lgkm0();  // stage and products have been read before they are written again
@@ -429,11 +434,11 @@ hipError_t tiles_go(const AdapterLaunch& p, uint32_t blocks, hipStream_t stream)
   return go(&k_adapter_tiles<RF, false, false, false>, blocks, kTileThreads, p, stream);
 }
 
-// Columns per block: all of them once the units (rows or tiles) fill the chip twice, at least `least` and whole strips
-// of a block.
-uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least) {
+// Columns per block, a multiple of `least`: as many splits of the columns as keep the blocks of `units` rows or tiles
+// within the `slots` that run at once, since every split of a unit computes its rank sums again.
+uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least, uint32_t slots) {
   const uint32_t parts = (n + least - 1) / least;
-  const uint32_t want = units >= 512 ? 1u : min(parts, (512 + units - 1) / units);
+  const uint32_t want = min(parts, max(1u, slots / units));
   return (parts + want - 1) / want * least;
 }
 
@@ -442,14 +447,14 @@ uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least) {
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled) {
   const uint64_t parts = (uint64_t(n) + kThreads - 1) / kThreads;
   const uint64_t units = tiled ? uint64_t(rows) / kAdapterTile + adapters + 7 : rows;
-  return (units >= 512 ? units : units * parts) + rows / (kCopyRows * kTileWaves) + 1;
+  return (units >= 1024 ? units : units * parts) + rows / (kCopyRows * kTileWaves) + 1;
 }
 
 hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
   if (p.rows == 0 || p.rank == 0 || p.rank > kAdapterMaxRank) return hipErrorInvalidValue;
   if (!p.vector_k) p.vector_rank = false;
   if (!tiled) {
-    p.split_cols = split_columns(p.n, p.rows, kThreads);
+    p.split_cols = split_columns(p.n, p.rows, kThreads, 512);
     p.splits = (p.n + p.split_cols - 1) / p.split_cols;
     const uint32_t blocks = p.rows * p.splits;
     if (p.vector_k && p.vector_rank) return go(&k_adapter_rows<true, true>, blocks, kThreads, p, stream);
@@ -457,7 +462,9 @@ hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
     return go(&k_adapter_rows<false, false>, blocks, kThreads, p, stream);
   }
   const uint32_t units = row_max_tiles(p.rows, p.adapters, kAdapterTile);
-  p.split_cols = split_columns(p.n, units, kTileWaves * kTileCols);
+  // blocks per CU by their LDS
+  const uint32_t slots = 256u * (p.rank <= 16 ? 4u : p.rank <= 32 ? 3u : p.rank <= 64 ? 2u : 1u);
+  p.split_cols = split_columns(p.n, units, kTileWaves * kTileCols, slots);
   p.splits = (p.n + p.split_cols - 1) / p.split_cols;
   p.tile_blocks = (units + 7) / 8 * 8 * p.splits;
   const uint32_t blocks = p.tile_blocks + (p.rows + kCopyRows * kTileWaves - 1) / (kCopyRows * kTileWaves);

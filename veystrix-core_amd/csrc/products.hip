@@ -34,9 +34,6 @@
 #ifndef VM_MEAN
 #define VM_MEAN 16
 #endif
-#ifndef VM_WIDEK
-#define VM_WIDEK 20
-#endif
 namespace vm {
 
 namespace {
@@ -238,11 +235,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows(ProductLaunch p) {
   float acc[kRowBatch] = {};
   uint4 xv, wv[kRowBatch];
   uint32_t xs = 0, ws[kRowBatch] = {};
+  const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_product_zeros);
+  VM_KEEP(zeros);
   auto load = [&](uint32_t at) {
     const bool in = at < p.k_bytes;
-    xv = ldg16(in ? x_row + at : reinterpret_cast<const uint8_t*>(g_product_zeros));
+    xv = ldg16(in ? x_row + at : zeros);
 #pragma unroll
-    for (int j = 0; j < kRowBatch; ++j) wv[j] = ldg16(in ? w_row[j] + at : reinterpret_cast<const uint8_t*>(g_product_zeros));
+    for (int j = 0; j < kRowBatch; ++j) wv[j] = ldg16(in ? w_row[j] + at : zeros);
     if constexpr (MX) {
       const uint32_t g = min(at, p.k_bytes - 1) / kMxGroup;
       xs = xs_row[g];
@@ -288,27 +287,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows(ProductLaunch p) {
 
 // ----------------------------------------------------------------- tiles ---
 
-// Stage J: the tile's rows, then the matrix rows, 128 bytes each; and the four scale bytes of each.  One LDS object
-// per stage, so that the compiler can tell the stage being read from the ones being filled.
+// Stage J: the tile's rows, then the matrix rows, 128 bytes each.  One LDS object per stage, so that the compiler can
+// tell the stage being read from the one being filled.
 template <int J, int ROWS>
 __device__ __forceinline__ uint8_t* tile_stage() {
   __shared__ uint4 buf[ROWS * kChunk / 16];
   return reinterpret_cast<uint8_t*>(buf);
 }
-template <int J, int ROWS>
-__device__ __forceinline__ uint32_t* tile_scales() {
-  __shared__ uint32_t buf[ROWS];
-  return buf;
-}
 
 // WM x WN waves of 16 RF rows by 64 matrix rows each, S stages.  WHOLE: K is whole chunks and scales are aligned.
 template <bool MX, bool SWIGLU, int OUT, int RF, int WM, int WN, int S, bool WHOLE>
-__global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   constexpr int kWaves = WM * WN;
   constexpr uint32_t kRows = 16 * RF * WM, kMatrix = 64 * WN;
   constexpr int kDmaX = kRows / 8 / kWaves;           // 1 KB loads (eight rows) per wave and chunk
   constexpr int kDmaW = kMatrix / 8 / kWaves;
-  static_assert(kDmaX * 8 * kWaves == kRows && kDmaW * 8 * kWaves == kMatrix, "whole 1 KB loads per wave");
+  static_assert(kDmaX * 8 * kWaves == kRows && kDmaW * 8 * kWaves == kMatrix, "whole loads per wave");
   constexpr uint32_t kCols = strip_cols<SWIGLU>() * WN;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, lm = lane & 15u, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -347,20 +341,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
     at[kDmaX + i] = (unit ^ tile_swz(r)) * 16u;
     src[kDmaX + i] = w + matrix_at(r) * p.w_stride + at[kDmaX + i];
   }
-  // scales: thread t serves rows t, t + threads, .. of the stage
-  constexpr uint32_t kThreads = 64 * kWaves, kScaleRows = MX ? (kRows + kMatrix + kThreads - 1) / kThreads : 1;
-  const uint8_t* scale_row[kScaleRows];
+  const uint32_t wm = wave % WM, wn = wave / WM;
+  // Scales: lane j holds the chunk's four bytes of the wave's row j and of its matrix row j; the lanes of a fragment
+  // fetch theirs from there, so that the scales take no LDS (with a few KB of it one block less fits a CU).
+  const uint8_t *xs_row = nullptr, *ws_row = nullptr;
   if constexpr (MX) {
-#pragma unroll
-    for (uint32_t i = 0; i < kScaleRows; ++i) {
-      const uint32_t r = min(i * kThreads + tid, kRows + kMatrix - 1);
-      const bool is_x = r < kRows;
-      const uint32_t pair = p.row_pair[row0 + min(r, rows - 1)];
-      scale_row[i] = is_x ? p.x_scales + static_cast<uint64_t>(pair / p.x_div) * p.x_scale_stride
-                          : p.w_scales + expert * p.w_scale_expert + matrix_at(r - kRows) * p.w_scale_stride;
-    }
+    const uint32_t pair = p.row_pair[row0 + min(wm * (16 * RF) + lane, rows - 1)];
+    xs_row = p.x_scales + static_cast<uint64_t>(pair / p.x_div) * p.x_scale_stride;
+    ws_row = p.w_scales + expert * p.w_scale_expert + matrix_at(wn * 64u + lane) * p.w_scale_stride;
   }
   const uint32_t chunks = (p.k_bytes + kChunk - 1) / kChunk, groups = p.k_bytes / kMxGroup;
+  const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_product_zeros);
+  if constexpr (!WHOLE) VM_KEEP(zeros);
   auto issue = [&](auto J, uint32_t c) {
     uint8_t* st = tile_stage<decltype(J)::value, kRows + kMatrix>();
 #pragma unroll
@@ -368,12 +360,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
       const uint32_t g = i < kDmaX ? wave * kDmaX + i : kRows / 8 + wave * kDmaW + (i - kDmaX);
       const uint8_t* s = src[i] + c * kChunk;
       if constexpr (!WHOLE)
-        if (c * kChunk + at[i] >= p.k_bytes) s = reinterpret_cast<const uint8_t*>(g_product_zeros);
+        if (c * kChunk + at[i] >= p.k_bytes) s = zeros;
       load_to_lds(s, st + g * 1024u);
     }
   };
 
-  const uint32_t wm = wave % WM, wn = wave / WM;
   const uint32_t s = tile_swz(lm);
   const uint32_t u0 = (kb ^ s) * 16u, u1 = ((4u | kb) ^ s) * 16u;
   const uint32_t x_base = (wm * (16 * RF) + lm) * kChunk, w_base = (kRows + wn * 64u + lm) * kChunk;
@@ -384,6 +375,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
   for (int i = 0; i < RF; ++i)
 #pragma unroll
     for (int f = 0; f < kStrip; ++f) acc[i][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  uint32_t held_x[S], held_w[S];   // the scale bytes of the stages
   // F fragments of stage J: all reads first, so that the second half's are under way while the first is multiplied
   auto compute = [&](auto J, auto frags) {
     constexpr int F = decltype(frags)::value;
@@ -391,11 +383,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
     uint32_t xs[F], ws[kStrip];
     uint4 xv[2][F], wv[2][kStrip];
     if constexpr (MX) {
-      const uint32_t* sc = tile_scales<decltype(J)::value, kRows + kMatrix>();
+      const auto from = [&](uint32_t j, uint32_t v) {
+        return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>((j * 16u + lm) * 4u), static_cast<int>(v)));
+      };
 #pragma unroll
-      for (int f = 0; f < kStrip; ++f) ws[f] = sc[kRows + wn * 64 + f * 16 + lm];
+      for (uint32_t f = 0; f < kStrip; ++f) ws[f] = from(f, held_w[decltype(J)::value]);
 #pragma unroll
-      for (int i = 0; i < F; ++i) xs[i] = sc[wm * (16 * RF) + i * 16 + lm];
+      for (uint32_t i = 0; i < F; ++i) xs[i] = from(i, held_x[decltype(J)::value]);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -422,11 +416,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
   // waits for all but the last S - 2 steps' of them; the scale loads stand before them and only add to what is in
   // flight.
   constexpr int kLoads = kDmaX + kDmaW;
-  uint32_t held[S][kScaleRows];   // the scale bytes on their way to a stage
   auto begin = [&](auto J, uint32_t c) {
     if constexpr (MX) {
-#pragma unroll
-      for (uint32_t i = 0; i < kScaleRows; ++i) held[decltype(J)::value][i] = chunk_scales<WHOLE>(scale_row[i], c, groups);
+      held_x[decltype(J)::value] = chunk_scales<WHOLE>(xs_row, c, groups);
+      held_w[decltype(J)::value] = chunk_scales<WHOLE>(ws_row, c, groups);
     }
     __builtin_amdgcn_sched_barrier(0);
     issue(J, c);
@@ -438,17 +431,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_tiles(ProductLaunch p) {
       constexpr int j = decltype(J)::value;
       if (c + j >= chunks) return;
       wait_vm<(S - 2) * kLoads>();   // this wave's loads of stage j have landed
-      if constexpr (MX) {
-#pragma unroll
-        for (uint32_t i = 0; i < kScaleRows; ++i)
-          if (i * kThreads + tid < kRows + kMatrix) tile_scales<j, kRows + kMatrix>()[i * kThreads + tid] = held[j][i];
-      }
-      wait_lgkm0();                  // its reads of the stage before and its scales are done
+      wait_lgkm0();                  // its reads of the stage before are done
       bare_barrier();
       begin(std::integral_constant<int, (j + S - 1) % S>{}, min(c + j + S - 1, chunks - 1));
-      if (live > RF / 2) compute(J, std::integral_constant<int, RF>{});
-      else if (live > RF / 4) compute(J, std::integral_constant<int, (RF + 1) / 2>{});
-      else if (live > 0) compute(J, std::integral_constant<int, (RF + 3) / 4>{});
+      if (live == RF) compute(J, std::integral_constant<int, RF>{});
+      else if (RF > 3 && live == 3) compute(J, std::integral_constant<int, RF < 3 ? RF : 3>{});
+      else if (RF > 2 && live == 2) compute(J, std::integral_constant<int, RF < 2 ? RF : 2>{});
+      else if (live > 0) compute(J, std::integral_constant<int, 1>{});
       __builtin_amdgcn_sched_barrier(0);
     });
   }
@@ -502,10 +491,14 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
   using I4 = std::integral_constant<int, 4>;
-  // 256 matrix rows per block read a tile's rows half as often as 128, but fewer such blocks fit a CU: for enough
-  // blocks of a long K
+  // 256 matrix rows per block read a tile's rows half as often as 128 and twice as many tile rows per wave reuse each
+  // matrix operand, but fewer blocks run: once they fill the chip four times over, if the product of a few rows is not
+  // a short one, too.  64-row tiles, 256 and 128: 2048 tokens MX 2560 -> 2 x 640, ten of 512 experts, 364 and 409 us,
+  // 8192 tokens bf16 2048 -> 2 x 512 616 and 666; four of 64 experts, 8192 tokens, 1024 -> 2 x 256 62 and 60, four of
+  // 20, 2048 tokens, 1024 -> 2 x 512 42 and 36.
   const uint32_t slices = (p.n + 4 * strip_cols<SWIGLU>() - 1) / (4 * strip_cols<SWIGLU>());
-  const bool wide = uint64_t(tiles) * slices >= 512 && (p.k_bytes + kChunk - 1) / kChunk >= VM_WIDEK;
+  const uint32_t chunks = (p.k_bytes + kChunk - 1) / kChunk;
+  const bool wide = uint64_t(tiles) * slices >= 2048 && chunks * tile_rows >= 256;
   if (tile_rows == 32) return wide ? tiles_go(I2{}, I1{}, I4{}) : tiles_go(I2{}, I1{}, I2{});
   return wide ? tiles_go(I4{}, I1{}, I4{}) : tiles_go(I2{}, I2{}, I2{});
 }

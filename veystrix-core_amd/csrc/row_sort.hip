@@ -39,8 +39,9 @@ __device__ __forceinline__ uint32_t scan_1024(uint32_t v, uint32_t* s_wave) {
   return before + sum - v;
 }
 
-// Adds one to a group's count for every lane with a group and returns the count before the lane's own.  Lanes of one
-// group, as in runs of rows of one request, take one addition together: 64 to one address come one after the other.
+// Adds one to a group's count for every lane with a group; with RANK returns the count before the lane's own.  Lanes of
+// one group, as in runs of rows of one request, take one addition together: 64 to one address come one after the other.
+template <bool RANK>
 __device__ __forceinline__ uint32_t count_one(uint32_t* counts, uint32_t g, uint32_t groups) {
   const uint64_t live = __ballot(g < groups);
   if (live == 0) return 0;
@@ -50,10 +51,13 @@ __device__ __forceinline__ uint32_t count_one(uint32_t* counts, uint32_t g, uint
   if (__ballot(g < groups && g != one) == 0) {
     uint32_t first = 0;
     if (lane == leader) first = atomicAdd(&counts[one], static_cast<uint32_t>(__popcll(live)));
+    if constexpr (!RANK) return 0;
     first = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), leader));
     return first + static_cast<uint32_t>(__popcll(live & ((1ull << lane) - 1)));
   }
-  return g < groups ? atomicAdd(&counts[g], 1u) : 0u;
+  uint32_t rank = 0;
+  if (g < groups) rank = atomicAdd(&counts[g], 1u);
+  return RANK ? rank : 0;
 }
 
 __global__ __launch_bounds__(kThreads) void k_row_count(RowSortLaunch p) {
@@ -65,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void k_row_count(RowSortLaunch p) {
   for (uint32_t j = 0; j < kPerThread; ++j) {
     const uint32_t i = base + j * kThreads + t;
     const uint32_t g = i < p.rows ? static_cast<uint32_t>(p.ids[i]) : p.groups;
-    count_one(s_count, g, p.groups);
+    count_one<false>(s_count, g, p.groups);
   }
   __syncthreads();
   if (t < p.groups) p.block_counts[static_cast<size_t>(blockIdx.x) * p.groups + t] = s_count[t];
@@ -84,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void k_row_place(RowSortLaunch p) {
   for (uint32_t j = 0; j < kPerThread; ++j) {
     const uint32_t i = first + j * kThreads + t;
     g[j] = i < last ? static_cast<uint32_t>(p.ids[i]) : p.groups;
-    rank[j] = count_one(s_own, g[j], p.groups);
+    rank[j] = count_one<true>(s_own, g[j], p.groups);
   }
   uint32_t before = 0, total = 0;
   if constexpr (COUNTED) {
@@ -98,10 +102,10 @@ __global__ __launch_bounds__(kThreads) void k_row_place(RowSortLaunch p) {
     }
   } else {
 #pragma unroll 4
-    for (uint32_t i = t; i < first; i += kThreads) count_one(s_before, static_cast<uint32_t>(p.ids[i]), p.groups);
+    for (uint32_t i = t; i < first; i += kThreads) count_one<false>(s_before, static_cast<uint32_t>(p.ids[i]), p.groups);
 #pragma unroll 4
     for (uint32_t i = first + kBlockRows + t; i < p.rows; i += kThreads)
-      count_one(s_after, static_cast<uint32_t>(p.ids[i]), p.groups);
+      count_one<false>(s_after, static_cast<uint32_t>(p.ids[i]), p.groups);
   }
   __syncthreads();
   if constexpr (!COUNTED) {

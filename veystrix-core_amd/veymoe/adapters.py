@@ -53,7 +53,7 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
             raise ValueError(f"scales must be contiguous float32 of shape ({adapters},) on {x.device}")
         scales_at = scales.data_ptr()
     if out is None:
-        out = base.new_empty(shape)
+        out = torch.empty_like(base)
     elif out.shape != shape:
         raise ValueError("out must have base's shape")
     out_at, out_stride = row_span("out", out, _BF16, index)

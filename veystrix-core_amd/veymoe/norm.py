@@ -83,7 +83,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
             raise ValueError("residual must have x's shape")
         r_at, r_stride = row_span("residual", residual, dtype, index)
         if residual_out is None:
-            residual_out = x.new_empty(shape)
+            residual_out = torch.empty_like(x)
         elif residual_out.shape != shape:
             raise ValueError("residual_out must have x's shape")
         s_at, s_stride = row_span("residual_out", residual_out, dtype, index)
@@ -97,7 +97,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
         y = mx_empty(shape, x.device)
         values_at, scales_at = y[0].data_ptr(), y[1].data_ptr()
     else:
-        y = x.new_empty(shape) if out is None else out
+        y = torch.empty_like(x) if out is None else out
         if y.shape != shape:
             raise ValueError("out must have x's shape")
         y_at, y_stride = row_span("out", y, dtype, index)
