@@ -55,19 +55,26 @@ __device__ __forceinline__ void load8(const void* row, uint32_t at, uint32_t wid
   }
 }
 
+// `past`: non-temporal, past the caches.
 template <class A, bool VEC>
-__device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t width, const float v[8]) {
+__device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t width, const float v[8], bool past = false) {
   if constexpr (VEC) {
     if (at >= width) return;
+    const auto put = [&](vm_u32x4* dst, vm_u32x4 w) {
+      if (past) __builtin_nontemporal_store(w, dst);
+      else *dst = w;
+    };
+    vm_u32x4* dst = reinterpret_cast<vm_u32x4*>(static_cast<uint8_t*>(row) + static_cast<size_t>(at) * A::kBytes);
     if constexpr (A::kBytes == 2) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(v[2 * j]) | (f32_to_bf16(v[2 * j + 1]) << 16);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+      put(dst, vm_u32x4{w[0], w[1], w[2], w[3]});
     } else {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(row) + at);
-      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        put(dst + j, vm_u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                              __float_as_uint(v[4 * j + 3])});
     }
   } else {
 #pragma unroll
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   if (p.sum_out != nullptr) {
     uint8_t* s = const_cast<uint8_t*>(row_of(p.sum_out, p.sum_stride));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store8<A, VEC>(s, (i * TPR + t) * 8u, p.width, h[i]);
+    for (int i = 0; i < NV; ++i) store8<A, VEC>(s, (i * TPR + t) * 8u, p.width, h[i], p.sum_past);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -189,7 +196,12 @@ hipError_t norm_dispatch(const NormLaunch& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_norm(const NormLaunch& p, hipStream_t stream) {
+// The sum of a large call is next read behind the whole block that the norm feeds: stored past the caches it leaves
+// them to the normed rows, which are read at once (8192 x 2560, MX out: FIG).
+constexpr uint64_t kSumPast = 16ull << 20;
+
+hipError_t launch_norm(NormLaunch p, hipStream_t stream) {
+  p.sum_past = uint64_t(p.rows) * p.width * (p.act_dtype == 0 ? 2 : 4) >= kSumPast;
   if (p.rows == 0 || p.width == 0 || p.width > kNormMaxWidth) return hipErrorInvalidValue;
   return p.act_dtype == 0 ? norm_dispatch<ActBF16>(p, stream) : norm_dispatch<ActF32>(p, stream);
 }

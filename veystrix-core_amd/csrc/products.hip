@@ -28,12 +28,6 @@
 #include "vm_internal.h"
 #include "vm_mx.h"
 
-#ifndef VM_ROWS
-#define VM_ROWS 160
-#endif
-#ifndef VM_MEAN
-#define VM_MEAN 16
-#endif
 namespace vm {
 
 namespace {
@@ -207,7 +201,7 @@ __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_floa
 
 // One routed row per block and 8 WAVES matrix rows, eight per wave: a wave reads a kilobyte of one matrix row at a
 // time, the row's unit of the lane stays in registers for all eight.
-template <bool MX, bool SWIGLU, int OUT, int WAVES>
+template <bool MX, bool SWIGLU, int OUT, int WAVES, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES) void k_rows(ProductLaunch p) {
   constexpr uint32_t kMatrix = kRowBatch * WAVES, kCols = SWIGLU ? kMatrix / 2 : kMatrix;
   static_assert(OUT == kOutBf16 || kCols == kMxGroup, "a block's outputs are one group");
@@ -241,7 +235,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_rows(ProductLaunch p) {
     const bool in = at < p.k_bytes;
     xv = ldg16(in ? x_row + at : zeros);
 #pragma unroll
-    for (int j = 0; j < kRowBatch; ++j) wv[j] = ldg16(in ? w_row[j] + at : zeros);
+    for (int j = 0; j < kRowBatch; ++j) {
+      const uint8_t* from = in ? w_row[j] + at : zeros;
+      wv[j] = ONCE ? ldg16_nt(from) : ldg16(from);
+    }
     if constexpr (MX) {
       const uint32_t g = min(at, p.k_bytes - 1) / kMxGroup;
       xs = xs_row[g];
@@ -295,8 +292,9 @@ __device__ __forceinline__ uint8_t* tile_stage() {
   return reinterpret_cast<uint8_t*>(buf);
 }
 
-// WM x WN waves of 16 RF rows by 64 matrix rows each, S stages.  WHOLE: K is whole chunks and scales are aligned.
-template <bool MX, bool SWIGLU, int OUT, int RF, int WM, int WN, int S, bool WHOLE>
+// WM x WN waves of 16 RF rows by 64 matrix rows each.  WHOLE: K is whole chunks and scales are aligned.  ONCE: the
+// matrices are read once (ProductLaunch::once).
+template <bool MX, bool SWIGLU, int OUT, int RF, int WM, int WN, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   constexpr int kWaves = WM * WN;
   constexpr uint32_t kRows = 16 * RF * WM, kMatrix = 64 * WN;
@@ -361,7 +359,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
       const uint8_t* s = src[i] + c * kChunk;
       if constexpr (!WHOLE)
         if (c * kChunk + at[i] >= p.k_bytes) s = zeros;
-      load_to_lds(s, st + g * 1024u);
+      if (i < kDmaX) load_to_lds(s, st + g * 1024u);
+      else load_to_lds<ONCE>(s, st + g * 1024u);
     }
   };
 
@@ -375,7 +374,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   for (int i = 0; i < RF; ++i)
 #pragma unroll
     for (int f = 0; f < kStrip; ++f) acc[i][f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  uint32_t held_x[S], held_w[S];   // the scale bytes of the stages
+  uint32_t held_x[2], held_w[2];   // the scale bytes of the stages
   // F fragments of stage J: all reads first, so that the second half's are under way while the first is multiplied
   auto compute = [&](auto J, auto frags) {
     constexpr int F = decltype(frags)::value;
@@ -411,11 +410,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
       }
   };
 
-  // Ring of S stages: stage c % S is multiplied while the next S - 1 chunks are in flight.  Chunks behind the last one
-  // are loaded from its place again (their stages are never read), so that every step issues the same DMA loads and
-  // waits for all but the last S - 2 steps' of them; the scale loads stand before them and only add to what is in
-  // flight.
-  constexpr int kLoads = kDmaX + kDmaW;
+  // Two stages: one is multiplied while the next chunk is on its way to the other (behind the last chunk that one again,
+  // which is not read).  More stages were slower than the second block per CU that their LDS costs.
   auto begin = [&](auto J, uint32_t c) {
     if constexpr (MX) {
       held_x[decltype(J)::value] = chunk_scales<WHOLE>(xs_row, c, groups);
@@ -425,15 +421,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
     issue(J, c);
     __builtin_amdgcn_sched_barrier(0);
   };
-  unroll<0, S - 1>([&](auto J) { begin(J, min(static_cast<uint32_t>(decltype(J)::value), chunks - 1)); });
-  for (uint32_t c = 0; c < chunks; c += S) {
-    unroll<0, S>([&](auto J) {
+  begin(std::integral_constant<int, 0>{}, 0);
+  for (uint32_t c = 0; c < chunks; c += 2) {
+    unroll<0, 2>([&](auto J) {
       constexpr int j = decltype(J)::value;
       if (c + j >= chunks) return;
-      wait_vm<(S - 2) * kLoads>();   // this wave's loads of stage j have landed
-      wait_lgkm0();                  // its reads of the stage before are done
+      wait_vm<0>();    // this wave's loads of the stage have landed
+      wait_lgkm0();    // its reads of the other stage are done
       bare_barrier();
-      begin(std::integral_constant<int, (j + S - 1) % S>{}, min(c + j + S - 1, chunks - 1));
+      begin(std::integral_constant<int, 1 - j>{}, min(c + j + 1, chunks - 1));
       if (live == RF) compute(J, std::integral_constant<int, RF>{});
       else if (RF > 3 && live == 3) compute(J, std::integral_constant<int, RF < 3 ? RF : 3>{});
       else if (RF > 2 && live == 2) compute(J, std::integral_constant<int, RF < 2 ? RF : 2>{});
@@ -476,7 +472,9 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
   if (tile_rows == 0) {
     constexpr int kWaves = OUT == kOutMx ? 8 : 4;
     constexpr uint32_t cols = kRowBatch * kWaves / (SWIGLU ? 2 : 1);
-    return go(&k_rows<MX, SWIGLU, OUT, kWaves>, (p.n + cols - 1) / cols * p.rows, 64 * kWaves, p, stream);
+    const uint32_t blocks = (p.n + cols - 1) / cols * p.rows;
+    return p.once ? go(&k_rows<MX, SWIGLU, OUT, kWaves, true>, blocks, 64 * kWaves, p, stream)
+                  : go(&k_rows<MX, SWIGLU, OUT, kWaves, false>, blocks, 64 * kWaves, p, stream);
   }
   const uint32_t tiles = (row_max_tiles(p.rows, p.experts, tile_rows) + 7) / 8 * 8;
   const bool whole = p.k_bytes % kChunk == 0 && (!MX || scales_aligned(p));
@@ -485,8 +483,10 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
     constexpr uint32_t kWaves = WM * WN, cols = strip_cols<SWIGLU>() * WN;
     p.tile_blocks = (p.n + cols - 1) / cols * tiles;
     const uint32_t blocks = p.tile_blocks + (p.rows + kWaves * kZeroRows - 1) / (kWaves * kZeroRows);
-    return whole ? go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, 2, true>, blocks, 64 * kWaves, p, stream)
-                 : go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, 2, false>, blocks, 64 * kWaves, p, stream);
+    if (!whole) return go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, false, false>, blocks, 64 * kWaves, p, stream);
+    if constexpr (WN == 4)
+      if (p.once) return go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, true, true>, blocks, 64 * kWaves, p, stream);
+    return go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, true, false>, blocks, 64 * kWaves, p, stream);
   };
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
@@ -505,9 +505,26 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
 
 }  // namespace
 
+// Rows up to which a call runs them one by one.  An expert met twice is then read twice, which sixteen tokens of ten
+// experts seldom do: 80 rows of 512 experts 58 us and 63 in sorted tiles, 128 of 64 experts 14.7 and 17.5, but 320 of
+// 512 with skewed popularity 177 and 116.
+constexpr uint32_t kOneByOne = 160;
+// Mean rows per expert from which tiles hold 64 rows rather than 32: ten of 512 experts, 2048 -> 2 x 512, 512 / 1024 /
+// 2048 tokens (10 / 20 / 40 rows) 363 / 373 / 390 us with 64 and 363 / 395 / 433 with 32.
+constexpr uint32_t kTallMean = 16;
+
 uint32_t product_tile_rows(uint32_t rows, uint32_t experts) {
-  if (rows <= VM_ROWS) return 0;
-  return rows / experts < VM_MEAN ? 32u : 64u;
+  if (rows <= kOneByOne) return 0;
+  return rows / experts < kTallMean ? 32u : 64u;
+}
+
+// Matrices that outgrow the 256 MB Infinity Cache and are mostly read by one tile stream past the caches: 512 tokens,
+// ten of 512 experts, 2048 -> 2 x 512 364 to 336 us, 2048 tokens MX 2560 -> 2 x 640 363 to 356, eight tokens 58 to 55.
+// Shared by several tiles or held by that cache they must not: 8192 tokens 613 to 941, 333 tokens of four of 64
+// experts, 1024 -> 2 x 256, 20 to 23.
+bool product_once(const ProductLaunch& p, uint32_t tile_rows) {
+  const uint64_t bytes = uint64_t(p.experts) * p.n * (p.swiglu ? 2 : 1) * p.k_bytes;
+  return bytes > (256ull << 20) && (tile_rows == 0 || p.rows / p.experts <= 48);
 }
 
 uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu) {
@@ -516,7 +533,8 @@ uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t ti
   return units * strips + rows / (2 * kZeroRows) + 1;
 }
 
-hipError_t launch_products(const ProductLaunch& p, uint32_t tile_rows, hipStream_t stream) {
+hipError_t launch_products(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) {
+  p.once = product_once(p, tile_rows);
   if (p.values != nullptr && !p.swiglu) return hipErrorInvalidValue;
   if (p.mx) {
     if (!p.swiglu) return products_go<true, false, kOutBf16>(p, tile_rows, stream);

@@ -15,9 +15,11 @@ constexpr uint32_t kChunk = 128;          // bytes of a row per step
 // 4 + lane / 16) then spreads over all 64 banks in every lane grouping of the read.
 __device__ __forceinline__ uint32_t tile_swz(uint32_t r) { return ((r >> 1) & 2u) | ((r << 1) & 4u); }
 
-// One kilobyte from the lanes' addresses to LDS, lane j's 16 bytes at dst + 16 j; dst is the same in all lanes.
+// One kilobyte from the lanes' addresses to LDS, lane j's 16 bytes at dst + 16 j; dst is the same in all lanes.  ONCE:
+// non-temporal, for data that is read once.
+template <bool ONCE = false>
 __device__ __forceinline__ void load_to_lds(const void* src, uint8_t* dst) {
-  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, ONCE ? 2 : 0);
 }
 
 // s_waitcnt for a vector memory count of N, or the LDS count at zero, the others left alone

@@ -436,9 +436,10 @@ struct NormLaunch {
   float eps;
   int act_dtype, weight_dtype;
   bool vector;                 // every row and the weight 16-byte aligned, width a multiple of 8
+  bool sum_past;               // sum_out past the caches (set by launch_norm)
 };
 
-hipError_t launch_norm(const NormLaunch& p, hipStream_t stream);
+hipError_t launch_norm(NormLaunch p, hipStream_t stream);
 
 // -------------------------------------------------------------- row sort --
 // Rows sorted by group (row_sort.hip).
@@ -481,6 +482,7 @@ struct ProductLaunch {
   uint32_t tile_blocks;        // blocks of the grid that serve tiles (set by launch_products)
   bool mx, swiglu;
   bool out_aligned;            // out is 16-byte aligned
+  bool once;                   // the matrices stream past the caches (set by launch_products)
 };
 
 // How a call of this many routed rows runs: 0 its rows one by one, or rows per
@@ -488,7 +490,7 @@ struct ProductLaunch {
 uint32_t product_tile_rows(uint32_t rows, uint32_t experts);
 // An upper bound of a call's blocks.
 uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu);
-hipError_t launch_products(const ProductLaunch& p, uint32_t tile_rows, hipStream_t stream);
+hipError_t launch_products(ProductLaunch p, uint32_t tile_rows, hipStream_t stream);
 
 // -------------------------------------------------------------- adapters --
 // Low-rank adapters added to a projection's output (adapters.hip).  Strides in
