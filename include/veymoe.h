@@ -483,7 +483,7 @@ int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* s
 uint64_t vm_grouped_matmul_workspace(uint32_t rows, uint32_t experts);
 int vm_grouped_matmul(const VmProductArgs* args, void* stream);
 
-uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t adapters);
+uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t rank, uint32_t adapters);
 int vm_add_adapters(const VmAdapterArgs* args, void* stream);
 
 /* out[t, h] = sum_j expert_outputs[t, j, h] * scores[t, j] in fp32, written in

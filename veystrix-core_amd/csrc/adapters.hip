@@ -444,6 +444,10 @@ uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least, uint32_t slot
 
 }  // namespace
 
+// Calls whose rank sums are few run one block per row and column split, without a sort: 100 / 200 rows of rank 16 11.2
+// us against 15.4 in sorted tiles, 100 rows of rank 64 18.9 against 21.1, 200 rows of it 28.4 against 22.2 (2560 wide).
+bool adapter_tiled(uint32_t rows, uint32_t rank) { return rows > 512 || uint64_t(rows) * rank > 6400; }
+
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled) {
   const uint64_t parts = (uint64_t(n) + kThreads - 1) / kThreads;
   const uint64_t units = tiled ? uint64_t(rows) / kAdapterTile + adapters + 7 : rows;
@@ -454,7 +458,7 @@ hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
   if (p.rows == 0 || p.rank == 0 || p.rank > kAdapterMaxRank) return hipErrorInvalidValue;
   if (!p.vector_k) p.vector_rank = false;
   if (!tiled) {
-    p.split_cols = split_columns(p.n, p.rows, kThreads, 512);
+    p.split_cols = split_columns(p.n, p.rows, kThreads, 256);
     p.splits = (p.n + p.split_cols - 1) / p.split_cols;
     const uint32_t blocks = p.rows * p.splits;
     if (p.vector_k && p.vector_rank) return go(&k_adapter_rows<true, true>, blocks, kThreads, p, stream);

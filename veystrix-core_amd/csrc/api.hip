@@ -1695,8 +1695,8 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
 
 // ----------------------------------------------------------- adapters ---
 
-uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t adapters) {
-  return rows <= vm::kAdapterRows ? 0 : row_sort_ws(rows, adapters, vm::kAdapterTile).total;
+uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t rank, uint32_t adapters) {
+  return adapters == 0 || !vm::adapter_tiled(rows, rank) ? 0 : row_sort_ws(rows, adapters, vm::kAdapterTile).total;
 }
 
 int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
@@ -1714,7 +1714,7 @@ int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
   if (a->rows > 1 && a->out_stride < a->n) return fail(VM_EINVAL, "the row stride of out must be at least n");
   if (a->out == a->base && a->out_stride != a->base_stride && a->rows > 1)
     return fail(VM_EINVAL, "in place, base and out must have one stride");
-  const bool tiled = a->rows > vm::kAdapterRows;
+  const bool tiled = vm::adapter_tiled(a->rows, a->rank);
   vm::AdapterLaunch p{};
   p.base = static_cast<const uint16_t*>(a->base);
   p.x = static_cast<const uint16_t*>(a->x);

@@ -13,7 +13,7 @@
 //   * few rows, or rows wider than a wave's registers: one block of 256 threads per row, so that a row's loads are one
 //     round trip.
 // Rows that are not 16-byte aligned, or whose width is not a multiple of eight, take the same code with element loads
-// and stores.
+// and stores, their values spread over the row's threads unless MX groups have to lie together.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
@@ -27,12 +27,17 @@ namespace {
 
 constexpr int kNormThreads = 256;
 
-// Eight consecutive values from element `at` of a row; those at `width` and behind it are zero.
-template <class A, bool VEC>
-__device__ __forceinline__ void load8(const void* row, uint32_t at, uint32_t width, float v[8]) {
+// How a thread's eight values of a step lie in a row: consecutive ones moved as 16-byte units or one by one, or spread
+// over the row's threads, so that those moved one by one are neighbours across lanes (3000 rows of 3333 bf16 values,
+// SPREADFIG).
+enum : int { kUnits = 0, kOnes = 1, kSpread = 2 };
+
+// The eight values of the step at element `at`; those at `width` and behind it are zero.
+template <class A, int LIE>
+__device__ __forceinline__ void load8(const void* row, uint32_t at, uint32_t step, uint32_t width, float v[8]) {
+  if constexpr (LIE == kUnits) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-  if constexpr (VEC) {
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
     if (at >= width) return;
     const uint8_t* src = static_cast<const uint8_t*>(row) + static_cast<size_t>(at) * A::kBytes;
     const uint4 a = ldg16(src);
@@ -50,41 +55,37 @@ __device__ __forceinline__ void load8(const void* row, uint32_t at, uint32_t wid
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (at + j < width) v[j] = A::load(row, at + j);
+    for (int j = 0; j < 8; ++j) {  // no branch: each would wait for its own load
+      const uint32_t i = at + j * step;
+      const float value = A::from_bits(A::load_bits(row, min(i, width - 1)));
+      v[j] = i < width ? value : 0.0f;
+    }
   }
 }
 
-// `past`: non-temporal, past the caches.
-template <class A, bool VEC>
-__device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t width, const float v[8], bool past = false) {
-  if constexpr (VEC) {
+template <class A, int LIE>
+__device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t step, uint32_t width, const float v[8]) {
+  if constexpr (LIE == kUnits) {
     if (at >= width) return;
-    const auto put = [&](vm_u32x4* dst, vm_u32x4 w) {
-      if (past) __builtin_nontemporal_store(w, dst);
-      else *dst = w;
-    };
-    vm_u32x4* dst = reinterpret_cast<vm_u32x4*>(static_cast<uint8_t*>(row) + static_cast<size_t>(at) * A::kBytes);
     if constexpr (A::kBytes == 2) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16(v[2 * j]) | (f32_to_bf16(v[2 * j + 1]) << 16);
-      put(dst, vm_u32x4{w[0], w[1], w[2], w[3]});
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + at) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        put(dst + j, vm_u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
-                              __float_as_uint(v[4 * j + 3])});
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(row) + at);
+      dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+      dst[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (at + j < width) A::store(row, at + j, v[j]);
+      if (at + j * step < width) A::store(row, at + j * step, v[j]);
   }
 }
 
 // TPR threads per row (64 or 256), up to NV steps of eight values per thread.
-template <class A, int TPR, int NV, bool VEC>
+template <class A, int TPR, int NV, int LIE>
 __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   const uint32_t t = threadIdx.x % TPR;
   const uint32_t row = blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR;
@@ -92,16 +93,19 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   const auto row_of = [&](const void* base, uint64_t stride) {
     return static_cast<const uint8_t*>(base) + static_cast<uint64_t>(row) * stride * A::kBytes;
   };
+  // element of the thread's first value in step i, and between its values
+  constexpr uint32_t kStep = LIE == kSpread ? TPR : 1;
+  const auto at = [&](int i) { return LIE == kSpread ? i * TPR * 8u + t : (i * TPR + t) * 8u; };
   float h[NV][8];
   const uint8_t* x = row_of(p.x, p.x_stride);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) load8<A, VEC>(x, (i * TPR + t) * 8u, p.width, h[i]);
+  for (int i = 0; i < NV; ++i) load8<A, LIE>(x, at(i), kStep, p.width, h[i]);
   if (p.residual != nullptr) {
     const uint8_t* r = row_of(p.residual, p.residual_stride);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float v[8];
-      load8<A, VEC>(r, (i * TPR + t) * 8u, p.width, v);
+      load8<A, LIE>(r, at(i), kStep, p.width, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[i][j] += v[j];
     }
@@ -127,30 +131,30 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   if (p.sum_out != nullptr) {
     uint8_t* s = const_cast<uint8_t*>(row_of(p.sum_out, p.sum_stride));
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store8<A, VEC>(s, (i * TPR + t) * 8u, p.width, h[i], p.sum_past);
+    for (int i = 0; i < NV; ++i) store8<A, LIE>(s, at(i), kStep, p.width, h[i]);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const uint32_t at = (i * TPR + t) * 8u;
     if (p.weight != nullptr) {
       float g[8];
-      if (p.weight_dtype == 0) load8<ActBF16, VEC>(p.weight, at, p.width, g);
-      else load8<ActF32, VEC>(p.weight, at, p.width, g);
+      if (p.weight_dtype == 0) load8<ActBF16, LIE>(p.weight, at(i), kStep, p.width, g);
+      else load8<ActF32, LIE>(p.weight, at(i), kStep, p.width, g);
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * scale * (p.one_centered ? g[j] : 1.0f + g[j]);
     }
     if (p.values == nullptr) {
-      store8<A, VEC>(const_cast<uint8_t*>(row_of(p.out, p.out_stride)), at, p.width, h[i]);
+      store8<A, LIE>(const_cast<uint8_t*>(row_of(p.out, p.out_stride)), at(i), kStep, p.width, h[i]);
       continue;
     }
+    if constexpr (LIE == kSpread) continue;  // MX rows need a group's values side by side
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(h[i][j]));
     m = max(m, dpp_u<kDppQuadXor1>(m));
     m = max(m, dpp_u<kDppQuadXor2>(m));
     const uint32_t e = mx_scale(m);
-    if (at < p.width) {  // the width is whole groups, so a lane's eight values are all in it
-      const uint64_t first = static_cast<uint64_t>(row) * p.width + at;
+    if (at(i) < p.width) {  // the width is whole groups, so a lane's eight values are all in it
+      const uint64_t first = static_cast<uint64_t>(row) * p.width + at(i);
       *reinterpret_cast<uint2*>(p.values + first) =
           make_uint2(mx_pack4(h[i][0], h[i][1], h[i][2], h[i][3], e), mx_pack4(h[i][4], h[i][5], h[i][6], h[i][7], e));
       if (t % 4 == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e);
@@ -162,7 +166,7 @@ template <class A, int TPR, int NV>
 hipError_t norm_go(const NormLaunch& p, hipStream_t stream) {
   const uint32_t per = kNormThreads / TPR;
   const dim3 grid((p.rows + per - 1) / per);
-  auto kernel = p.vector ? &k_norm<A, TPR, NV, true> : &k_norm<A, TPR, NV, false>;
+  auto kernel = p.vector ? &k_norm<A, TPR, NV, kUnits> : p.values != nullptr ? &k_norm<A, TPR, NV, kOnes> : &k_norm<A, TPR, NV, kSpread>;
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("norm", &start, &stop))
     hipExtLaunchKernelGGL(kernel, grid, dim3(kNormThreads), 0, stream, start, stop, 0, p);
@@ -196,12 +200,7 @@ hipError_t norm_dispatch(const NormLaunch& p, hipStream_t stream) {
 
 }  // namespace
 
-// The sum of a large call is next read behind the whole block that the norm feeds: stored past the caches it leaves
-// them to the normed rows, which are read at once (8192 x 2560, MX out: FIG).
-constexpr uint64_t kSumPast = 16ull << 20;
-
-hipError_t launch_norm(NormLaunch p, hipStream_t stream) {
-  p.sum_past = uint64_t(p.rows) * p.width * (p.act_dtype == 0 ? 2 : 4) >= kSumPast;
+hipError_t launch_norm(const NormLaunch& p, hipStream_t stream) {
   if (p.rows == 0 || p.width == 0 || p.width > kNormMaxWidth) return hipErrorInvalidValue;
   return p.act_dtype == 0 ? norm_dispatch<ActBF16>(p, stream) : norm_dispatch<ActF32>(p, stream);
 }

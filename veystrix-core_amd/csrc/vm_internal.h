@@ -436,10 +436,9 @@ struct NormLaunch {
   float eps;
   int act_dtype, weight_dtype;
   bool vector;                 // every row and the weight 16-byte aligned, width a multiple of 8
-  bool sum_past;               // sum_out past the caches (set by launch_norm)
 };
 
-hipError_t launch_norm(NormLaunch p, hipStream_t stream);
+hipError_t launch_norm(const NormLaunch& p, hipStream_t stream);
 
 // -------------------------------------------------------------- row sort --
 // Rows sorted by group (row_sort.hip).
@@ -515,8 +514,8 @@ struct AdapterLaunch {
   bool vector_n;               // base and out: rows of whole aligned 16-byte units
 };
 
-// Rows up to which a call runs one block per row and column split, without a sort.
-constexpr uint32_t kAdapterRows = 128;
+// Whether a call runs in sorted tiles rather than one block per row and column split.
+bool adapter_tiled(uint32_t rows, uint32_t rank);
 // An upper bound of a call's blocks.
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled);
 hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream);

@@ -241,7 +241,7 @@ SIGNATURES = {
     "vm_mx_quantize": (ctypes.c_int, [_vp, _c_u64, _vp, _vp, _c_u32, _c_u32, _c_u32, _vp]),
     "vm_grouped_matmul_workspace": (_c_u64, [_c_u32, _c_u32]),
     "vm_grouped_matmul": (ctypes.c_int, [ctypes.POINTER(VmProductArgs), _vp]),
-    "vm_add_adapters_workspace": (_c_u64, [_c_u32, _c_u32]),
+    "vm_add_adapters_workspace": (_c_u64, [_c_u32, _c_u32, _c_u32]),
     "vm_add_adapters": (ctypes.c_int, [ctypes.POINTER(VmAdapterArgs), _vp]),
     "vm_pool_stage": (ctypes.c_int, [_vp, _c_u64, _c_u64, _c_u64, _vp, _c_u64, _c_u64, _c_u64,
                                      ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),

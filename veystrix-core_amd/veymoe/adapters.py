@@ -61,7 +61,7 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     if rows == 0 or n == 0:
         return out
     lib = _lib.lib()
-    nbytes = lib.vm_add_adapters_workspace(rows, adapters)
+    nbytes = lib.vm_add_adapters_workspace(rows, rank, adapters)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     p = _lib.VmAdapterArgs(base_at, x_at, a_at, b_at, scales_at, ids.data_ptr(), out_at,
                            ws.data_ptr() if nbytes else None, nbytes, base_stride, x_stride, out_stride, rows, k, n,
