@@ -18,6 +18,8 @@
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "vm_internal.h"
 #include "vm_mx.h"
 
@@ -28,8 +30,8 @@ namespace {
 constexpr int kNormThreads = 256;
 
 // How a thread's eight values of a step lie in a row: consecutive ones moved as 16-byte units or one by one, or spread
-// over the row's threads, so that those moved one by one are neighbours across lanes (3000 rows of 3333 bf16 values,
-// SPREADFIG).
+// over the row's threads, so that those moved one by one are neighbours across lanes (3000 rows of 3333 bf16 values
+// 33 us, eight of them side by side 54).
 enum : int { kUnits = 0, kOnes = 1, kSpread = 2 };
 
 // The eight values of the step at element `at`; those at `width` and behind it are zero.
@@ -84,8 +86,37 @@ __device__ __forceinline__ void store8(void* row, uint32_t at, uint32_t step, ui
   }
 }
 
+__device__ __forceinline__ float wave_total(float v) { return wave_sum_all(v); }
+__device__ __forceinline__ double wave_total(double v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// h * (hi + lo) * gain of a factor given as a float and its rest: the nearest float, and what it leaves.
+__device__ __forceinline__ float exact_product(float h, float hi, float lo, float gain, float* off = nullptr) {
+#pragma clang fp contract(off)
+  const float s = hi * gain;
+  const float s_rest = fmaf(hi, gain, -s) + lo * gain;
+  const float p = h * s;
+  const float p_rest = fmaf(h, s_rest, fmaf(h, s, -p));
+  const float f = p + p_rest;
+  if (off != nullptr) *off = p_rest - (f - p);
+  return f;
+}
+
+// A float that is rounded once more, to e4m3, must not lie on a border there that the product itself does not lie on:
+// one step towards it then.  Borders have the last 19 bits of a float clear.
+constexpr uint32_t kBorderBits = 0x7ffffu;
+__device__ __forceinline__ float off_border(float f, float off) {
+  const uint32_t bits = __float_as_uint(f);
+  const bool finite = (bits & 0x7fffffffu) - 0x0d000000u < 0x7f800000u - 0x0d000000u;  // and far above subnormals
+  if ((bits & kBorderBits) != 0 || !finite || off == 0.0f) return f;
+  return __uint_as_float((off < 0.0f) == (f < 0.0f) ? bits + 1 : bits - 1);
+}
+
 // TPR threads per row (64 or 256), up to NV steps of eight values per thread.
-template <class A, int TPR, int NV, int LIE>
+template <class A, int TPR, int NV, int LIE, bool MXOUT>
 __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   const uint32_t t = threadIdx.x % TPR;
   const uint32_t row = blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR;
@@ -93,6 +124,11 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   const auto row_of = [&](const void* base, uint64_t stride) {
     return static_cast<const uint8_t*>(base) + static_cast<uint64_t>(row) * stride * A::kBytes;
   };
+  // MX rows: a row's factor in 64 bits (of sums of eight squares in 32) and its products with their rests.  In plain
+  // fp32 about ten of 8192 x 2560 values came out on the wrong side of an e4m3 border, of these one to three; the call
+  // takes 35.6 us, plain 31.3, all in 64 bits 48.
+  using Real = std::conditional_t<MXOUT, double, float>;
+  static_assert(!MXOUT || LIE != kSpread, "MX rows need a group's values side by side");
   // element of the thread's first value in step i, and between its values
   constexpr uint32_t kStep = LIE == kSpread ? TPR : 1;
   const auto at = [&](int i) { return LIE == kSpread ? i * TPR * 8u + t : (i * TPR + t) * 8u; };
@@ -110,24 +146,30 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
       for (int j = 0; j < 8; ++j) h[i][j] += v[j];
     }
   }
-  float scale = 1.0f;
-  if (p.weight != nullptr) {
-    float ss = 0.0f;
+  const bool normed = !MXOUT || p.weight != nullptr;
+  Real scale = 1;
+  if (normed) {
+    Real ss = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float s8 = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
-    ss = wave_sum_all(ss);
+      for (int j = 0; j < 8; ++j) s8 = fmaf(h[i][j], h[i][j], s8);
+      ss += s8;
+    }
+    ss = wave_total(ss);
     if constexpr (TPR > 64) {
-      __shared__ float s_part[TPR / 64];
+      __shared__ Real s_part[TPR / 64];
       if (t % 64 == 0) s_part[t / 64] = ss;
       __syncthreads();
-      ss = 0.0f;
+      ss = 0;
 #pragma unroll
       for (int w = 0; w < TPR / 64; ++w) ss += s_part[w];
     }
-    scale = 1.0f / sqrtf(ss / static_cast<float>(p.width) + p.eps);
+    scale = 1 / sqrt(ss / static_cast<Real>(p.width) + static_cast<Real>(p.eps));
   }
+  const float hi = static_cast<float>(scale);
+  const float lo = MXOUT ? static_cast<float>(scale - static_cast<Real>(hi)) : 0.0f;
   if (p.sum_out != nullptr) {
     uint8_t* s = const_cast<uint8_t*>(row_of(p.sum_out, p.sum_stride));
 #pragma unroll
@@ -135,29 +177,52 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (p.weight != nullptr) {
+    if (normed) {
       float g[8];
       if (p.weight_dtype == 0) load8<ActBF16, LIE>(p.weight, at(i), kStep, p.width, g);
       else load8<ActF32, LIE>(p.weight, at(i), kStep, p.width, g);
+      if (!p.one_centered) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * scale * (p.one_centered ? g[j] : 1.0f + g[j]);
+        for (int j = 0; j < 8; ++j) g[j] = 1.0f + g[j];
+      }
+      if constexpr (MXOUT) {
+        float y[8];
+        uint32_t least = ~0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          y[j] = exact_product(h[i][j], hi, lo, g[j]);
+          least = min(least, __float_as_uint(y[j]) & kBorderBits);
+        }
+        if (least == 0) {  // seldom: one of them may lie on a border
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float off;
+            const float f = exact_product(h[i][j], hi, lo, g[j], &off);
+            y[j] = off_border(f, off);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] = y[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * hi * g[j];
+      }
     }
-    if (p.values == nullptr) {
+    if constexpr (!MXOUT) {
       store8<A, LIE>(const_cast<uint8_t*>(row_of(p.out, p.out_stride)), at(i), kStep, p.width, h[i]);
-      continue;
-    }
-    if constexpr (LIE == kSpread) continue;  // MX rows need a group's values side by side
-    uint32_t m = 0;
+    } else {
+      uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(h[i][j]));
-    m = max(m, dpp_u<kDppQuadXor1>(m));
-    m = max(m, dpp_u<kDppQuadXor2>(m));
-    const uint32_t e = mx_scale(m);
-    if (at(i) < p.width) {  // the width is whole groups, so a lane's eight values are all in it
-      const uint64_t first = static_cast<uint64_t>(row) * p.width + at(i);
-      *reinterpret_cast<uint2*>(p.values + first) =
-          make_uint2(mx_pack4(h[i][0], h[i][1], h[i][2], h[i][3], e), mx_pack4(h[i][4], h[i][5], h[i][6], h[i][7], e));
-      if (t % 4 == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e);
+      for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(h[i][j]));
+      m = max(m, dpp_u<kDppQuadXor1>(m));
+      m = max(m, dpp_u<kDppQuadXor2>(m));
+      const uint32_t e = mx_scale(m);
+      if (at(i) < p.width) {  // the width is whole groups, so a lane's eight values are all in it
+        const uint64_t first = static_cast<uint64_t>(row) * p.width + at(i);
+        *reinterpret_cast<uint2*>(p.values + first) =
+            make_uint2(mx_pack4(h[i][0], h[i][1], h[i][2], h[i][3], e), mx_pack4(h[i][4], h[i][5], h[i][6], h[i][7], e));
+        if (t % 4 == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e);
+      }
     }
   }
 }
@@ -166,7 +231,8 @@ template <class A, int TPR, int NV>
 hipError_t norm_go(const NormLaunch& p, hipStream_t stream) {
   const uint32_t per = kNormThreads / TPR;
   const dim3 grid((p.rows + per - 1) / per);
-  auto kernel = p.vector ? &k_norm<A, TPR, NV, kUnits> : p.values != nullptr ? &k_norm<A, TPR, NV, kOnes> : &k_norm<A, TPR, NV, kSpread>;
+  auto kernel = p.values != nullptr ? (p.vector ? &k_norm<A, TPR, NV, kUnits, true> : &k_norm<A, TPR, NV, kOnes, true>)
+                                    : (p.vector ? &k_norm<A, TPR, NV, kUnits, false> : &k_norm<A, TPR, NV, kSpread, false>);
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("norm", &start, &stop))
     hipExtLaunchKernelGGL(kernel, grid, dim3(kNormThreads), 0, stream, start, stop, 0, p);
