@@ -42,8 +42,8 @@ enum : int { kOutBf16 = 0, kOutMx = 1 };
 
 __device__ uint4 g_product_zeros[kChunk / 16];  // units at and behind the end of a row load from here
 
-// One lane's MFMA operands of a 16-byte unit: itself, or two of bf16 values, e4m3 times 2^scale.  `scale` is the float
-// 2^(s - 127) of the scale byte s; bf16's subnormals and groups of scale 2^-127 come out as zero.
+// One lane's MFMA operands of a 16-byte unit: itself, or two of bf16 values, e4m3 ones times the power of two whose
+// exponent bits `scale` holds (0: 2^-127, 255: NaN).
 template <bool MX>
 struct Operand {
   uint4 part[MX ? 2 : 1];
@@ -124,7 +124,7 @@ __device__ __forceinline__ void store_strip(const ProductLaunch& p, const f32x4_
   const uint32_t at = col + kOut * kb;
   const uint64_t row = static_cast<uint64_t>(pair) * p.n;
   if constexpr (OUT == kOutMx) {
-    static_assert(SWIGLU || OUT == kOutBf16, "a strip of SwiGLU outputs is one group");
+    static_assert(SWIGLU, "a strip of SwiGLU outputs is one group");
     uint32_t m = 0;
 #pragma unroll
     for (uint32_t j = 0; j < kOut; ++j) m = max(m, mx_magnitude(y[j]));
@@ -292,9 +292,8 @@ __device__ __forceinline__ uint8_t* tile_stage() {
   return reinterpret_cast<uint8_t*>(buf);
 }
 
-// WM x WN waves of 16 RF rows by 64 matrix rows each.  WHOLE: K is whole chunks and scales are aligned.  ONCE: the
-// matrices are read once (ProductLaunch::once).
-template <bool MX, bool SWIGLU, int OUT, int RF, int WM, int WN, bool WHOLE, bool ONCE>
+// WM x WN waves of 16 RF rows by 64 matrix rows each.  WHOLE: K is whole chunks and scales are aligned.
+template <bool MX, bool SWIGLU, int OUT, int RF, int WM, int WN, bool WHOLE>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   constexpr int kWaves = WM * WN;
   constexpr uint32_t kRows = 16 * RF * WM, kMatrix = 64 * WN;
@@ -351,16 +350,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   const uint32_t chunks = (p.k_bytes + kChunk - 1) / kChunk, groups = p.k_bytes / kMxGroup;
   const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_product_zeros);
   if constexpr (!WHOLE) VM_KEEP(zeros);
+  const auto from = [&](int i, uint32_t c) {
+    const uint8_t* s = src[i] + c * kChunk;
+    if constexpr (!WHOLE)
+      if (c * kChunk + at[i] >= p.k_bytes) s = zeros;
+    return s;
+  };
+  const bool once = p.once && td.group_rows <= kRows;
   auto issue = [&](auto J, uint32_t c) {
     uint8_t* st = tile_stage<decltype(J)::value, kRows + kMatrix>();
+    uint8_t* st_w = st + kRows / 8 * 1024u + wave * kDmaW * 1024u;
 #pragma unroll
-    for (int i = 0; i < kDmaX + kDmaW; ++i) {
-      const uint32_t g = i < kDmaX ? wave * kDmaX + i : kRows / 8 + wave * kDmaW + (i - kDmaX);
-      const uint8_t* s = src[i] + c * kChunk;
-      if constexpr (!WHOLE)
-        if (c * kChunk + at[i] >= p.k_bytes) s = zeros;
-      if (i < kDmaX) load_to_lds(s, st + g * 1024u);
-      else load_to_lds<ONCE>(s, st + g * 1024u);
+    for (int i = 0; i < kDmaX; ++i) load_to_lds(from(i, c), st + (wave * kDmaX + i) * 1024u);
+    if (once) {
+#pragma unroll
+      for (int i = 0; i < kDmaW; ++i) load_to_lds<true>(from(kDmaX + i, c), st_w + i * 1024u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDmaW; ++i) load_to_lds(from(kDmaX + i, c), st_w + i * 1024u);
     }
   };
 
@@ -483,10 +490,8 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
     constexpr uint32_t kWaves = WM * WN, cols = strip_cols<SWIGLU>() * WN;
     p.tile_blocks = (p.n + cols - 1) / cols * tiles;
     const uint32_t blocks = p.tile_blocks + (p.rows + kWaves * kZeroRows - 1) / (kWaves * kZeroRows);
-    if (!whole) return go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, false, false>, blocks, 64 * kWaves, p, stream);
-    if constexpr (WN == 4)
-      if (p.once) return go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, true, true>, blocks, 64 * kWaves, p, stream);
-    return go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, true, false>, blocks, 64 * kWaves, p, stream);
+    return whole ? go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, true>, blocks, 64 * kWaves, p, stream)
+                 : go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, false>, blocks, 64 * kWaves, p, stream);
   };
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
@@ -518,13 +523,12 @@ uint32_t product_tile_rows(uint32_t rows, uint32_t experts) {
   return rows / experts < kTallMean ? 32u : 64u;
 }
 
-// Matrices that outgrow the 256 MB Infinity Cache and are mostly read by one tile stream past the caches: 512 tokens,
-// ten of 512 experts, 2048 -> 2 x 512 364 to 336 us, 2048 tokens MX 2560 -> 2 x 640 363 to 356, eight tokens 58 to 55.
-// Shared by several tiles or held by that cache they must not: 8192 tokens 613 to 941, 333 tokens of four of 64
-// experts, 1024 -> 2 x 256, 20 to 23.
-bool product_once(const ProductLaunch& p, uint32_t tile_rows) {
-  const uint64_t bytes = uint64_t(p.experts) * p.n * (p.swiglu ? 2 : 1) * p.k_bytes;
-  return bytes > (256ull << 20) && (tile_rows == 0 || p.rows / p.experts <= 48);
+// Matrices that together outgrow the 256 MB Infinity Cache stream past the caches where one tile reads them (k_tiles
+// looks at each group): 2048 -> 2 x 512, ten of 512 experts, 512 tokens 364 to 336 us, eight tokens 58 to 55, 2048 tokens
+// with skewed popularity 448 to 419; MX 2560 -> 2 x 640, 2048 tokens, 363 to 356.  Read by several tiles or held by that
+// cache they must not: 8192 tokens 613 to 941, 333 tokens of four of 64 experts, 1024 -> 2 x 256, 20 to 23.
+bool product_once(const ProductLaunch& p) {
+  return uint64_t(p.experts) * p.n * (p.swiglu ? 2 : 1) * p.k_bytes > (256ull << 20);
 }
 
 uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu) {
@@ -534,7 +538,7 @@ uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t ti
 }
 
 hipError_t launch_products(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) {
-  p.once = product_once(p, tile_rows);
+  p.once = product_once(p);
   if (p.values != nullptr && !p.swiglu) return hipErrorInvalidValue;
   if (p.mx) {
     if (!p.swiglu) return products_go<true, false, kOutBf16>(p, tile_rows, stream);

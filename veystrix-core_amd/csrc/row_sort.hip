@@ -7,7 +7,8 @@
 // Calls of up to kOneLaunchRows rows take one launch: every block counts all ids (its own rows, those before and those
 // behind) in LDS, lays the groups out by one scan, and places its own rows; nothing has to be zeroed or waited for
 // between blocks.  Larger calls count by blocks first (a launch), and every block adds those counts up instead.
-//   8192 rows of 32 groups 5.2 us, in the four launches of the layer's sort 20; 1332 of 64 5.1 and 5.6.
+// 1332 rows of 64 groups 5.2 us, 8192 in runs of one of 32 8.4 (22 in the four launches of the layer's sort); 81920 of
+// 512 in two launches 4.9 + 9.5.  It is bound by latency: LDS additions, a scan and the tile list one after the other.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
@@ -137,9 +138,9 @@ __global__ __launch_bounds__(kThreads) void k_row_place(RowSortLaunch p) {
         if (s_own[mid] <= k) lo = mid;
         else hi = mid;
       }
-      const uint32_t start = s_after[lo] + (k - s_own[lo]) * p.tile_rows;
-      const uint32_t end = lo + 1 < kThreads ? s_after[lo + 1] : s_total[1];
-      p.tiles[k] = RowTile{lo, start, min(end - start, p.tile_rows), 0};
+      const uint32_t begin = s_after[lo], end = lo + 1 < kThreads ? s_after[lo + 1] : s_total[1];
+      const uint32_t start = begin + (k - s_own[lo]) * p.tile_rows;
+      p.tiles[k] = RowTile{lo, start, min(end - start, p.tile_rows), end - begin};
     }
   }
   __syncthreads();

@@ -443,7 +443,8 @@ hipError_t launch_norm(const NormLaunch& p, hipStream_t stream);
 // -------------------------------------------------------------- row sort --
 // Rows sorted by group (row_sort.hip).
 struct RowTile {
-  uint32_t group, row, rows, pad;  // first sorted row and how many
+  uint32_t group, row, rows;   // first sorted row and how many
+  uint32_t group_rows;         // rows of the whole group
 };
 struct RowSortLaunch {
   const int32_t* ids;          // [rows]
@@ -481,7 +482,7 @@ struct ProductLaunch {
   uint32_t tile_blocks;        // blocks of the grid that serve tiles (set by launch_products)
   bool mx, swiglu;
   bool out_aligned;            // out is 16-byte aligned
-  bool once;                   // the matrices stream past the caches (set by launch_products)
+  bool once;                   // matrices read by one tile stream past the caches (set by launch_products)
 };
 
 // How a call of this many routed rows runs: 0 its rows one by one, or rows per
