@@ -358,8 +358,9 @@ typedef struct VmGroupedArgs {
  *   out = h / sqrt(mean(h^2) + eps) * gain    gain = weight (one_centered) or 1 + weight
  * as `out` [rows, width] in act_dtype, or as MX rows `values` [rows, width] and
  * `scales` [rows, width / 32], contiguous (width a multiple of 32, values
- * 8-byte aligned).  `sum_out` optionally receives h in act_dtype; it may be x
- * or residual, and out may be x.  Strides count elements between rows.
+ * 8-byte aligned).  `sum_out` optionally receives h in act_dtype.  out and
+ * sum_out may each be x or residual, row for row; outputs overlap nothing
+ * otherwise.  Strides count elements between rows.
  * width up to VM_NORM_MAX_WIDTH.  No counterpart in the reference's surface
  * beyond its norm (patch_rmsnorm.py:108-135). */
 #define VM_NORM_MAX_WIDTH 16384
@@ -387,10 +388,13 @@ typedef struct VmNormArgs {
  * VM_ACTIVATION_SWIGLU: the matrix has 2 n rows, gate then up, and
  * out = silu(gate) * up in fp32.  bf16 or MX operands (both the same), output
  * in bf16 or, with swiglu and n a multiple of 32, as MX rows.  An id outside
- * 0..experts-1 gives a row of zeros.
+ * 0..experts-1 gives a row of zeros.  MX values enter as bf16: those below
+ * 2^-126 are rounded to multiples of 2^-133.  Outputs overlap no operand.
  * k: a multiple of 8 (bf16) or 32 (MX); rows of x and weight 16-byte aligned,
- * `out_values` 8-byte aligned; out, out_values and out_scales contiguous.  experts up to VM_PRODUCT_MAX_EXPERTS.  Strides count elements
- * (of an MX scale array: scales).  The workspace needs no initialisation. */
+ * `out_values` 8-byte aligned; out, out_values and out_scales contiguous.
+ * experts up to VM_PRODUCT_MAX_EXPERTS, k and n up to 2^24, rows up to 2^28.
+ * Strides count elements (of an MX scale array: scales).  The workspace needs
+ * no initialisation; calls that may run at once need one each. */
 #define VM_PRODUCT_MAX_EXPERTS 1024
 typedef struct VmProductArgs {
   const void* x;                 /* [ceil(rows / x_div), k] */
@@ -412,9 +416,9 @@ typedef struct VmProductArgs {
  * they share, bf16 with fp32 sums:
  *   out[t] = base[t] + scales[i] * b[i] (a[i] x[t]),  i = ids[t]
  * and out[t] = base[t] for an id outside 0..adapters-1.  out may be base, and
- * overlaps no other operand.  rank up to VM_ADAPTER_MAX_RANK, adapters up to
- * VM_PRODUCT_MAX_EXPERTS.  Strides count elements.  The workspace needs no
- * initialisation. */
+ * overlaps nothing otherwise.  rank up to VM_ADAPTER_MAX_RANK, adapters up to
+ * VM_PRODUCT_MAX_EXPERTS, k and n up to 2^24.  Strides count elements.  The
+ * workspace needs no initialisation; calls that may run at once need one each. */
 #define VM_ADAPTER_MAX_RANK 128
 typedef struct VmAdapterArgs {
   const void* base;              /* [rows, n] */

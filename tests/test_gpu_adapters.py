@@ -68,6 +68,41 @@ def test_adapters_ids_strides_and_dimensions(device, rows):
     assert add_adapters(base[:0], x[:0], a, b, ids[:0]).shape == (0, 96)
 
 
+@pytest.mark.parametrize("rows", [9, 600])
+def test_adapters_of_banks_off_the_vector_units(device, rows):
+    """Banks that start two bytes into a buffer take element loads; the results stay the same."""
+    gen = torch.Generator().manual_seed(rows)
+    base, x, a, b, ids = _bank(gen, rows, 128, 96, 16, 5, device)
+    want = _check(base, x, a, b, ids)
+    for which in ("a", "b", "ab"):
+        banks = []
+        for name, t in (("a", a), ("b", b)):
+            off = torch.empty(t.numel() + 1, dtype=torch.bfloat16, device=device)[1:].view(t.shape)
+            banks.append(off.copy_(t) if name in which else t)
+        got = _check(base, x, *banks, ids)
+        assert torch.equal(got[ids < 0], want[ids < 0])
+
+
+def test_adapters_of_many_rows_and_as_many_as_may_be(device):
+    gen = torch.Generator().manual_seed(16385)
+    for rows, k, n, rank, adapters in ((16385, 64, 72, 16, 3), (40000, 32, 40, 8, 1024), (16384, 32, 64, 8, 1024)):
+        base, x, a, b, ids = _bank(gen, rows, k, n, rank, adapters, device)
+        ids[:3] = adapters - 1
+        _check(base, x, a, b, ids)
+
+
+def test_adapters_side_by_side_in_one_buffer(device):
+    """base, x and out as column ranges of the same rows do not overlap."""
+    gen = torch.Generator().manual_seed(5)
+    base, x, a, b, ids = _bank(gen, 700, 64, 96, 16, 5, device)
+    rows = torch.zeros((700, 96 + 64 + 96), dtype=torch.bfloat16, device=device)
+    rows[:, :96], rows[:, 96:160] = base, x
+    want = add_adapters(base, x, a, b, ids)
+    got = add_adapters(rows[:, :96], rows[:, 96:160], a, b, ids, out=rows[:, 160:])
+    assert torch.equal(got, want)
+    assert torch.equal(rows[:, :96], base) and torch.equal(rows[:, 96:160], x)
+
+
 @pytest.mark.parametrize("rows", [4, 200])
 def test_adapters_without_any_and_with_one(device, rows):
     gen = torch.Generator().manual_seed(12)
@@ -119,3 +154,12 @@ def test_adapters_refusals(device):
         add_adapters(base, x, a, b, ids, scales=torch.ones(2, device=device))
     with pytest.raises(RuntimeError):
         add_adapters(base, x, a.repeat(1, 17, 1), b.repeat(1, 1, 17), ids)    # rank 136
+    with pytest.raises(ValueError):
+        add_adapters(base, x[:, :32], a[:, :, :32].contiguous(), b, ids, out=x[:, :32])
+    with pytest.raises(ValueError):
+        both = torch.zeros((5, 32), dtype=torch.bfloat16, device=device)
+        add_adapters(both[:4], x, a, b, ids, out=both[1:])
+    with pytest.raises(ValueError):
+        add_adapters(base, x, a, b, ids, out=base[:1].expand(4, 32))          # one row for all results
+    with pytest.raises(ValueError):
+        add_adapters(base, x, a, b, ids, scales=0.5)

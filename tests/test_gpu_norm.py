@@ -157,3 +157,43 @@ def test_norm_refusals(device):
     wide = torch.zeros((1, 16416), dtype=torch.bfloat16, device=device)
     with pytest.raises(RuntimeError):
         rms_norm(wide, torch.ones(16416, dtype=torch.bfloat16, device=device))
+    with pytest.raises(ValueError):
+        rms_norm(x[:, :32], w[:32], out=x[:, 16:48])
+    with pytest.raises(ValueError):
+        rms_norm(x, w, out=x[:1].expand(4, 64))
+    with pytest.raises(ValueError):
+        rms_norm(x, w, residual=x.clone(), out=x, residual_out=x)
+    with pytest.raises(ValueError):
+        rms_norm(x[:1, :1].expand(2 ** 32 + 2, 1), w[:1])
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float32])
+def test_norm_over_its_operands(device, act):
+    """The normed rows over residual and h over x, and all of them as column ranges of one buffer."""
+    gen = torch.Generator().manual_seed(3)
+    x, r = (torch.randn((1500, 96), generator=gen).to(act).to(device) for _ in range(2))
+    w = torch.rand(96, generator=gen).to(device)
+    y, h = rms_norm(x, w, residual=r)
+    xs, rs = x.clone(), r.clone()
+    rms_norm(xs, w, residual=rs, out=rs, residual_out=xs)
+    assert torch.equal(rs, y) and torch.equal(xs, h)
+    buf = torch.cat([x, r, torch.zeros_like(x), torch.zeros_like(x)], 1)
+    parts = buf.split(96, 1)
+    rms_norm(parts[0], w, residual=parts[1], out=parts[2], residual_out=parts[3])
+    for part, want in zip(parts, (x, r, y, h)):
+        assert torch.equal(part, want)
+
+
+def test_dequantize_of_the_least_scales(device):
+    x = torch.zeros((2, 64), device=device)
+    x[0, :32], x[0, 32:], x[1, :32], x[1, 32:] = 2.0 ** -127, 3.0 * 2.0 ** -128, 2.0 ** 127, 2.0 ** -110
+    assert torch.equal(mx_quantize(x).dequantize(), x)
+    assert torch.equal(mx_quantize(x).dequantize(torch.bfloat16), x.bfloat16())
+
+
+@pytest.mark.parametrize("rows", [3, 2000])
+def test_norm_to_mx_with_a_gain_of_one_and_weight(device, rows):
+    gen = torch.Generator().manual_seed(rows)
+    x, w = torch.randn((rows, 96), generator=gen).bfloat16().to(device), (torch.rand(96, generator=gen) - 0.5).to(device)
+    want, _, err = norm_exact(x, w, one_centered=False)
+    assert_mx_within(rms_norm(x, w, one_centered=False, quantize=True), want, err)

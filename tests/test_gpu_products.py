@@ -117,6 +117,107 @@ def test_a_row_with_infinities_keeps_to_itself(device):
         assert not torch.isfinite(got[1]).any() and torch.isnan(got[2]).all()
 
 
+@pytest.mark.parametrize("tokens", [3, 60, 200])
+def test_mx_groups_that_are_not_numbers(device, tokens):
+    """A row with a NaN group makes its own outputs NaN and no others'; so does a matrix row its own column."""
+    gen = torch.Generator().manual_seed(tokens)
+    x = torch.randn((tokens, 160), generator=gen).to(device)
+    w = torch.randn((4, 64, 160), generator=gen).to(device)
+    inds = (torch.arange(tokens) % 4).int().reshape(-1, 1).to(device)
+    clean = grouped_matmul(mx_quantize(x), mx_quantize(w), inds)
+    x[1, 159], w[2, 5, 3] = float("inf"), float("nan")
+    got = grouped_matmul(mx_quantize(x), mx_quantize(w), inds).view(tokens, 64)
+    bad = torch.zeros((tokens, 64), dtype=torch.bool, device=device)
+    bad[1] = True
+    bad[inds[:, 0] == 2, 5] = True
+    assert torch.isnan(got[bad]).all()
+    assert torch.equal(got[~bad], clean.view(tokens, 64)[~bad])
+
+
+@pytest.mark.parametrize("tokens", [4, 40, 400])
+def test_mx_extremes_of_scale(device, tokens):
+    """Scales far apart cancel in the product.  Below bf16's normal range values are rounded to multiples of 2^-133:
+    off by 2^-134 at most, times the matrix value."""
+    x, w = torch.full((tokens, 64), 1e-30), torch.full((2, 64, 64), 1e30)
+    x[:, 32:] = 0
+    x[3] = 1e-40
+    x[2, 40] = 1e-37
+    inds = torch.zeros((tokens, 1), dtype=torch.int32, device=device)
+    xq, wq = mx_quantize(x.to(device)), mx_quantize(w.to(device))
+    xv, wv = mx_value(xq).cpu().double(), mx_value(wq).cpu().double()[0]
+    want = xv @ wv.T
+    err = (xv != 0).double() @ wv.abs().T * 2.0 ** -134 + 64 * 2.0 ** -24 * want.abs()
+    got = grouped_matmul(xq, wq, inds).cpu().view(tokens, 64).double()
+    assert ((got - want).abs() <= err + (want.abs() + err) * HALF_STEP[torch.bfloat16]).all()
+
+
+@pytest.mark.parametrize("mx", [False, True], ids=["bf16", "mx"])
+@pytest.mark.parametrize("tokens", [9, 130, 700])
+def test_matrices_larger_than_the_cache(device, tokens, mx):
+    """More than 256 MB of matrices, which stream past the caches but for those of several tiles: most rows of the
+    larger calls go to one expert."""
+    gen = torch.Generator().manual_seed(tokens)
+    experts, k, n = (300, 1024, 512) if not mx else (300, 1024, 1024)
+    w = torch.randn((8, n, k), generator=gen).bfloat16().to(device) * k ** -0.5
+    w = w.repeat((experts + 7) // 8, 1, 1)[:experts]
+    x = torch.randn((tokens, k), generator=gen).bfloat16().to(device)
+    if mx:
+        x, w = mx_quantize(x), mx_quantize(w)
+    inds = _ids(gen, tokens, 2, experts)
+    inds[tokens // 3:, 0] = 5
+    inds[inds[:, 0] == inds[:, 1], 1] = 6
+    got = grouped_matmul(x, w, inds.to(device))
+    small = MxTensor(w.values[:8], w.scales[:8]) if mx else w[:8]
+    want, err = product_exact(_wide(x)[:, None].expand(tokens, 2, k), _wide(small), inds % 8, False)
+    assert_within(got, want, err + (want.abs() + err) * HALF_STEP[torch.bfloat16])
+
+
+# 64-row tiles of more than 16384 rows, and 32-row ones of as many experts as there may be: the widest blocks, with k of
+# whole chunks and not
+@pytest.mark.parametrize("mx", [False, True], ids=["bf16", "mx"])
+@pytest.mark.parametrize("kind", ["plain", "swiglu", "swiglu_mx"])
+@pytest.mark.parametrize("tokens,slots,experts,k,n", [(4300, 4, 40, 512, 2048), (8601, 2, 40, 544, 2112),
+                                                      (4000, 2, 1024, 1024, 512), (4000, 2, 1024, 1056, 576)])
+def test_large_calls(device, tokens, slots, experts, k, n, kind, mx):
+    gen = torch.Generator().manual_seed(tokens + k)
+    swiglu = kind != "plain"
+    x, w = _operands(gen, (tokens, k), (8, n, k), mx, device)
+    bank = (lambda t: t.repeat((experts + 7) // 8, 1, 1)[:experts])
+    full = MxTensor(bank(w.values.view(torch.uint8)).view(w.values.dtype),
+                    bank(w.scales.view(torch.uint8)).view(w.scales.dtype)) if mx else bank(w)
+    inds = torch.randint(-1, experts, (tokens, slots), generator=gen, dtype=torch.int32)
+    got = grouped_matmul(x, full, inds.to(device), activation="swiglu" if swiglu else None, quantize=kind == "swiglu_mx")
+    some = torch.cat([torch.arange(40), torch.randint(0, tokens, (300,), generator=gen), torch.arange(tokens - 40, tokens)])
+    ids = torch.where(inds < 0, -1, inds % 8)[some]
+    want, err = product_exact(_wide(x)[some][:, None].expand(len(some), slots, k), _wide(w), ids, swiglu)
+    pick = some.to(device)
+    if kind == "swiglu_mx":
+        got = MxTensor(got.values.view(torch.uint8)[pick].view(got.values.dtype),
+                       got.scales.view(torch.uint8)[pick].view(got.scales.dtype))
+        assert_mx_within(got, want, err)
+    else:
+        assert_within(got[pick], want, err + (want.abs() + err) * HALF_STEP[torch.bfloat16])
+        assert (got[(inds < 0).to(device)] == 0).all()
+
+
+def test_two_streams_at_once(device):
+    gen = torch.Generator().manual_seed(77)
+    x, w = _operands(gen, (600, 256), (12, 256, 256), False, device)
+    inds = [_ids(gen, 600, 4, 12).to(device) for _ in range(2)]
+    want = [grouped_matmul(x, w, i, activation="swiglu") for i in inds]
+    streams = [torch.cuda.Stream() for _ in inds]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(grouped_matmul(x, w, inds[j], activation="swiglu"))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for y in got[j]:
+            assert torch.equal(y, want[j])
+
+
 @pytest.mark.parametrize("mx", [False, True], ids=["bf16", "mx"])
 @pytest.mark.parametrize("tokens", [2, 50, 400])
 def test_strided_operands(device, tokens, mx):
@@ -204,3 +305,9 @@ def test_refusals(device):
         grouped_matmul(x[:, :60].contiguous(), w[:, :, :60].contiguous(), inds)      # k not a multiple of 8
     with pytest.raises(ValueError):
         grouped_matmul(x[:, 1:57], w[:, :, :56], inds)                               # rows off 16 bytes
+    with pytest.raises(ValueError):
+        both = torch.zeros((8, 64), dtype=torch.bfloat16, device=device)
+        grouped_matmul(both, w, inds[:, :1].repeat(2, 1), out=both.view(16, 32)[:8].view(8, 1, 32))
+    with pytest.raises(ValueError):
+        many = torch.zeros((1, 1), dtype=torch.int32, device=device).expand(2 ** 16 + 1, 2 ** 16)
+        grouped_matmul(x[:1].expand(2 ** 16 + 1, 64), w, many)

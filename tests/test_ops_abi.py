@@ -160,3 +160,48 @@ def test_adapters_rejects(fields, code, message):
 def test_adapters_of_nothing():
     assert _adapters(rows=0) == _lib.VM_OK
     assert _lib.lib().vm_add_adapters(None, None) == _lib.VM_EINVAL
+
+
+# x at 1 << 20, two rows of 128 bytes; the other arrays of the helpers lie below it
+APART = 1 << 20
+
+
+@pytest.mark.parametrize("fields", [
+    {"out": 4096 + 2},                                               # x a value further
+    {"out": 4096, "out_stride": 72},                                 # x at another stride
+    {"x": APART, "out": APART + 100, "out_stride": 128, "x_stride": 128},
+    {"out": 8192},                                                   # weight
+    {"out": 8192 - 128},                                             # its second row is the weight
+    {"residual": APART, "out": APART + 128},                         # residual's second row
+    {"residual": APART, "sum_out": 12288},                           # sum_out is out
+    {"residual": APART, "sum_out": 4096 + 64},
+    {"residual": APART, "sum_out": APART + 64},
+    {"residual": APART, "sum_out": 8192 + 64},
+    {"out": None, "values": 4096 + 64, "scales": 1 << 21},
+    {"out": None, "values": 1 << 21, "scales": 8192},
+    {"out": None, "values": 1 << 21, "scales": 1 << 22, "residual": APART, "sum_out": (1 << 21) + 64},
+])
+def test_norm_rejects_outputs_over_operands(fields):
+    assert _norm(**fields) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("fields", [
+    {"out": 4096}, {"out": 4096 + 127}, {"out": 8192}, {"out": 8192 + 4 * 32 * 128 - 2}, {"out": 12288 + 4},
+    {"out": 12288 - 64},                                             # its second row
+    {**MX, "x_scales": 1 << 21, "weight_scales": 1 << 22, "out": (1 << 21) + 2, "x_scale_stride": 2},
+    {"activation": 1, "out": None, "out_values": 4096 + 64, "out_scales": 1 << 21},
+    {"activation": 1, "out": None, "out_values": 1 << 21, "out_scales": 8192 + 2},
+])
+def test_product_rejects_outputs_over_operands(fields):
+    assert _product(**fields) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("fields", [
+    {"out": 4096 + 2}, {"out": 4096 + 64}, {"out": 8192}, {"out": 8192 + 32, "out_stride": 64}, {"out": 12288}, {"out": 16384},
+    {"out": 20480}, {"scales": 24576 + 8},
+])
+def test_adapters_reject_outputs_over_operands(fields):
+    assert _adapters(**fields) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()

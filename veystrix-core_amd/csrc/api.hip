@@ -1501,6 +1501,28 @@ static bool rows_aligned(const void* p, uint64_t stride_bytes, uint32_t unit) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % unit == 0 && stride_bytes % unit == 0);
 }
 
+// Rows of `width` bytes, `stride` bytes apart.
+struct RowBytes {
+  const void* at;
+  uint64_t rows, stride, width;
+};
+
+static bool same_rows(const RowBytes& a, const RowBytes& b) {
+  return a.at == b.at && (a.stride == b.stride || a.rows == 1);
+}
+
+// No byte in common: extents apart, or rows of one stride side by side.
+static bool rows_apart(const RowBytes& a, const RowBytes& b) {
+  if (a.at == nullptr || b.at == nullptr) return true;
+  const uint64_t a0 = reinterpret_cast<uintptr_t>(a.at), a1 = a0 + (a.rows - 1) * a.stride + a.width;
+  const uint64_t b0 = reinterpret_cast<uintptr_t>(b.at), b1 = b0 + (b.rows - 1) * b.stride + b.width;
+  if (a1 <= b0 || b1 <= a0) return true;
+  const uint64_t s = a.rows == 1 ? b.stride : a.stride;
+  if (s == 0 || (b.rows > 1 && b.stride != s)) return false;
+  const uint64_t d = a0 <= b0 ? (b0 - a0) % s : (s - (a0 - b0) % s) % s;  // from a row of a to the next one of b
+  return d >= a.width && d + b.width <= s;
+}
+
 static int check_mx_rows(const uint8_t* values, const uint8_t* scales, uint32_t width) {
   if (values == nullptr || scales == nullptr) return fail(VM_EINVAL, "MX rows need both values and scales");
   if (width % VM_MX_GROUP) return fail(VM_EINVAL, "MX rows need a width that is a multiple of %d", VM_MX_GROUP);
@@ -1536,6 +1558,17 @@ int vm_rms_norm(const VmNormArgs* a, void* stream) {
   const uint64_t w = a->width;
   if (a->rows > 1 && ((a->out != nullptr && a->out_stride < w) || (a->sum_out != nullptr && a->sum_stride < w)))
     return fail(VM_EINVAL, "the row strides of outputs must be at least the width");
+  const uint64_t size = a->act_dtype == VM_F32 ? 4 : 2;
+  const RowBytes x{a->x, a->rows, a->x_stride * size, w * size}, r{a->residual, a->rows, a->residual_stride * size, w * size};
+  const RowBytes weight{a->weight, 1, 0, w * (a->weight_dtype == VM_F32 ? 4 : 2)};
+  const RowBytes out{a->out, a->rows, a->out_stride * size, w * size}, sum{a->sum_out, a->rows, a->sum_stride * size, w * size};
+  const RowBytes values{a->values, a->rows, w, w}, scales{a->scales, a->rows, w / VM_MX_GROUP, w / VM_MX_GROUP};
+  if (!(same_rows(out, x) || rows_apart(out, x)) || !(same_rows(sum, x) || rows_apart(sum, x)) ||
+      !(same_rows(out, r) || rows_apart(out, r)) || !(same_rows(sum, r) || rows_apart(sum, r)) || !rows_apart(out, sum) ||
+      !rows_apart(out, weight) || !rows_apart(sum, weight))
+    return fail(VM_EINVAL, "outputs overlap each other or an operand");
+  for (const RowBytes& in : {x, r, weight, sum})
+    if (!rows_apart(values, in) || !rows_apart(scales, in)) return fail(VM_EINVAL, "MX rows overlap an operand");
   vm::NormLaunch p{};
   p.x = a->x;
   p.residual = a->residual;
@@ -1654,11 +1687,27 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   const uint32_t tile = vm::product_tile_rows(a->rows, a->experts);
   if (vm::product_blocks(a->rows, a->experts, a->n, tile, swiglu) > kMaxBlocks)
     return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
+  const RowSortWs w = tile == 0 ? RowSortWs{} : row_sort_ws(a->rows, a->experts, tile);
+  if (tile != 0 && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
+    return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
+  const uint64_t x_rows = (uint64_t(a->rows) - 1) / a->x_div + 1, w_rows = uint64_t(a->n) * (swiglu ? 2 : 1);
+  const auto matrices = [&](const void* at, uint64_t row, uint64_t expert, uint64_t width) {  // first to last byte
+    return RowBytes{at, 1, 0, ((a->experts - 1) * expert + (w_rows - 1) * row) + width};
+  };
+  const RowBytes outs[] = {{a->out, a->rows, a->n * 2ull, a->n * 2ull},
+                           {a->out_values, a->rows, a->n, a->n},
+                           {a->out_scales, a->rows, a->n / VM_MX_GROUP, a->n / VM_MX_GROUP}};
+  const RowBytes ins[] = {{a->x, x_rows, a->x_stride * size, uint64_t(a->k) * size},
+                          matrices(a->weight, a->weight_stride * size, a->weight_expert_stride * size, uint64_t(a->k) * size),
+                          {mx ? a->x_scales : nullptr, x_rows, a->x_scale_stride, a->k / VM_MX_GROUP},
+                          matrices(mx ? a->weight_scales : nullptr, a->weight_scale_stride, a->weight_scale_expert_stride,
+                                   a->k / VM_MX_GROUP),
+                          {a->ids, 1, 0, uint64_t(a->rows) * 4}};
+  for (const RowBytes& out : outs)
+    for (const RowBytes& in : ins)
+      if (!rows_apart(out, in)) return fail(VM_EINVAL, "outputs overlap an operand");
   vm::ProductLaunch p{};
   if (tile != 0) {
-    const RowSortWs w = row_sort_ws(a->rows, a->experts, tile);
-    if (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace))
-      return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
     vm::RowSortLaunch s{};
     const hipError_t e = sort_rows(a->ids, a->rows, a->experts, tile, w, a->workspace, stream, s);
     if (e != hipSuccess) return hip_fail(e, "sort launch");
@@ -1736,10 +1785,16 @@ int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
   p.vector_n = a->n % 8 == 0 && rows_aligned(a->base, a->base_stride * 2, 16) && rows_aligned(a->out, a->out_stride * 2, 16);
   if (vm::adapter_blocks(a->rows, a->adapters, a->n, tiled) > kMaxBlocks)
     return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
+  const RowSortWs w = tiled ? row_sort_ws(a->rows, a->adapters, vm::kAdapterTile) : RowSortWs{};
+  if (tiled && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
+    return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
+  const RowBytes out{a->out, a->rows, a->out_stride * 2, a->n * 2ull}, base{a->base, a->rows, a->base_stride * 2, a->n * 2ull};
+  const uint64_t bank = uint64_t(a->adapters) * a->rank * 2;
+  if (!(same_rows(out, base) || rows_apart(out, base)) || !rows_apart(out, {a->x, a->rows, a->x_stride * 2, a->k * 2ull}) ||
+      !rows_apart(out, {a->a, 1, 0, bank * a->k}) || !rows_apart(out, {a->b, 1, 0, bank * a->n}) ||
+      !rows_apart(out, {a->scales, 1, 0, a->adapters * 4ull}) || !rows_apart(out, {a->ids, 1, 0, a->rows * 4ull}))
+    return fail(VM_EINVAL, "out overlaps an operand, other than base in place");
   if (tiled) {
-    const RowSortWs w = row_sort_ws(a->rows, a->adapters, vm::kAdapterTile);
-    if (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace))
-      return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
     vm::RowSortLaunch s{};
     const hipError_t e = sort_rows(a->ids, a->rows, a->adapters, vm::kAdapterTile, w, a->workspace, stream, s);
     if (e != hipSuccess) return hip_fail(e, "sort launch");

@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import device_call, route_ids, row_span
+from .device import device_call, require_32_bits, route_ids, row_span
 
 _BF16 = torch.bfloat16
 
@@ -31,7 +31,7 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     base [.., n] the shared projection's output and x [.., k] its input, bfloat16 with equally spaced rows; a
     [adapters, rank, k] and b [adapters, n, rank] bfloat16, contiguous; ids [..] int32/int64; scales [adapters] float32
     (1 without).  Up to 1024 adapters of rank up to 128.  The rank sums stay in fp32, and the result is rounded once.
-    ``out`` may be base.
+    ``out`` may be base, and overlaps nothing otherwise.
     """
     index = x.get_device() if isinstance(x, torch.Tensor) else None
     x_at, x_stride = row_span("x", x, _BF16, index)
@@ -46,10 +46,12 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     ids = route_ids("ids", ids, adapters, index)
     if ids.shape != lead:
         raise ValueError(f"ids must have shape {tuple(lead)}")
+    rows = ids.numel()
+    require_32_bits(rows, k, n, rank)
     scales_at = None
     if scales is not None:
-        if scales.dtype != torch.float32 or scales.shape != (adapters,) or not scales.is_contiguous() \
-                or scales.device != x.device:
+        if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or scales.shape != (adapters,) \
+                or not scales.is_contiguous() or scales.device != x.device:
             raise ValueError(f"scales must be contiguous float32 of shape ({adapters},) on {x.device}")
         scales_at = scales.data_ptr()
     if out is None:
@@ -57,7 +59,6 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     elif out.shape != shape:
         raise ValueError("out must have base's shape")
     out_at, out_stride = row_span("out", out, _BF16, index)
-    rows = ids.numel()
     if rows == 0 or n == 0:
         return out
     lib = _lib.lib()

@@ -98,6 +98,12 @@ def row_span(name: str, tensor, dtype, index):
     return tensor.data_ptr(), shape[-1] if step is None else step
 
 
+def require_32_bits(*sizes):
+    """Sizes that the C ABI takes in 32 bits."""
+    if max(sizes) >> 32:
+        raise ValueError(f"a call takes sizes below 2^32 (got {sizes})")
+
+
 def route_ids(name: str, ids, count: int, index):
     """Contiguous int32 group ids on GPU ``index``; 64-bit ids outside 0..count-1 stay outside."""
     if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.get_device() != index:

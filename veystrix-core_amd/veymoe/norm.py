@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .device import ACT_DTYPES, device_call, row_span
+from .device import ACT_DTYPES, device_call, require_32_bits, row_span
 
 MX_GROUP = _lib.VM_MX_GROUP
 _SCALE_DTYPES = (torch.float8_e8m0fnu, torch.uint8)
@@ -67,12 +67,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     x [.., width] bfloat16 or float32 with equally spaced rows, width up to 16384; residual of x's shape and type;
     weight [width] in either type.  Returns the normed rows in x's type, or as an :class:`MxTensor` with ``quantize``
     (width a multiple of 32).  With a residual it returns ``(normed, h)``, h rounded to x's type; the norm itself reads
-    the unrounded sum.  ``out`` may be x, ``residual_out`` may be x or residual.
+    the unrounded sum.  ``out`` and ``residual_out`` may each be x or residual, and overlap nothing otherwise.
     """
     act = _act_dtype("x", x)
     dtype, shape, index = x.dtype, x.shape, x.get_device()
     x_at, x_stride = row_span("x", x, dtype, index)
-    width = shape[-1]
+    width, count = shape[-1], x.numel()
+    if count:
+        require_32_bits(count // width, width)
     weight_act = _act_dtype("weight", weight)
     if weight.shape != (width,) or not weight.is_contiguous():
         raise ValueError(f"weight must be contiguous of shape ({width},)")
@@ -101,7 +103,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
         if y.shape != shape:
             raise ValueError("out must have x's shape")
         y_at, y_stride = row_span("out", y, dtype, index)
-    count = x.numel()
     if count:
         a = _lib.VmNormArgs(x_at, r_at or None, w_at, y_at or None, s_at or None, values_at or None, scales_at or None,
                             x_stride, r_stride, y_stride, s_stride, count // width, width, act, weight_act,
@@ -117,10 +118,12 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     width = x.shape[-1]
     if width % MX_GROUP:
         raise ValueError(f"MX rows need a width that is a multiple of {MX_GROUP}")
+    rows = x.numel() // max(width, 1)
+    require_32_bits(rows, width)
     y = mx_empty(x.shape, x.device)
-    if x.numel():
+    if rows:
         _lib.check(device_call(x.get_device(), _lib.lib().vm_mx_quantize, at, stride, y.values.data_ptr(),
-                               y.scales.data_ptr(), x.numel() // width, width, act))
+                               y.scales.data_ptr(), rows, width, act))
     return y
 
 

@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import device_call, route_ids, row_span
+from .device import device_call, require_32_bits, route_ids, row_span
 from .norm import MX_GROUP, MxTensor, mx_empty, require_mx
 
 
@@ -39,7 +39,8 @@ def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, qua
     id, or [*inds.shape[:-1], k], a token's row for all its slots.  x and weight are both bfloat16 tensors (k a
     multiple of 8) or both :class:`MxTensor` (k a multiple of 32); their rows must be 16-byte aligned.  Returns
     [*inds.shape, n] in bfloat16, or as an MxTensor with ``quantize`` (swiglu only, n a multiple of 32).  The row of an
-    id outside 0..experts-1 is zero.  Up to 1024 experts.
+    id outside 0..experts-1 is zero.  Up to 1024 experts.  ``out`` overlaps no operand.  MX values enter as bfloat16:
+    those below 2^-126 are rounded to multiples of 2^-133.
     """
     mx = isinstance(x, MxTensor)
     if mx != isinstance(weight, MxTensor):
@@ -70,6 +71,8 @@ def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, qua
         x_div = max(shape[-1], 1)
     if xv.shape[-1] != k:
         raise ValueError(f"x {tuple(xv.shape)} does not fit weight {tuple(wv.shape)}")
+    rows = inds.numel()
+    require_32_bits(rows, x_div, k, wv.shape[1])
     y_at = values_at = scales_at = None
     if quantize:
         if n % MX_GROUP:
@@ -85,7 +88,6 @@ def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, qua
         else:
             y = out
         y_at = y.data_ptr()
-    rows = inds.numel()
     if rows == 0 or n == 0:
         return y
     xs_at = ws_at = None
