@@ -29,7 +29,8 @@ def _check(base, x, a, b, ids, scales=None, **kw):
 SIZES = [(1, 256, 256, 16, 4), (1, 2560, 2560, 16, 3), (5, 1000, 300, 32, 9), (128, 64, 1030, 8, 2), (17, 77, 51, 7, 5),
          (129, 256, 256, 16, 4), (200, 640, 1280, 64, 7), (333, 1000, 77, 33, 64), (300, 75, 130, 5, 3),
          (257, 128, 64, 128, 2), (400, 64, 256, 1, 1), (5000, 64, 96, 24, 40), (600, 2048, 1024, 17, 600),
-         (512, 64, 40, 12, 30), (513, 64, 40, 12, 30), (100, 256, 520, 64, 9), (101, 256, 520, 64, 9), (70, 40, 72, 96, 2)]
+         (512, 64, 40, 12, 30), (513, 64, 40, 12, 30), (100, 256, 520, 64, 9), (101, 256, 520, 64, 9), (70, 40, 72, 96, 2),
+         (2048, 64, 64, 8, 1024), (2048, 64, 72, 16, 3), (2049, 64, 64, 8, 1024), (1999, 72, 64, 40, 257)]
 
 
 @pytest.mark.parametrize("rows,k,n,rank,adapters", SIZES)

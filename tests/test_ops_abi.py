@@ -112,8 +112,8 @@ MX = {"format": _lib.VM_FORMAT_MX, "x_scales": 64, "weight_scales": 64}
     ({"x_stride": 68}, _lib.VM_EINVAL, "16-byte"),
     ({"weight_stride": 68}, _lib.VM_EINVAL, "16-byte"),
     ({"weight_expert_stride": 2052}, _lib.VM_EINVAL, "16-byte"),
-    ({"rows": 1000}, _lib.VM_EWORKSPACE, "workspace"),
-    ({"rows": 1000, "workspace": 264, "workspace_bytes": 1 << 30}, _lib.VM_EWORKSPACE, "aligned"),
+    ({"rows": 5000}, _lib.VM_EWORKSPACE, "workspace"),
+    ({"rows": 5000, "workspace": 264, "workspace_bytes": 1 << 30}, _lib.VM_EWORKSPACE, "aligned"),
     ({"rows": 1 << 28, "n": 1 << 24}, _lib.VM_EUNSUPPORTED, "too large"),
 ])
 def test_product_rejects(fields, code, message):

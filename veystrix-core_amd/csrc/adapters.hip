@@ -21,6 +21,7 @@
 
 #include "vm_dma.h"
 #include "vm_internal.h"
+#include "vm_rows.h"
 
 namespace vm {
 
@@ -157,7 +158,7 @@ __device__ __forceinline__ uint8_t* lds_side(uint32_t at) {
 
 // Rank sums of the tile, this wave's chunks w, w + 4, .. of 64 inputs.  Operands by DMA, a chunk ahead.
 template <int RF>
-__device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t id, uint32_t first_row, uint32_t rows,
+__device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t id, uint32_t tile_row,
                                               uint32_t wave, uint32_t lane, f32x4_t acc[RF]) {
   constexpr int kLoads = (kAdapterTile + 16 * RF) / 8;
   const uint32_t lm = lane & 15u, kb = lane >> 4, sub = lane / 8u;
@@ -167,7 +168,7 @@ __device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t i
   for (int i = 0; i < kLoads; ++i) {
     const uint32_t r = i * 8u + sub;
     if (i < 2) {
-      const uint32_t row = p.row_pair[first_row + min(r, rows - 1)];
+      const uint32_t row = static_cast<uint32_t>(__shfl(static_cast<int>(tile_row), r));
       src[i] = reinterpret_cast<const uint8_t*>(p.x + static_cast<uint64_t>(row) * p.x_stride) + unit;
     } else {
       const uint32_t j = min(r - kAdapterTile, p.rank - 1);
@@ -212,10 +213,10 @@ __device__ __forceinline__ void rank_sums_dma(const AdapterLaunch& p, uint32_t i
 
 // The same with every lane fetching its own operands: rows off the 16-byte units.
 template <int RF>
-__device__ __forceinline__ void rank_sums_direct(const AdapterLaunch& p, uint32_t id, uint32_t first_row, uint32_t rows,
+__device__ __forceinline__ void rank_sums_direct(const AdapterLaunch& p, uint32_t id, uint32_t tile_row,
                                                  uint32_t wave, uint32_t lane, f32x4_t acc[RF]) {
   const uint32_t lm = lane & 15u, kb = lane >> 4;
-  const uint16_t* x = p.x + static_cast<uint64_t>(p.row_pair[first_row + min(lm, rows - 1)]) * p.x_stride;
+  const uint16_t* x = p.x + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(tile_row), lm))) * p.x_stride;
   for (uint32_t c = wave * 64u; c < p.k; c += kTileWaves * 64u) {
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
@@ -252,18 +253,23 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
   }
   // each XCD takes a contiguous run of the tiles with all their splits
   const uint32_t local = (lin >> 3) / p.splits, split = (lin >> 3) % p.splits;
-  const uint32_t count = *p.tile_count, run = (count + 7) / 8;
-  const uint32_t tile = (lin & 7u) * run + local;
-  if (local >= run || tile >= count) return;
-  const RowTile td = p.tiles[tile];
+  BlockTile td;
+  if (p.tiles != nullptr) {
+    if (!listed_tile(p.tiles, p.tile_count, p.row_pair, lin & 7u, local, &td)) return;
+  } else {
+    uint32_t* words = reinterpret_cast<uint32_t*>(lds_main<0, RF>(0));
+    static_assert(kFindWords * 4 <= kTileWaves * main_bytes<RF>(), "a stage holds find_tile's words");
+    if (!find_tile<kTileThreads, kAdapterTile>(p.ids, p.rows, p.adapters, lin & 7u, local, words, &td)) return;
+  }
   const uint32_t id = td.group, rows = td.rows;
+  const auto row_of = [&](uint32_t r) { return static_cast<uint32_t>(__shfl(static_cast<int>(td.row), r)); };
   const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
 
   f32x4_t acc[RF];
 #pragma unroll
   for (int f = 0; f < RF; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  if constexpr (VEC_K) rank_sums_dma<RF>(p, id, td.row, rows, wave, lane, acc);
-  else rank_sums_direct<RF>(p, id, td.row, rows, wave, lane, acc);
+  if constexpr (VEC_K) rank_sums_dma<RF>(p, id, td.row, wave, lane, acc);
+  else rank_sums_direct<RF>(p, id, td.row, wave, lane, acc);
 
   // Strips of 64 columns.  B's rows of a strip lie side by side: one copy of 64 rank values to LDS, whose units are
   // swizzled within their rows where a row is a power of two of them; base goes to registers.  Both are fetched a strip
@@ -292,7 +298,7 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
   };
   // lane j serves eight columns of row j / 4: 32 h + 8 (j % 4) of each half h of a strip
   const uint32_t my_row = lane >> 2, sub = 8u * (lane & 3u);
-  const uint32_t out_row = p.row_pair[td.row + min(my_row, rows - 1)];
+  const uint32_t out_row = row_of(my_row);
   const uint16_t* base_row = p.base + static_cast<uint64_t>(out_row) * p.base_stride;
   uint16_t* const out = p.out + static_cast<uint64_t>(out_row) * p.out_stride;
   uint4 base[2][2];
@@ -454,6 +460,10 @@ uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least, uint32_t slot
 // us against 15.4 in sorted tiles, 100 rows of rank 64 18.9 against 21.1, 200 rows of it 28.4 against 22.2 (2560 wide).
 bool adapter_tiled(uint32_t rows, uint32_t rank) { return rows > 512 || uint64_t(rows) * rank > 6400; }
 
+// Every block of a tiled call of few rows finds its own tile: 300 rows of rank 32, 2560 wide, 12.4 us, behind a sort 17;
+// 1777 of rank 64, 2560 -> 1280, 20.4 and 24; 4000 of rank 32 28.7 and 28.3, to 10240 columns 69.8 and 67.8.
+bool adapter_sorted(uint32_t rows) { return rows > 2048; }
+
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled) {
   const uint64_t parts = (uint64_t(n) + kThreads - 1) / kThreads;
   const uint64_t units = tiled ? uint64_t(rows) / kAdapterTile + adapters + 7 : rows;
@@ -471,6 +481,7 @@ hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
     if (p.vector_k) return go(&k_adapter_rows<true, false>, blocks, kThreads, p, stream);
     return go(&k_adapter_rows<false, false>, blocks, kThreads, p, stream);
   }
+  if (p.tiles == nullptr && p.rows > kFindRounds * kTileThreads) return hipErrorInvalidValue;
   const uint32_t units = row_max_tiles(p.rows, p.adapters, kAdapterTile);
   // blocks per CU by their LDS
   const uint32_t slots = 256u * (p.rank <= 16 ? 4u : p.rank <= 32 ? 3u : p.rank <= 64 ? 2u : 1u);

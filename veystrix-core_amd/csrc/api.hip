@@ -1653,7 +1653,7 @@ static hipError_t sort_rows(const int32_t* ids, uint32_t rows, uint32_t groups, 
 
 uint64_t vm_grouped_matmul_workspace(uint32_t rows, uint32_t experts) {
   const uint32_t tile = experts == 0 ? 0 : vm::product_tile_rows(rows, experts);
-  return tile == 0 ? 0 : row_sort_ws(rows, experts, tile).total;
+  return tile == 0 || !vm::product_sorted(rows, experts) ? 0 : row_sort_ws(rows, experts, tile).total;
 }
 
 int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
@@ -1687,8 +1687,9 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   const uint32_t tile = vm::product_tile_rows(a->rows, a->experts);
   if (vm::product_blocks(a->rows, a->experts, a->n, tile, swiglu) > kMaxBlocks)
     return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
-  const RowSortWs w = tile == 0 ? RowSortWs{} : row_sort_ws(a->rows, a->experts, tile);
-  if (tile != 0 && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
+  const bool sorted = tile != 0 && vm::product_sorted(a->rows, a->experts);
+  const RowSortWs w = sorted ? row_sort_ws(a->rows, a->experts, tile) : RowSortWs{};
+  if (sorted && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
     return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
   const uint64_t x_rows = (uint64_t(a->rows) - 1) / a->x_div + 1, w_rows = uint64_t(a->n) * (swiglu ? 2 : 1);
   const auto matrices = [&](const void* at, uint64_t row, uint64_t expert, uint64_t width) {  // first to last byte
@@ -1707,7 +1708,7 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
     for (const RowBytes& in : ins)
       if (!rows_apart(out, in)) return fail(VM_EINVAL, "outputs overlap an operand");
   vm::ProductLaunch p{};
-  if (tile != 0) {
+  if (sorted) {
     vm::RowSortLaunch s{};
     const hipError_t e = sort_rows(a->ids, a->rows, a->experts, tile, w, a->workspace, stream, s);
     if (e != hipSuccess) return hip_fail(e, "sort launch");
@@ -1745,7 +1746,8 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
 // ----------------------------------------------------------- adapters ---
 
 uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t rank, uint32_t adapters) {
-  return adapters == 0 || !vm::adapter_tiled(rows, rank) ? 0 : row_sort_ws(rows, adapters, vm::kAdapterTile).total;
+  const bool sorted = adapters != 0 && vm::adapter_tiled(rows, rank) && vm::adapter_sorted(rows);
+  return sorted ? row_sort_ws(rows, adapters, vm::kAdapterTile).total : 0;
 }
 
 int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
@@ -1785,8 +1787,9 @@ int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
   p.vector_n = a->n % 8 == 0 && rows_aligned(a->base, a->base_stride * 2, 16) && rows_aligned(a->out, a->out_stride * 2, 16);
   if (vm::adapter_blocks(a->rows, a->adapters, a->n, tiled) > kMaxBlocks)
     return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
-  const RowSortWs w = tiled ? row_sort_ws(a->rows, a->adapters, vm::kAdapterTile) : RowSortWs{};
-  if (tiled && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
+  const bool sorted = tiled && vm::adapter_sorted(a->rows);
+  const RowSortWs w = sorted ? row_sort_ws(a->rows, a->adapters, vm::kAdapterTile) : RowSortWs{};
+  if (sorted && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
     return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
   const RowBytes out{a->out, a->rows, a->out_stride * 2, a->n * 2ull}, base{a->base, a->rows, a->base_stride * 2, a->n * 2ull};
   const uint64_t bank = uint64_t(a->adapters) * a->rank * 2;
@@ -1794,7 +1797,7 @@ int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
       !rows_apart(out, {a->a, 1, 0, bank * a->k}) || !rows_apart(out, {a->b, 1, 0, bank * a->n}) ||
       !rows_apart(out, {a->scales, 1, 0, a->adapters * 4ull}) || !rows_apart(out, {a->ids, 1, 0, a->rows * 4ull}))
     return fail(VM_EINVAL, "out overlaps an operand, other than base in place");
-  if (tiled) {
+  if (sorted) {
     vm::RowSortLaunch s{};
     const hipError_t e = sort_rows(a->ids, a->rows, a->adapters, vm::kAdapterTile, w, a->workspace, stream, s);
     if (e != hipSuccess) return hip_fail(e, "sort launch");

@@ -27,6 +27,7 @@
 #include "vm_dma.h"
 #include "vm_internal.h"
 #include "vm_mx.h"
+#include "vm_rows.h"
 
 namespace vm {
 
@@ -305,15 +306,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t slices = (p.n + kCols - 1) / kCols;
   const uint32_t lin = blockIdx.x, local = (lin >> 3) / slices, slice = (lin >> 3) % slices;
-  const uint32_t count = *p.tile_count, run = (count + 7) / 8;
-  const uint32_t tile = (lin & 7u) * run + local;
   if (lin >= p.tile_blocks) {
     zero_rows<OUT>(p, ((lin - p.tile_blocks) * kWaves + wave) * kZeroRows, lane);
     return;
   }
-  if (local >= run || tile >= count) return;
-  const RowTile td = p.tiles[tile];
-  const uint32_t expert = td.group, row0 = td.row, rows = td.rows;
+  BlockTile td;
+  if (p.tiles != nullptr) {
+    if (!listed_tile(p.tiles, p.tile_count, p.row_pair, lin & 7u, local, &td)) return;
+  } else {
+    uint32_t* words = reinterpret_cast<uint32_t*>(tile_stage<0, kRows + kMatrix>());
+    static_assert(kFindWords * 4 <= (kRows + kMatrix) * kChunk, "a stage holds find_tile's words");
+    if (!find_tile<64 * kWaves, kRows>(p.ids, p.rows, p.experts, lin & 7u, local, words, &td)) return;
+  }
+  const uint32_t expert = td.group, rows = td.rows;
+  const auto row_of = [&](uint32_t r) { return static_cast<uint32_t>(__shfl(static_cast<int>(td.row), r)); };
   const uint32_t col0 = slice * kCols;
   const uint8_t* w = p.w + expert * p.w_expert;
   const auto matrix_at = [&](uint32_t r) {   // matrix row of the block's row r
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
 #pragma unroll
   for (int i = 0; i < kDmaX; ++i) {
     const uint32_t r = (wave * kDmaX + i) * 8u + sub;
-    const uint32_t pair = p.row_pair[row0 + min(r, rows - 1)];
+    const uint32_t pair = row_of(r);
     at[i] = (unit ^ tile_swz(r)) * 16u;
     src[i] = p.x + static_cast<uint64_t>(pair / p.x_div) * p.x_stride + at[i];
   }
@@ -343,7 +349,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   // fetch theirs from there, so that the scales take no LDS (with a few KB of it one block less fits a CU).
   const uint8_t *xs_row = nullptr, *ws_row = nullptr;
   if constexpr (MX) {
-    const uint32_t pair = p.row_pair[row0 + min(wm * (16 * RF) + lane, rows - 1)];
+    const uint32_t pair = row_of(min(wm * (16 * RF) + lane, 63u));
     xs_row = p.x_scales + static_cast<uint64_t>(pair / p.x_div) * p.x_scale_stride;
     ws_row = p.w_scales + expert * p.w_scale_expert + matrix_at(wn * 64u + lane) * p.w_scale_stride;
   }
@@ -451,7 +457,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
 #pragma unroll
   for (int i = 0; i < RF; ++i) {
     const uint32_t r = wm * (16 * RF) + i * 16u + lm;
-    const uint32_t pair = p.row_pair[row0 + min(r, rows - 1)];
+    const uint32_t pair = row_of(r);
     store_strip<SWIGLU, OUT>(p, acc[i], col, pair, r < rows, kb);
   }
 }
@@ -489,6 +495,7 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
     constexpr int RF = decltype(rf)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
     constexpr uint32_t kWaves = WM * WN, cols = strip_cols<SWIGLU>() * WN;
     p.tile_blocks = (p.n + cols - 1) / cols * tiles;
+    if (p.tiles == nullptr && p.rows > kFindRounds * 64 * kWaves) return hipErrorInvalidValue;
     const uint32_t blocks = p.tile_blocks + (p.rows + kWaves * kZeroRows - 1) / (kWaves * kZeroRows);
     return whole ? go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, true>, blocks, 64 * kWaves, p, stream)
                  : go(&k_tiles<MX, SWIGLU, OUT, RF, WM, WN, false>, blocks, 64 * kWaves, p, stream);
@@ -522,6 +529,12 @@ uint32_t product_tile_rows(uint32_t rows, uint32_t experts) {
   if (rows <= kOneByOne) return 0;
   return rows / experts < kTallMean ? 32u : 64u;
 }
+
+// Every block of a call of few rows and experts finds its own tile: 333 tokens of four of 64 experts, 1024 -> 2 x 256,
+// 15.5 us, behind a sort 19.3; 1000 tokens 19.9 and 22.5; of 20 experts, 2 x 512, 23.4 and 25.1.  Hundreds of experts mean
+// thousands of blocks, which would all count: 32 tokens of ten of 512 experts MX 2560 -> 2 x 640 50.4 and 49.4, 200 of
+// eight of 256 176 and 174.  Tiles of 32 rows mean less than 2048 rows then, which blocks of two waves can list.
+bool product_sorted(uint32_t rows, uint32_t experts) { return rows > 4096 || experts > 128; }
 
 // Matrices that together outgrow the 256 MB Infinity Cache stream past the caches where one tile reads them (k_tiles
 // looks at each group): 2048 -> 2 x 512, ten of 512 experts, 512 tokens 364 to 336 us, eight tokens 58 to 55, 2048 tokens

@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include "vm_internal.h"
+#include "vm_rows.h"
 
 namespace vm {
 
@@ -23,42 +24,16 @@ constexpr uint32_t kThreads = 1024;
 constexpr uint32_t kPerThread = 4;
 constexpr uint32_t kBlockRows = kThreads * kPerThread;
 
-// Exclusive scans of one value per thread over the block.
+// Exclusive scan of one value per thread over the block.
 __device__ __forceinline__ uint32_t scan_1024(uint32_t v, uint32_t* s_wave) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint32_t sum = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t u = __shfl_up(sum, d, 64);
-    if (lane >= static_cast<uint32_t>(d)) sum += u;
-  }
+  const uint32_t sum = wave_scan(v);
   if (lane == 63) s_wave[wave] = sum;
   __syncthreads();
   uint32_t before = 0;
   for (uint32_t i = 0; i < wave; ++i) before += s_wave[i];
   __syncthreads();
   return before + sum - v;
-}
-
-// Adds one to a group's count for every lane with a group; with RANK returns the count before the lane's own.  Lanes of
-// one group, as in runs of rows of one request, take one addition together: 64 to one address come one after the other.
-template <bool RANK>
-__device__ __forceinline__ uint32_t count_one(uint32_t* counts, uint32_t g, uint32_t groups) {
-  const uint64_t live = __ballot(g < groups);
-  if (live == 0) return 0;
-  const uint32_t leader = static_cast<uint32_t>(__builtin_ctzll(live));
-  const uint32_t one = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(g), leader));
-  const uint32_t lane = threadIdx.x & 63u;
-  if (__ballot(g < groups && g != one) == 0) {
-    uint32_t first = 0;
-    if (lane == leader) first = atomicAdd(&counts[one], static_cast<uint32_t>(__popcll(live)));
-    if constexpr (!RANK) return 0;
-    first = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(first), leader));
-    return first + static_cast<uint32_t>(__popcll(live & ((1ull << lane) - 1)));
-  }
-  uint32_t rank = 0;
-  if (g < groups) rank = atomicAdd(&counts[g], 1u);
-  return RANK ? rank : 0;
 }
 
 __global__ __launch_bounds__(kThreads) void k_row_count(RowSortLaunch p) {

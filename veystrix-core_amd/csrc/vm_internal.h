@@ -455,6 +455,10 @@ struct RowSortLaunch {
   uint32_t rows, groups, tile_rows;
 };
 constexpr uint32_t kOneLaunchRows = 16384;
+constexpr uint32_t kMaxGroups = 1024;
+// Tiled calls whose blocks find their tiles themselves (vm_rows.h) rather than behind a sort: at most so many ids per
+// thread.
+constexpr uint32_t kFindRounds = 16;
 uint32_t row_sort_blocks(uint32_t rows);
 // Tiles of `rows` rows over `groups` groups: no group begins more than one that is not full.
 inline uint32_t row_max_tiles(uint32_t rows, uint32_t groups, uint32_t tile_rows) {
@@ -488,6 +492,8 @@ struct ProductLaunch {
 // How a call of this many routed rows runs: 0 its rows one by one, or rows per
 // tile (32 or 64) after a sort by expert.
 uint32_t product_tile_rows(uint32_t rows, uint32_t experts);
+// Whether a call in tiles needs a sort.
+bool product_sorted(uint32_t rows, uint32_t experts);
 // An upper bound of a call's blocks.
 uint64_t product_blocks(uint32_t rows, uint32_t experts, uint32_t n, uint32_t tile_rows, bool swiglu);
 hipError_t launch_products(ProductLaunch p, uint32_t tile_rows, hipStream_t stream);
@@ -506,7 +512,7 @@ struct AdapterLaunch {
   const int32_t* ids;          // [rows]
   uint16_t* out;               // [rows, n], may be base
   uint64_t base_stride, x_stride, out_stride;
-  const RowTile* tiles;        // tiled calls
+  const RowTile* tiles;        // sorted calls
   const uint32_t* tile_count;
   const uint32_t* row_pair;    // row of every sorted row
   uint32_t rows, k, n, rank, adapters;
@@ -517,6 +523,8 @@ struct AdapterLaunch {
 
 // Whether a call runs in sorted tiles rather than one block per row and column split.
 bool adapter_tiled(uint32_t rows, uint32_t rank);
+// Whether a call in tiles needs a sort.
+bool adapter_sorted(uint32_t rows);
 // An upper bound of a call's blocks.
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled);
 hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream);
