@@ -30,7 +30,8 @@ SIZES = [(1, 256, 256, 16, 4), (1, 2560, 2560, 16, 3), (5, 1000, 300, 32, 9), (1
          (129, 256, 256, 16, 4), (200, 640, 1280, 64, 7), (333, 1000, 77, 33, 64), (300, 75, 130, 5, 3),
          (257, 128, 64, 128, 2), (400, 64, 256, 1, 1), (5000, 64, 96, 24, 40), (600, 2048, 1024, 17, 600),
          (512, 64, 40, 12, 30), (513, 64, 40, 12, 30), (100, 256, 520, 64, 9), (101, 256, 520, 64, 9), (70, 40, 72, 96, 2),
-         (2048, 64, 64, 8, 1024), (2048, 64, 72, 16, 3), (2049, 64, 64, 8, 1024), (1999, 72, 64, 40, 257)]
+         (2048, 64, 64, 8, 1024), (2048, 64, 72, 16, 3), (2049, 64, 64, 8, 1024), (1999, 72, 64, 40, 257), (128, 96, 64, 16, 30), (129, 96, 64, 16, 30),
+         (7, 96, 64, 64, 30), (8, 96, 64, 64, 30), (4, 96, 264, 128, 3)]
 
 
 @pytest.mark.parametrize("rows,k,n,rank,adapters", SIZES)

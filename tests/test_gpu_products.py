@@ -41,7 +41,9 @@ def _check(x, w, inds, swiglu, quantize, shared, **kw):
 SIZES = [(1, 10, 512, 256, 64), (1, 1, 1, 32, 32), (3, 10, 64, 2048, 96), (2, 4, 9, 1056, 160),
          (8, 10, 100, 640, 320), (24, 10, 512, 256, 96), (33, 1, 7, 2048, 32), (20, 4, 64, 1088, 224),
          (90, 4, 8, 256, 64), (100, 3, 6, 160, 96), (300, 2, 9, 384, 256), (333, 4, 64, 224, 128),
-         (130, 1, 1, 512, 96), (1024, 4, 128, 96, 96), (1024, 4, 129, 96, 96), (1025, 4, 40, 96, 96), (2047, 1, 128, 64, 160), (700, 4, 16, 256, 160), (515, 2, 8, 96, 32), (1200, 4, 20, 128, 64)]
+         (130, 1, 1, 512, 96), (700, 4, 16, 256, 160), (515, 2, 8, 96, 32), (1200, 4, 20, 128, 64),
+         (1024, 4, 128, 96, 96), (1024, 4, 129, 96, 96), (1025, 4, 40, 96, 96), (2047, 1, 128, 64, 160), (20, 4, 9, 160, 96),
+         (27, 3, 9, 160, 96)]
 
 
 @pytest.mark.parametrize("mx", [False, True], ids=["bf16", "mx"])

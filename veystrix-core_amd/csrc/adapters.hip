@@ -456,9 +456,14 @@ uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least, uint32_t slot
 
 }  // namespace
 
-// Calls whose rank sums are few run one block per row and column split, without a sort: 100 / 200 rows of rank 16 11.2
-// us against 15.4 in sorted tiles, 100 rows of rank 64 18.9 against 21.1, 200 rows of it 28.4 against 22.2 (2560 wide).
-bool adapter_tiled(uint32_t rows, uint32_t rank) { return rows > 512 || uint64_t(rows) * rank > 6400; }
+// Calls whose rank sums are few run one block per row and column split, each of which computes its row's rank sums
+// itself; in tiles sixteen rows share them, but a block has to find its rows.  2560 wide, kernel time of rows and tiles:
+// rank 16, 64 / 128 / 200 rows 5.6 / 6.7 / 9.2 us and 7.3 / 7.7 / 7.7; rank 32, 32 / 64 / 100 rows 8.0 / 8.6 / 9.7 and
+// 8.5 / 8.4 / 8.5; rank 64, 2 / 8 / 32 rows 8.4 / 11.4 / 13.2 and 10.0 / 10.6 / 11.1; rank 128, 2 / 4 rows 16.1 / 19.6 and
+// 16.1 / 16.3.
+bool adapter_tiled(uint32_t rows, uint32_t rank) {
+  return rows > 512 || uint64_t(rows) * rank > (rank <= 32 ? 2048u : 480u);
+}
 
 // Every block of a tiled call of few rows finds its own tile: 300 rows of rank 32, 2560 wide, 12.4 us, behind a sort 17;
 // 1777 of rank 64, 2560 -> 1280, 20.4 and 24; 4000 of rank 32 28.7 and 28.3, to 10240 columns 69.8 and 67.8.

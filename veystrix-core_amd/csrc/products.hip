@@ -517,24 +517,25 @@ hipError_t products_go(ProductLaunch p, uint32_t tile_rows, hipStream_t stream) 
 
 }  // namespace
 
-// Rows up to which a call runs them one by one.  An expert met twice is then read twice, which sixteen tokens of ten
-// experts seldom do: 80 rows of 512 experts 58 us and 63 in sorted tiles, 128 of 64 experts 14.7 and 17.5, but 320 of
-// 512 with skewed popularity 177 and 116.
-constexpr uint32_t kOneByOne = 160;
-// Mean rows per expert from which tiles hold 64 rows rather than 32: ten of 512 experts, 2048 -> 2 x 512, 512 / 1024 /
-// 2048 tokens (10 / 20 / 40 rows) 363 / 373 / 390 us with 64 and 363 / 395 / 433 with 32.
-constexpr uint32_t kTallMean = 16;
-
-uint32_t product_tile_rows(uint32_t rows, uint32_t experts) {
-  if (rows <= kOneByOne) return 0;
-  return rows / experts < kTallMean ? 32u : 64u;
-}
-
 // Every block of a call of few rows and experts finds its own tile: 333 tokens of four of 64 experts, 1024 -> 2 x 256,
 // 15.5 us, behind a sort 19.3; 1000 tokens 19.9 and 22.5; of 20 experts, 2 x 512, 23.4 and 25.1.  Hundreds of experts mean
 // thousands of blocks, which would all count: 32 tokens of ten of 512 experts MX 2560 -> 2 x 640 50.4 and 49.4, 200 of
 // eight of 256 176 and 174.  Tiles of 32 rows mean less than 2048 rows then, which blocks of two waves can list.
 bool product_sorted(uint32_t rows, uint32_t experts) { return rows > 4096 || experts > 128; }
+
+// Rows up to which a call runs them one by one, if its tiles need a sort and if not.  An expert met twice is then read
+// twice, which sixteen tokens of ten experts seldom do: 80 rows of 512 experts 58 us and 63 in sorted tiles, but 320 with
+// skewed popularity 177 and 116.  1024 -> 2 x 512, one by one and in tiles: 64 / 96 rows of 20 experts 12.7 / 15.9 and 13.7 /
+// 13.8, of 64 experts 18.0 / 25.0 and 19.4 / 21.6, 64 / 128 rows of 128 experts 20.5 / 37.1 and 22.0 / 33.1.
+constexpr uint32_t kOneByOneSorted = 160, kOneByOneFound = 80;
+// Mean rows per expert from which tiles hold 64 rows rather than 32: ten of 512 experts, 2048 -> 2 x 512, 512 / 1024 /
+// 2048 tokens (10 / 20 / 40 rows) 363 / 373 / 390 us with 64 and 363 / 395 / 433 with 32.
+constexpr uint32_t kTallMean = 16;
+
+uint32_t product_tile_rows(uint32_t rows, uint32_t experts) {
+  if (rows <= (product_sorted(rows, experts) ? kOneByOneSorted : kOneByOneFound)) return 0;
+  return rows / experts < kTallMean ? 32u : 64u;
+}
 
 // Matrices that together outgrow the 256 MB Infinity Cache stream past the caches where one tile reads them (k_tiles
 // looks at each group): 2048 -> 2 x 512, ten of 512 experts, 512 tokens 364 to 336 us, eight tokens 58 to 55, 2048 tokens
