@@ -12,9 +12,11 @@
 //                    the second product is bound by base and out, so this is free.
 //
 // Operands come by DMA in whole 128-byte runs of their rows: loads straight in the matrix units' pattern reach 16 bytes a
-// clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, 17.4 us behind a sort of 5.6; 8192 of rank 32, 2560 ->
-// 2560, 45 behind 8.4, where x, base and out (126 MB) alone take 26.5 at the rate of a copy.  The latter has 544 tiles
-// for 768 blocks that run at once: tile after tile the waves wait for x, then for base.
+// clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, take 20.6 us, of which finding the rows 3 and, from three
+// blocks per tile that each compute the rank sums, ten; 8192 of rank 32, 2560 -> 2560, 45.7 behind a sort of 8.1, where x,
+// base and out (126 MB) alone take 26.5 at the rate of a copy: with about two tiles per CU, each block's waves wait for x,
+// then for base and B.  Rank sums in a launch of their own (20.8 to 24, 54 to 53 .. 58) and a third stage (54 to 60) were
+// no faster.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>

@@ -12,6 +12,7 @@
 //   * many rows: one wave per row, no barrier, four rows per block;
 //   * few rows, or rows wider than a wave's registers: one block of 256 threads per row, so that a row's loads are one
 //     round trip.
+// 8192 rows of 2560 with residual to MX 35.6 us (147 MB, 4.1 TB/s; a copy reaches 4.7), one row 4.2, 37 of 2048 3.2.
 // Rows that are not 16-byte aligned, or whose width is not a multiple of eight, take the same code with element loads
 // and stores, their values spread over the row's threads unless MX groups have to lie together.
 

@@ -1,5 +1,6 @@
 // Rows sorted by group on the device, for the grouped products and the adapters: the rows of every group side by side
-// and a list of tiles of up to tile_rows of them.  Rows whose id names no group are left out.
+// and a list of tiles of up to tile_rows of them.  Rows whose id names no group are left out.  Blocks of small calls find
+// their tiles without it (vm_rows.h).
 //
 // The order of a group's rows is the order in which a block's threads counted them, which changes no result: every row
 // is its own set of sums.
@@ -7,8 +8,8 @@
 // Calls of up to kOneLaunchRows rows take one launch: every block counts all ids (its own rows, those before and those
 // behind) in LDS, lays the groups out by one scan, and places its own rows; nothing has to be zeroed or waited for
 // between blocks.  Larger calls count by blocks first (a launch), and every block adds those counts up instead.
-// 1332 rows of 64 groups 5.2 us, 8192 in runs of one of 32 8.4 (22 in the four launches of the layer's sort); 81920 of
-// 512 in two launches 4.9 + 9.5.  It is bound by latency: LDS additions, a scan and the tile list one after the other.
+// 320 rows of 512 groups 4.8 us, 8192 in runs of one of 32 8.1 (22 in the four launches of the layer's sort); 81920 of
+// 512 in two launches 4.9 + 9.4.  It is bound by latency: LDS additions, a scan and the tile list one after the other.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
