@@ -12,11 +12,10 @@
 //                    the second product is bound by base and out, so this is free.
 //
 // Operands come by DMA in whole 128-byte runs of their rows: loads straight in the matrix units' pattern reach 16 bytes a
-// clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, take 20.6 us, of which finding the rows 3 and, from three
-// blocks per tile that each compute the rank sums, ten; 8192 of rank 32, 2560 -> 2560, 45.7 behind a sort of 8.1, where x,
-// base and out (126 MB) alone take 26.5 at the rate of a copy: with about two tiles per CU, each block's waves wait for x,
-// then for base and B.  Rank sums in a launch of their own (20.8 to 24, 54 to 53 .. 58) and a third stage (54 to 60) were
-// no faster.
+// clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, take 16.6 us, of which finding the rows 3; 8192 of rank 32,
+// 2560 -> 2560, 46 behind a sort of 8, where x, base and out (126 MB) alone take 26.5 at the rate of a copy: with about two
+// tiles per CU, each block's waves wait for x, then for base and B.  Rank sums in a launch of their own (53 to 58 with the
+// sort, for 54) and a third stage (60) were no faster.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
@@ -448,8 +447,7 @@ hipError_t tiles_go(const AdapterLaunch& p, uint32_t blocks, hipStream_t stream)
 }
 
 // Columns per block, a multiple of `least`: as many splits of the columns as keep the blocks of `units` rows or tiles
-// within `slots`, since every split of a unit computes its rank sums again.  For rows that is one block per CU, for tiles
-// as many as run at once.
+// within `slots`, since every split of a unit computes its rank sums again.
 uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least, uint32_t slots) {
   const uint32_t parts = (n + least - 1) / least;
   const uint32_t want = min(parts, max(1u, slots / units));
@@ -490,8 +488,10 @@ hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
   }
   if (p.tiles == nullptr && p.rows > kFindRounds * kTileThreads) return hipErrorInvalidValue;
   const uint32_t units = row_max_tiles(p.rows, p.adapters, kAdapterTile);
-  // blocks per CU by their LDS
-  const uint32_t slots = 256u * (p.rank <= 16 ? 4u : p.rank <= 32 ? 3u : p.rank <= 64 ? 2u : 1u);
+  // By their LDS four, three, two or one block run per CU; five eighths of those, since each more repeats the rank sums
+  // (all: 1777 rows of rank 64, 2560 -> 1280, 21.2 us, so 17.0; 600 of rank 64 19.2 and 15.6; 1500 of rank 32, 5120 -> 2560,
+  // 24.9 and 21.1; half: 600 rows 16.4, three quarters: 1777 rows 21.2).
+  const uint32_t slots = 160u * (p.rank <= 16 ? 4u : p.rank <= 32 ? 3u : p.rank <= 64 ? 2u : 1u);
   p.split_cols = split_columns(p.n, units, kTileWaves * kTileCols, slots);
   p.splits = (p.n + p.split_cols - 1) / p.split_cols;
   p.tile_blocks = (units + 7) / 8 * 8 * p.splits;
