@@ -488,10 +488,10 @@ hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream) {
   }
   if (p.tiles == nullptr && p.rows > kFindRounds * kTileThreads) return hipErrorInvalidValue;
   const uint32_t units = row_max_tiles(p.rows, p.adapters, kAdapterTile);
-  // By their LDS four, three, two or one block run per CU; five eighths of those, since each more repeats the rank sums
-  // (all: 1777 rows of rank 64, 2560 -> 1280, 21.2 us, so 17.0; 600 of rank 64 19.2 and 15.6; 1500 of rank 32, 5120 -> 2560,
-  // 24.9 and 21.1; half: 600 rows 16.4, three quarters: 1777 rows 21.2).
-  const uint32_t slots = 160u * (p.rank <= 16 ? 4u : p.rank <= 32 ? 3u : p.rank <= 64 ? 2u : 1u);
+  // By their LDS four, three, two or one block run per CU; five eighths of those, or the one, since each more repeats the
+  // rank sums (all: 1777 rows of rank 64, 2560 -> 1280, 21.2 us, so 17.0; 600 of rank 64 19.2 and 15.6; 1500 of rank 32,
+  // 5120 -> 2560, 24.9 and 21.1; 300 of rank 128 16.4 and 17.5; half: 600 rows 16.4, three quarters: 1777 rows 21.2).
+  const uint32_t slots = p.rank <= 16 ? 640u : p.rank <= 32 ? 480u : p.rank <= 64 ? 320u : 256u;
   p.split_cols = split_columns(p.n, units, kTileWaves * kTileCols, slots);
   p.splits = (p.n + p.split_cols - 1) / p.split_cols;
   p.tile_blocks = (units + 7) / 8 * 8 * p.splits;
