@@ -111,10 +111,15 @@ constexpr uint32_t strip_cols() {
   return SWIGLU ? 32u : 64u;
 }
 
-// silu(g) * u with the hardware exp2 and reciprocal, two or three units of fp32's last place each and one rounding to
-// the output's type behind them.
+// silu(g) * u with the hardware exp2 and reciprocal, off by 16 + 2 |g| half steps of fp32 at most (|g| of them from the
+// rounding of exp2's argument).  A negative gate's exponential comes as its root on either factor, h g and h u, so that
+// neither it nor the reciprocal, of 1 to 2, is subnormal, which the hardware flushes: from the product's own range on
+// down to gates of -174, where |silu| is 2^-244, the result keeps its bits however large u is.
 __device__ __forceinline__ float swiglu(float g, float u) {
-  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f)) * u;
+  const float h = __builtin_amdgcn_exp2f(fabsf(g) * -0x1.715476p-1f);   // e^(-|g| / 2)
+  const float r = __builtin_amdgcn_rcpf(fmaf(h, h, 1.0f));
+  const float w = g < 0.0f ? h : 1.0f;
+  return g * w * r * (w * u);
 }
 
 // Stores one strip of one 16-row fragment: a lane holds 16 (SwiGLU: 8) neighbouring outputs of its routed row.
