@@ -52,3 +52,9 @@ def test_adapter_tiles_take_no_scratch(tmp_path_factory):
         assert k["private_segment_fixed_size"] == 0, (name, k)
         if "k_adapter_tilesILi8E" not in name:
             assert k["next_free_vgpr"] <= 256 and k["group_segment_fixed_size"] <= 80 * 1024, (name, k)
+
+
+def test_no_product_instance_takes_scratch(tmp_path_factory):
+    """Rows off whole chunks included."""
+    kernels = _kernels("products.hip", tmp_path_factory)
+    assert {n: k["private_segment_fixed_size"] for n, k in kernels.items() if k["private_segment_fixed_size"]} == {}

@@ -339,19 +339,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   // swizzle costs nothing.  Rows behind the tile's last one load it again.
   const uint32_t sub = lane / 8u, unit = (lane % 8u);
   const uint8_t* src[kDmaX + kDmaW];
-  uint32_t at[kDmaX + kDmaW];   // byte of the lane's unit in a chunk
+  const uint32_t at = (unit ^ tile_swz(sub)) * 16u;   // byte of the lane's unit in a chunk, of rows sub, 8 + sub, ..
 #pragma unroll
   for (int i = 0; i < kDmaX; ++i) {
     const uint32_t r = (wave * kDmaX + i) * 8u + sub;
     const uint32_t pair = row_of(r);
-    at[i] = (unit ^ tile_swz(r)) * 16u;
-    src[i] = p.x + static_cast<uint64_t>(pair / p.x_div) * p.x_stride + at[i];
+    src[i] = p.x + static_cast<uint64_t>(pair / p.x_div) * p.x_stride + at;
   }
 #pragma unroll
   for (int i = 0; i < kDmaW; ++i) {
     const uint32_t r = (wave * kDmaW + i) * 8u + sub;
-    at[kDmaX + i] = (unit ^ tile_swz(r)) * 16u;
-    src[kDmaX + i] = w + matrix_at(r) * p.w_stride + at[kDmaX + i];
+    src[kDmaX + i] = w + matrix_at(r) * p.w_stride + at;
   }
   const uint32_t wm = wave % WM, wn = wave / WM;
   // Scales: lane j holds the chunk's four bytes of the wave's row j and of its matrix row j; the lanes of a fragment
@@ -368,7 +366,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_tiles(ProductLaunch p) {
   const auto from = [&](int i, uint32_t c) {
     const uint8_t* s = src[i] + c * kChunk;
     if constexpr (!WHOLE)
-      if (c * kChunk + at[i] >= p.k_bytes) s = zeros;
+      if (c * kChunk + at >= p.k_bytes) s = zeros;
     return s;
   };
   const bool once = p.once && td.group_rows <= kRows;
