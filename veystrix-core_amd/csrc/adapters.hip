@@ -7,9 +7,9 @@
 //                    computes the row's rank sums itself (A_i comes from the L2 for all but the first) rather than
 //                    wait for another launch.  48 rows of rank 16, 2560 -> 2560: 7.0 us.
 //   k_adapter_tiles  tiles of 16 rows sorted by adapter: the rank sums by MFMA with k split over the block's four
-//                    waves, joined in LDS, then B_i's product strip by strip, added to base.  The rank sums are split
-//                    into a bf16 value and the bf16 rest, two MFMAs, so they lose no more than 2^-16 of themselves;
-//                    the second product is bound by base and out, so this is free.
+//                    waves, joined in LDS, then B_i's product strip by strip, added to base.  The rank sums enter it as
+//                    three bf16 parts of eight bits each, three MFMAs, so they lose none of fp32's 24; the second product
+//                    is bound by base and out.
 //
 // Operands come by DMA in whole 128-byte runs of their rows: loads straight in the matrix units' pattern reach 16 bytes a
 // clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, take 16.6 us, of which finding the rows 3; 8192 of rank 32,
@@ -137,6 +137,20 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t acc) {
                                                  0, 0, 0);
 }
 
+// A rank sum as three bf16 values of its sign, cut off rather than rounded, so that none is infinite unless the sum is.
+// Where nothing is left for the second or third it takes 2^-40 of the first, not zero, whose product with an infinity of
+// B would be NaN.
+__device__ __forceinline__ void split_sum(float r, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = __float_as_uint(r) >> 16;
+  const float first = bf16_to_f32(hi), rest = r - first;
+  mid = __float_as_uint(rest) >> 16;
+  const float last = rest - bf16_to_f32(mid);
+  lo = __float_as_uint(last) >> 16;
+  const uint32_t least = __float_as_uint(first * 0x1p-40f) >> 16;
+  if (!(fabsf(rest) > 0.0f)) mid = least;   // zero, or none where the sum is infinite
+  if (!(fabsf(last) > 0.0f)) lo = least;
+}
+
 // LDS of the waves, each its own part.  For the rank sums stage J is A's 16 RF rows of a chunk (main J) and the tile's 16
 // rows of x (side J).  After them main J holds a strip of B (64 rows of at most 16 RF ranks: as many bytes), and the two
 // sides the strip's products.  Four objects, and whole offsets in one step: past a few of those the compiler no longer
@@ -237,7 +251,7 @@ template <int RF, bool VEC_K, bool VEC_R, bool VEC_N>
 __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p) {
   constexpr int kSteps = (RF + 1) / 2;                      // MFMA steps over the rank
   constexpr uint32_t kPitch = kSteps * 64 + 16;             // bytes of a row of rank sums in LDS
-  static_assert(2 * kAdapterTile * kPitch <= kTileWaves * main_bytes<RF>(), "the rank sums fit");
+  static_assert(3 * kAdapterTile * kPitch <= kTileWaves * main_bytes<RF>(), "the rank sums fit");
   const uint32_t tid = threadIdx.x, lane = tid & 63u, lm = lane & 15u, kb = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lin = blockIdx.x;
@@ -312,7 +326,7 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
     }
   };
 
-  // the waves' rank sums join: in main 0, and in main 1 their bf16 values and rests
+  // the waves' rank sums join: in main 0, and in main 1 their bf16 parts
   f32x4_t* part = reinterpret_cast<f32x4_t*>(lds_main<0, RF>(0));
   constexpr uint32_t kWavePart = main_bytes<RF>() / 16;
 #pragma unroll
@@ -321,34 +335,30 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
   load_base(0, col);
   lds_barrier();
   // lane holds rank sums 16 f + 4 kb .. +3 of its row; ranks at and behind `rank` are zero
-  uint8_t* v_hi = lds_main<1, RF>(0);
-  uint8_t* v_lo = v_hi + kAdapterTile * kPitch;
+  uint8_t* v_part = lds_main<1, RF>(0);
   for (uint32_t f = wave; f < kSteps * 2; f += kTileWaves) {
-    uint32_t hi[4], lo[4];
+    uint32_t bits[3][4];
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (f < RF) {
 #pragma unroll
       for (uint32_t w = 0; w < kTileWaves; ++w) v += part[w * kWavePart + f * 64 + lane];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float r = f * 16u + kb * 4u + i < p.rank ? v[i] * scale : 0.0f;
-      hi[i] = f32_to_bf16(r);
-      const float rest = r - bf16_to_f32(hi[i]);
-      lo[i] = __builtin_isfinite(rest) ? f32_to_bf16(rest) : 0u;  // a sum that rounds to infinity leaves no rest
-    }
+    for (int i = 0; i < 4; ++i) split_sum(f * 16u + kb * 4u + i < p.rank ? v[i] * scale : 0.0f, bits[0][i], bits[1][i], bits[2][i]);
     const uint32_t at = lm * kPitch + (f * 16u + kb * 4u) * 2u;
-    *reinterpret_cast<uint2*>(v_hi + at) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-    *reinterpret_cast<uint2*>(v_lo + at) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      *reinterpret_cast<uint2*>(v_part + q * kAdapterTile * kPitch + at) =
+          make_uint2(bits[q][0] | (bits[q][1] << 16), bits[q][2] | (bits[q][3] << 16));
   }
   lds_barrier();
   copy_b(std::integral_constant<int, 0>{}, col);
-  uint4 hi[kSteps], lo[kSteps];
+  uint4 sums[3][kSteps];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    hi[s] = *reinterpret_cast<const uint4*>(v_hi + lm * kPitch + s * 64 + kb * 16);
-    lo[s] = *reinterpret_cast<const uint4*>(v_lo + lm * kPitch + s * 64 + kb * 16);
-  }
+  for (int q = 0; q < 3; ++q)
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      sums[q][s] = *reinterpret_cast<const uint4*>(v_part + q * kAdapterTile * kPitch + lm * kPitch + s * 64 + kb * 16);
   lds_barrier();  // the rank sums have been read before a strip of B takes their place
 
   auto strip = [&](auto J) {
@@ -364,20 +374,24 @@ __global__ __launch_bounds__(kTileThreads) void k_adapter_tiles(AdapterLaunch p)
 #pragma unroll
     for (uint32_t f = 0; f < 4; ++f) {
       const uint32_t r = 16u * f + lm;
+      uint4 w[kSteps];
 #pragma unroll
       for (uint32_t s = 0; s < kSteps; ++s) {
         const uint32_t unit = s * 4u + kb;
-        uint4 w = make_uint4(0, 0, 0, 0);
+        w[s] = make_uint4(0, 0, 0, 0);
         if constexpr (VEC_R) {
-          if (unit < units) w = *reinterpret_cast<const uint4*>(
+          if (unit < units) w[s] = *reinterpret_cast<const uint4*>(
                 lds_main<j, RF>(wave * main_bytes<RF>() + (r * units + (unit ^ ((r >> shift) & mask))) * 16u));
         } else {
           const uint16_t* row = p.b + (static_cast<uint64_t>(id) * p.n + min(col + r, p.n - 1)) * p.rank;
-          w = unit_of<false>(row, unit * 8u, p.rank);
+          w[s] = unit_of<false>(row, unit * 8u, p.rank);
         }
-        y[f] = mfma(w, hi[s], y[f]);
-        y[f] = mfma(w, lo[s], y[f]);
       }
+      // the first parts of all ranks, then the others: small parts next to sums that the first ones have left
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (uint32_t s = 0; s < kSteps; ++s) y[f] = mfma(w[s], sums[q][s], y[f]);
     }
     // lane holds columns 16 f + 4 kb .. +3 of row lm, unit 4 (f % 2) + kb of half f / 2, stored at that ^ (lm % 8)
 #pragma unroll
