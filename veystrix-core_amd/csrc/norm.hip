@@ -94,11 +94,20 @@ __device__ __forceinline__ double wave_total(double v) {
   return v;
 }
 
-// h * (hi + lo) * gain of a factor given as a float and its rest: the nearest float, and what it leaves.
-__device__ __forceinline__ float exact_product(float h, float hi, float lo, float gain, float* off = nullptr) {
+// 1 + w: the nearest float, and what it leaves.
+__device__ __forceinline__ float one_plus(float w, float* rest) {
+#pragma clang fp contract(off)
+  const float g = 1.0f + w, part = g - 1.0f;
+  *rest = (1.0f - (g - part)) + (w - part);
+  return g;
+}
+
+// h * (hi + lo) * (gain + rest) of a factor and a gain given as floats and their rests: the nearest float, and what it
+// leaves.
+__device__ __forceinline__ float exact_product(float h, float hi, float lo, float gain, float rest, float* off = nullptr) {
 #pragma clang fp contract(off)
   const float s = hi * gain;
-  const float s_rest = fmaf(hi, gain, -s) + lo * gain;
+  const float s_rest = fmaf(hi, rest, fmaf(lo, gain, fmaf(hi, gain, -s)));
   const float p = h * s;
   const float p_rest = fmaf(h, s_rest, fmaf(h, s, -p));
   const float f = p + p_rest;
@@ -182,23 +191,24 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
       float g[8];
       if (p.weight_dtype == 0) load8<ActBF16, LIE>(p.weight, at(i), kStep, p.width, g);
       else load8<ActF32, LIE>(p.weight, at(i), kStep, p.width, g);
+      float g_rest[8] = {};   // of MX rows' gains
       if (!p.one_centered) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = 1.0f + g[j];
+        for (int j = 0; j < 8; ++j) g[j] = one_plus(g[j], &g_rest[j]);
       }
       if constexpr (MXOUT) {
         float y[8];
         uint32_t least = ~0u;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          y[j] = exact_product(h[i][j], hi, lo, g[j]);
+          y[j] = exact_product(h[i][j], hi, lo, g[j], g_rest[j]);
           least = min(least, __float_as_uint(y[j]) & kBorderBits);
         }
         if (least == 0) {  // seldom: one of them may lie on a border
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             float off;
-            const float f = exact_product(h[i][j], hi, lo, g[j], &off);
+            const float f = exact_product(h[i][j], hi, lo, g[j], g_rest[j], &off);
             y[j] = off_border(f, off);
           }
         }
