@@ -74,3 +74,18 @@ def test_norm_to_mx_of_random_rows(device, rows, width, centered):
     assert ((mx_value(got) - y).abs() <= step / 2 * mine.repeat_interleave(32, -1) + err).all()
     top = y.abs().unflatten(-1, (-1, 32)).amax(-1)
     assert (top * (1 - 4.1 * F32) <= 448 * mine).all() and (top * (1 + 4.1 * F32) > 224 * mine).all()
+
+
+@pytest.mark.parametrize("rows,width,pad", [(6, 64, 0), (6, 2560, 3), (1200, 512, 0), (1200, 1023, 3), (300, 16384, 0)])
+def test_norm_of_fp32_rows(device, rows, width, pad):
+    """h of whole numbers up to 8, whose squares' sum is exact in fp32: what is left are the roundings of the factor and of
+    two products, a half step each (and 2^-48 of their products)."""
+    gen = torch.Generator().manual_seed(rows + width)
+    x = torch.zeros(rows, width + pad)[:, :width]
+    x[:] = torch.randint(-8, 9, (rows, width), generator=gen).float()
+    w = 1 + 0.2 * torch.randn(width, generator=gen)
+    eps = 2.0 ** -20
+    y = x.double() / torch.sqrt(x.double().square().mean(-1, keepdim=True) + eps) * w.double()
+    got = rms_norm(x.to(device), w.to(device), eps=eps).cpu().double()
+    off = (got - y).abs() / (y.abs() * F32).clamp(min=1e-300)
+    assert off.max() <= 3.001, float(off.max())
