@@ -205,3 +205,12 @@ def test_product_rejects_outputs_over_operands(fields):
 def test_adapters_reject_outputs_over_operands(fields):
     assert _adapters(**fields) == _lib.VM_EINVAL
     assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("values,scales,x_stride", [(APART, 64, 64), (APART + 64, 64, 64), (APART - 120, 64, 64),
+                                                    (64, APART + 127, 64), (64, APART - 3, 64), (APART + 256, 64, 128)])
+def test_quantize_rejects_outputs_over_its_input(values, scales, x_stride):
+    """x: two bf16 rows of 64 at APART; rows of another stride are no way past it."""
+    lib = _lib.lib()
+    assert lib.vm_mx_quantize(APART, x_stride, values, scales, 2, 64, 0, None) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()

@@ -1599,6 +1599,11 @@ int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* s
   if (x == nullptr) return fail(VM_EINVAL, "x is required");
   const int rc = check_mx_rows(values, scales, width);
   if (rc != VM_OK) return rc;
+  const uint64_t size = act_dtype == VM_F32 ? 4 : 2;
+  const RowBytes in{x, rows, x_stride * size, width * size};
+  if (!rows_apart({values, rows, width, width}, in) ||
+      !rows_apart({scales, rows, width / VM_MX_GROUP, width / VM_MX_GROUP}, in))
+    return fail(VM_EINVAL, "MX rows overlap an operand");
   vm::NormLaunch p{};
   p.x = x;
   p.x_stride = x_stride;

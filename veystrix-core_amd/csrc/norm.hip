@@ -137,7 +137,8 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
   // MX rows: a row's factor in 64 bits (of sums of eight squares in 32) and its products with their rests.  In plain
   // fp32 about ten of 8192 x 2560 values came out on the wrong side of an e4m3 border, of these one to three; the call
   // takes 35.6 us, plain 31.3, all in 64 bits 48.
-  // Of fp32 rows to fp32 the factor comes from 64 bits too: in fp32 its mean, sum, root and quotient are a rounding each (64 bits: 0.2 us a call).
+  // Of fp32 rows to fp32 the factor comes from 64 bits too: in fp32 its mean, sum, root and quotient are a rounding each
+  // (64 bits: 0.2 us a call).
   using Real = std::conditional_t<MXOUT || A::kBytes == 4, double, float>;
   static_assert(!MXOUT || LIE != kSpread, "MX rows need a group's values side by side");
   // element of the thread's first value in step i, and between its values
