@@ -214,3 +214,17 @@ def test_quantize_rejects_outputs_over_its_input(values, scales, x_stride):
     lib = _lib.lib()
     assert lib.vm_mx_quantize(APART, x_stride, values, scales, 2, 64, 0, None) == _lib.VM_EINVAL
     assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("scales", [APART, APART + 127, APART - 3])
+def test_values_over_scales_are_rejected(scales):
+    """Two rows of 64 values at APART, two scales each."""
+    lib = _lib.lib()
+    assert lib.vm_mx_quantize(4096, 64, APART, scales, 2, 64, 0, None) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()
+    assert _norm(out=None, values=APART, scales=scales) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()
+    # n = 64: a gate/up bank of 4 x 128 rows of 64
+    assert _product(x=1 << 24, weight=1 << 25, weight_expert_stride=64 * 128, n=64, activation=1, out=None,
+                    out_values=APART, out_scales=scales) == _lib.VM_EINVAL
+    assert "overlap" in _lib.last_error()

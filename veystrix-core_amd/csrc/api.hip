@@ -1523,10 +1523,12 @@ static bool rows_apart(const RowBytes& a, const RowBytes& b) {
   return d >= a.width && d + b.width <= s;
 }
 
-static int check_mx_rows(const uint8_t* values, const uint8_t* scales, uint32_t width) {
+static int check_mx_rows(const uint8_t* values, const uint8_t* scales, uint32_t rows, uint32_t width) {
   if (values == nullptr || scales == nullptr) return fail(VM_EINVAL, "MX rows need both values and scales");
   if (width % VM_MX_GROUP) return fail(VM_EINVAL, "MX rows need a width that is a multiple of %d", VM_MX_GROUP);
   if (reinterpret_cast<uintptr_t>(values) % 8) return fail(VM_EINVAL, "MX values must be 8-byte aligned");
+  if (!rows_apart({values, 1, 0, uint64_t(rows) * width}, {scales, 1, 0, uint64_t(rows) * (width / VM_MX_GROUP)}))
+    return fail(VM_EINVAL, "MX values and scales overlap");
   return VM_OK;
 }
 
@@ -1552,7 +1554,7 @@ int vm_rms_norm(const VmNormArgs* a, void* stream) {
   const bool mx = a->values != nullptr || a->scales != nullptr;
   if (mx == (a->out != nullptr)) return fail(VM_EINVAL, "either out or MX values and scales are required");
   if (mx) {
-    const int rc = check_mx_rows(a->values, a->scales, a->width);
+    const int rc = check_mx_rows(a->values, a->scales, a->rows, a->width);
     if (rc != VM_OK) return rc;
   }
   const uint64_t w = a->width;
@@ -1597,7 +1599,7 @@ int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* s
   if (rows > kMaxBlocks) return fail(VM_EUNSUPPORTED, "at most %llu rows per call", (unsigned long long)kMaxBlocks);
   if (rows == 0) return VM_OK;
   if (x == nullptr) return fail(VM_EINVAL, "x is required");
-  const int rc = check_mx_rows(values, scales, width);
+  const int rc = check_mx_rows(values, scales, rows, width);
   if (rc != VM_OK) return rc;
   const uint64_t size = act_dtype == VM_F32 ? 4 : 2;
   const RowBytes in{x, rows, x_stride * size, width * size};
@@ -1683,7 +1685,7 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   if (mx_out == (a->out != nullptr)) return fail(VM_EINVAL, "either out or out_values and out_scales are required");
   if (mx_out) {
     if (!swiglu) return fail(VM_EUNSUPPORTED, "MX output is written by the swiglu activation");
-    const int rc = check_mx_rows(a->out_values, a->out_scales, a->n);
+    const int rc = check_mx_rows(a->out_values, a->out_scales, a->rows, a->n);
     if (rc != VM_OK) return rc;
   }
   if (!rows_aligned(a->x, a->x_stride * size, 16) || !rows_aligned(a->weight, a->weight_stride * size, 16) ||
