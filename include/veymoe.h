@@ -394,7 +394,8 @@ typedef struct VmNormArgs {
  * `out_values` 8-byte aligned; out, out_values and out_scales contiguous.
  * experts up to VM_PRODUCT_MAX_EXPERTS, k and n up to 2^24, rows up to 2^28.
  * Strides count elements (of an MX scale array: scales).  The workspace needs
- * no initialisation; calls that may run at once need one each. */
+ * no initialisation and overlaps nothing; calls that may run at once need one
+ * each. */
 #define VM_PRODUCT_MAX_EXPERTS 1024
 typedef struct VmProductArgs {
   const void* x;                 /* [ceil(rows / x_div), k] */
@@ -418,7 +419,8 @@ typedef struct VmProductArgs {
  * and out[t] = base[t] for an id outside 0..adapters-1.  out may be base, and
  * overlaps nothing otherwise.  rank up to VM_ADAPTER_MAX_RANK, adapters up to
  * VM_PRODUCT_MAX_EXPERTS, k and n up to 2^24.  Strides count elements.  The
- * workspace needs no initialisation; calls that may run at once need one each. */
+ * workspace needs no initialisation and overlaps nothing; calls that may run at
+ * once need one each. */
 #define VM_ADAPTER_MAX_RANK 128
 typedef struct VmAdapterArgs {
   const void* base;              /* [rows, n] */

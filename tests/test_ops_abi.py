@@ -228,3 +228,28 @@ def test_values_over_scales_are_rejected(scales):
     assert _product(x=1 << 24, weight=1 << 25, weight_expert_stride=64 * 128, n=64, activation=1, out=None,
                     out_values=APART, out_scales=scales) == _lib.VM_EINVAL
     assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("over", ["x", "weight", "ids", "out"])
+def test_product_rejects_a_workspace_over_its_operands(over):
+    """5000 rows sort: x 5000 x 128 bytes, the bank 4 x 32 x 128, ids 20,000 bytes, out 5000 x 64 bytes."""
+    lib = _lib.lib()
+    need = lib.vm_grouped_matmul_workspace(5000, 4)
+    at = {"x": 1 << 24, "weight": 1 << 25, "ids": 1 << 26, "out": 1 << 27}
+    size = {"x": 640000, "weight": 16384, "ids": 20000, "out": 320000}
+    assert need > 0
+    for where in (at[over], at[over] + size[over] // 32 * 16, at[over] - need // 32 * 16):
+        assert _product(rows=5000, workspace=where, workspace_bytes=need, **at) == _lib.VM_EINVAL
+        assert "the workspace overlaps an o" in _lib.last_error()
+
+
+@pytest.mark.parametrize("over", ["base", "x", "a", "b", "scales", "ids", "out"])
+def test_adapters_reject_a_workspace_over_their_operands(over):
+    lib = _lib.lib()
+    need = lib.vm_add_adapters_workspace(5000, 8, 4)
+    at = {"base": 1 << 24, "x": 1 << 25, "a": 1 << 26, "b": 1 << 27, "scales": 1 << 28, "ids": 1 << 29, "out": 1 << 30}
+    size = {"base": 320000, "x": 640000, "a": 4096, "b": 2048, "scales": 16, "ids": 20000, "out": 320000}
+    assert need > 0
+    for where in (at[over], at[over] + (size[over] - 1) // 16 * 16, at[over] - need // 32 * 16):
+        assert _adapters(rows=5000, workspace=where, workspace_bytes=need, **at) == _lib.VM_EINVAL
+        assert "the workspace overlaps an o" in _lib.last_error()

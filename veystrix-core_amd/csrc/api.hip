@@ -1714,6 +1714,11 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   for (const RowBytes& out : outs)
     for (const RowBytes& in : ins)
       if (!rows_apart(out, in)) return fail(VM_EINVAL, "outputs overlap an operand");
+  const RowBytes scratch{sorted ? a->workspace : nullptr, 1, 0, w.total};
+  for (const RowBytes& out : outs)
+    if (!rows_apart(scratch, out)) return fail(VM_EINVAL, "the workspace overlaps an output");
+  for (const RowBytes& in : ins)
+    if (!rows_apart(scratch, in)) return fail(VM_EINVAL, "the workspace overlaps an operand");
   vm::ProductLaunch p{};
   if (sorted) {
     vm::RowSortLaunch s{};
@@ -1800,10 +1805,17 @@ int vm_add_adapters(const VmAdapterArgs* a, void* stream_ptr) {
     return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
   const RowBytes out{a->out, a->rows, a->out_stride * 2, a->n * 2ull}, base{a->base, a->rows, a->base_stride * 2, a->n * 2ull};
   const uint64_t bank = uint64_t(a->adapters) * a->rank * 2;
-  if (!(same_rows(out, base) || rows_apart(out, base)) || !rows_apart(out, {a->x, a->rows, a->x_stride * 2, a->k * 2ull}) ||
-      !rows_apart(out, {a->a, 1, 0, bank * a->k}) || !rows_apart(out, {a->b, 1, 0, bank * a->n}) ||
-      !rows_apart(out, {a->scales, 1, 0, a->adapters * 4ull}) || !rows_apart(out, {a->ids, 1, 0, a->rows * 4ull}))
+  const RowBytes ins[] = {{a->x, a->rows, a->x_stride * 2, a->k * 2ull}, {a->a, 1, 0, bank * a->k}, {a->b, 1, 0, bank * a->n},
+                          {a->scales, 1, 0, a->adapters * 4ull}, {a->ids, 1, 0, a->rows * 4ull}};
+  if (!(same_rows(out, base) || rows_apart(out, base)))
     return fail(VM_EINVAL, "out overlaps an operand, other than base in place");
+  for (const RowBytes& in : ins)
+    if (!rows_apart(out, in)) return fail(VM_EINVAL, "out overlaps an operand, other than base in place");
+  const RowBytes scratch{sorted ? a->workspace : nullptr, 1, 0, w.total};
+  if (!rows_apart(scratch, out)) return fail(VM_EINVAL, "the workspace overlaps an output");
+  if (!rows_apart(scratch, base)) return fail(VM_EINVAL, "the workspace overlaps an operand");
+  for (const RowBytes& in : ins)
+    if (!rows_apart(scratch, in)) return fail(VM_EINVAL, "the workspace overlaps an operand");
   if (sorted) {
     vm::RowSortLaunch s{};
     const hipError_t e = sort_rows(a->ids, a->rows, a->adapters, vm::kAdapterTile, w, a->workspace, stream, s);
