@@ -1688,8 +1688,11 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
     const int rc = check_mx_rows(a->out_values, a->out_scales, a->rows, a->n);
     if (rc != VM_OK) return rc;
   }
-  if (!rows_aligned(a->x, a->x_stride * size, 16) || !rows_aligned(a->weight, a->weight_stride * size, 16) ||
-      a->weight_expert_stride * size % 16)
+  const uint64_t x_rows = (uint64_t(a->rows) - 1) / a->x_div + 1, w_rows = uint64_t(a->n) * (swiglu ? 2 : 1);
+  // a stride that leads to no row aligns none
+  if (!rows_aligned(a->x, x_rows > 1 ? a->x_stride * size : 0, 16) ||
+      !rows_aligned(a->weight, w_rows > 1 ? a->weight_stride * size : 0, 16) ||
+      (a->experts > 1 && a->weight_expert_stride * size % 16))
     return fail(VM_EINVAL, "rows of x and weight must be 16-byte aligned");
   const uint32_t tile = vm::product_tile_rows(a->rows, a->experts);
   if (vm::product_blocks(a->rows, a->experts, a->n, tile, swiglu) > kMaxBlocks)
@@ -1698,7 +1701,6 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   const RowSortWs w = sorted ? row_sort_ws(a->rows, a->experts, tile) : RowSortWs{};
   if (sorted && (a->workspace == nullptr || a->workspace_bytes < w.total || !aligned16(a->workspace)))
     return fail(VM_EWORKSPACE, "16-byte aligned workspace of %llu bytes needed", (unsigned long long)w.total);
-  const uint64_t x_rows = (uint64_t(a->rows) - 1) / a->x_div + 1, w_rows = uint64_t(a->n) * (swiglu ? 2 : 1);
   const auto matrices = [&](const void* at, uint64_t row, uint64_t expert, uint64_t width) {  // first to last byte
     return RowBytes{at, 1, 0, ((a->experts - 1) * expert + (w_rows - 1) * row) + width};
   };
