@@ -41,3 +41,28 @@ def test_swiglu_of_gates_far_below_zero(device, tokens, quantize, mx):
         assert_mx_within(MxTensor(*(t.view(tokens, -1) for t in got)), want, err)
     else:
         assert_within(got.view(tokens, n), want, err + (want.abs() + err) * HALF_STEP[torch.bfloat16])
+
+
+@pytest.mark.parametrize("mx", [False, True], ids=["bf16", "mx"])
+@pytest.mark.parametrize("tokens", [3, 70, 300, 2500])
+@pytest.mark.parametrize("k", [32, 96, 256, 2560])
+def test_terms_that_cancel(device, k, tokens, mx):
+    """Every group of 32 holds 256, -256 and m 2^-9, m up to 3, and the matrix ones of either sign: sums of whole multiples of
+    2^-9 below 2^15, exact in fp32 in any order, and m 2^-9 times the groups (up to 80), exact in bf16.  A product that drops
+    what is below 2^-16 of a group's largest term finds nothing."""
+    n, experts = 40, 3
+    m = (torch.arange(tokens) % 3 + 1).float()
+    gen = torch.Generator().manual_seed(k + tokens)
+    x = torch.zeros(tokens, k // 32, 32)
+    at = torch.rand((tokens, k // 32, 32), generator=gen).argsort(-1)[..., :3]
+    x.scatter_(2, at, torch.stack([torch.full_like(m, 256), torch.full_like(m, -256), m * 2.0 ** -9], -1)[:, None].expand_as(at))
+    sign = torch.where(torch.arange(n) % 2 == 0, 1.0, -1.0)
+    w = sign[:, None].expand(experts, n, k)
+    x, w = x.view(tokens, k).bfloat16().to(device), w.bfloat16().contiguous().to(device)
+    if mx:
+        wide = x
+        x, w = mx_quantize(x), mx_quantize(w)
+        assert torch.equal(x.dequantize(torch.bfloat16), wide)
+    inds = (torch.arange(tokens) % experts).int().reshape(-1, 1).to(device)
+    want = m[:, None] * (k // 32) * 2.0 ** -9 * sign
+    assert torch.equal(grouped_matmul(x, w, inds).view(tokens, n).float().cpu(), want)
