@@ -353,14 +353,16 @@ typedef struct VmGroupedArgs {
  * even.  A group with an infinity or a NaN has scale 0xff and NaN values. */
 #define VM_MX_GROUP 32
 
-/* vm_rms_norm: per row, fp32 throughout and rounded once where it is stored,
+/* vm_rms_norm: per row, in fp32,
  *   h   = x + residual                        (residual NULL: h = x)
  *   out = h / sqrt(mean(h^2) + eps) * gain    gain = weight (one_centered) or 1 + weight
  * as `out` [rows, width] in act_dtype, or as MX rows `values` [rows, width] and
  * `scales` [rows, width / 32], contiguous (width a multiple of 32, values
- * 8-byte aligned).  `sum_out` optionally receives h in act_dtype.  out and
+ * 8-byte aligned).  fp32 and MX rows take the row's factor from 64 bits (of
+ * sums of eight squares in fp32), and MX rows' products keep what fp32 would
+ * drop, so that e4m3's is their one rounding behind h.  `sum_out` optionally receives h in act_dtype.  out and
  * sum_out may each be x or residual, row for row; outputs overlap nothing
- * otherwise.  Strides count elements between rows.
+ * otherwise, each other included.  Strides count elements between rows.
  * width up to VM_NORM_MAX_WIDTH.  No counterpart in the reference's surface
  * beyond its norm (patch_rmsnorm.py:108-135). */
 #define VM_NORM_MAX_WIDTH 16384
@@ -389,7 +391,8 @@ typedef struct VmNormArgs {
  * out = silu(gate) * up in fp32.  bf16 or MX operands (both the same), output
  * in bf16 or, with swiglu and n a multiple of 32, as MX rows.  An id outside
  * 0..experts-1 gives a row of zeros.  MX values enter as bf16: those below
- * 2^-126 are rounded to multiples of 2^-133.  Outputs overlap no operand.
+ * 2^-126 are rounded to multiples of 2^-133, those of 2^128 and above are
+ * infinite.  Outputs overlap no operand and not each other.
  * k: a multiple of 8 (bf16) or 32 (MX); rows of x and weight 16-byte aligned,
  * `out_values` 8-byte aligned; out, out_values and out_scales contiguous.
  * experts up to VM_PRODUCT_MAX_EXPERTS, k and n up to 2^24, rows up to 2^28.

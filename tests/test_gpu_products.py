@@ -36,7 +36,7 @@ def _check(x, w, inds, swiglu, quantize, shared, **kw):
     return got
 
 
-# tokens, slots, experts, k, n: rows one by one (short and long k), tiles of 16, 64 and 128 rows, with full and ragged
+# tokens, slots, experts, k, n: rows one by one (short and long k), tiles of 32 and 64 rows, with full and ragged
 # last tiles, k of whole chunks or not, n off every tile size, one expert, more experts than rows
 SIZES = [(1, 10, 512, 256, 64), (1, 1, 1, 32, 32), (3, 10, 64, 2048, 96), (2, 4, 9, 1056, 160),
          (8, 10, 100, 640, 320), (24, 10, 512, 256, 96), (33, 1, 7, 2048, 32), (20, 4, 64, 1088, 224),

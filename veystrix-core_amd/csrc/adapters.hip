@@ -5,17 +5,18 @@
 // Two forms:
 //   k_adapter_rows   a block per row and column split: decode, where every row has an adapter of its own.  Each block
 //                    computes the row's rank sums itself (A_i comes from the L2 for all but the first) rather than
-//                    wait for another launch.  48 rows of rank 16, 2560 -> 2560: 7.0 us.
+//                    wait for another launch.  64 rows of rank 16, 2560 -> 2560: 6.3 us.
 //   k_adapter_tiles  tiles of 16 rows sorted by adapter: the rank sums by MFMA with k split over the block's four
 //                    waves, joined in LDS, then B_i's product strip by strip, added to base.  The rank sums enter it as
 //                    three bf16 parts of eight bits each, three MFMAs, so they lose none of fp32's 24; the second product
 //                    is bound by base and out.
 //
 // Operands come by DMA in whole 128-byte runs of their rows: loads straight in the matrix units' pattern reach 16 bytes a
-// clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, take 16.6 us, of which finding the rows 3; 8192 of rank 32,
+// clock and CU, these 55.  1777 rows of rank 64, 2560 -> 1280, take 16.7 us, of which finding the rows 2; 8192 of rank 32,
 // 2560 -> 2560, 46 behind a sort of 8, where x, base and out (126 MB) alone take 26.5 at the rate of a copy: with about two
 // tiles per CU, each block's waves wait for x, then for base and B.  Rank sums in a launch of their own (53 to 58 with the
-// sort, for 54) and a third stage (60) were no faster.
+// sort, for 54) and a third stage (60) were no faster.  Rows off the vector units move by elements: 600 of rank 33, 2560
+// wide, 18.1 us (of rank 40 14.1), 600 of rank 32, 2555 wide, 91 (2560 wide 13.2).
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
@@ -471,16 +472,17 @@ uint32_t split_columns(uint32_t n, uint32_t units, uint32_t least, uint32_t slot
 }  // namespace
 
 // Calls whose rank sums are few run one block per row and column split, each of which computes its row's rank sums
-// itself; in tiles sixteen rows share them, but a block has to find its rows.  2560 wide, kernel time of rows and tiles:
-// rank 16, 64 / 128 / 200 rows 5.6 / 6.7 / 9.2 us and 7.3 / 7.7 / 7.7; rank 32, 32 / 64 / 100 rows 8.0 / 8.6 / 9.7 and
-// 8.5 / 8.4 / 8.5; rank 64, 2 / 8 / 32 rows 8.4 / 11.4 / 13.2 and 10.0 / 10.6 / 11.1; rank 128, 2 / 4 rows 16.1 / 19.6 and
-// 16.1 / 16.3.
+// itself; in tiles sixteen rows share them, but a block has to find its rows.  2560 wide, 16 adapters, kernel time of rows
+// and tiles: rank 16, 64 / 128 / 200 rows 6.3 / 7.3 / 9.5 us and 7.8 / 7.8 / 8.0; rank 32, 32 / 64 / 100 rows 8.1 / 9.0 / 10.0
+// and 8.7 / 8.6 / 9.0; rank 64, 2 / 8 / 32 rows 8.3 / 11.5 / 13.3 and 10.0 / 10.7 / 12.1; rank 128, 2 / 4 rows 19.0 / 19.6 and
+// 15.9 / 16.6.
 bool adapter_tiled(uint32_t rows, uint32_t rank) {
   return rows > 512 || uint64_t(rows) * rank > (rank <= 32 ? 2048u : 480u);
 }
 
-// Every block of a tiled call of few rows finds its own tile: 300 rows of rank 32, 2560 wide, 12.4 us, behind a sort 17;
-// 1777 of rank 64, 2560 -> 1280, 20.4 and 24; 4000 of rank 32 28.7 and 28.3, to 10240 columns 69.8 and 67.8.
+// Every block of a tiled call of few rows finds its own tile: 300 rows of rank 32, 2560 wide, 9.8 us, behind a sort 4.2 +
+// 8.9; 1777 of rank 64, 2560 -> 1280, 16.6 and 5.1 + 14.4; 2560 of rank 32 20.6 and 5.5 + 16.5; 4000 26.3 and 6.1 + 20.6, to
+// 10240 columns 87.6 and 6.8 + 81.0.
 bool adapter_sorted(uint32_t rows) { return rows > 2048; }
 
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled) {

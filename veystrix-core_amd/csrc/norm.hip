@@ -3,16 +3,18 @@
 //   h = x + residual                       fp32; stored rounded to the input's type where sum_out is given
 //   y = h * (1 / sqrt(mean(h^2) + eps)) * gain, gain = weight or 1 + weight
 //
-// The norm reads the unrounded h: the sum is rounded once, where it is stored.  y is rounded once, to the input's
-// type or to e4m3 under the scale of its group of 32.  Without a weight the rows are only converted to MX.
+// The norm reads h as fp32 holds it, before it is rounded to a stored sum.  y is rounded to the input's type, or to e4m3
+// under the scale of its group of 32.  Without a weight the rows are only converted to MX.
 //
 // A row is read once and stays in registers, eight consecutive values per thread and step, so that four lanes hold a
 // scale's group and its maximum takes two DPP steps.  Calls are bound by HBM (two rows in, one and a half out, five
-// operations a value) or, with few rows, by one row's latency:
+// operations a value), to MX by the compensated products that keep values on their side of e4m3's borders, or, with few
+// rows, by one row's latency:
 //   * many rows: one wave per row, no barrier, four rows per block;
 //   * few rows, or rows wider than a wave's registers: one block of 256 threads per row, so that a row's loads are one
 //     round trip.
-// 8192 rows of 2560 with residual to MX 35.6 us (147 MB, 4.1 TB/s; a copy reaches 4.7), one row 4.2, 37 of 2048 3.2.
+// 8192 rows of 2560 with residual to MX 35.5 to 36.5 us (147 MB, 4.1 TB/s; with plain fp32 products 31.3, the 4.7 of a
+// copy), one row 4.2, 37 of 2048 3.3.
 // Rows that are not 16-byte aligned, or whose width is not a multiple of eight, take the same code with element loads
 // and stores, their values spread over the row's threads unless MX groups have to lie together.
 
@@ -31,8 +33,9 @@ namespace {
 constexpr int kNormThreads = 256;
 
 // How a thread's eight values of a step lie in a row: consecutive ones moved as 16-byte units or one by one, or spread
-// over the row's threads, so that those moved one by one are neighbours across lanes (3000 rows of 3333 bf16 values
-// 33 us, eight of them side by side 54).
+// over the row's threads, so that those moved one by one are neighbours across lanes (3000 rows of 3333 bf16 values and a
+// residual 31 to 33 us, eight of them side by side 54; the bytes alone take 17 at a copy's rate, but every value is a load
+// of its own, and eight steps of them hold so many registers that one wave runs per SIMD).
 enum : int { kUnits = 0, kOnes = 1, kSpread = 2 };
 
 // The eight values of the step at element `at`; those at `width` and behind it are zero.
@@ -135,8 +138,8 @@ __global__ __launch_bounds__(kNormThreads) void k_norm(NormLaunch p) {
     return static_cast<const uint8_t*>(base) + static_cast<uint64_t>(row) * stride * A::kBytes;
   };
   // MX rows: a row's factor in 64 bits (of sums of eight squares in 32) and its products with their rests.  In plain
-  // fp32 about ten of 8192 x 2560 values came out on the wrong side of an e4m3 border, of these one to three; the call
-  // takes 35.6 us, plain 31.3, all in 64 bits 48.
+  // fp32 7 to 22 of 8192 x 2560 values came out on the wrong side of an e4m3 border, of these one to four; the call takes
+  // 36 us, plain 31.3, all in 64 bits 48.
   // Of fp32 rows to fp32 the factor comes from 64 bits too: in fp32 its mean, sum, root and quotient are a rounding each
   // (64 bits: 0.2 us a call).
   using Real = std::conditional_t<MXOUT || A::kBytes == 4, double, float>;

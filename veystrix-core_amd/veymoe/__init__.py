@@ -10,6 +10,9 @@ Public surface (reference counterparts in joyboyreturns/Veystrix-Core):
   ExpertPool / HostRecordStore                              expert_pool.py
   RecordLayout                                              slab_pack.py
   router_topk                                               compiled.py
+  norm.rms_norm / mx_quantize / MxTensor                    patch_rmsnorm.py (MX rows: none)
+  products.grouped_matmul (bf16 and MX experts)             the gather_qmm call of expert_cache.py
+  adapters.add_adapters                                     none
 """
 from .executor import (BITS, GROUP_SIZE, MAX_EXPERTS, MAX_TOKENS, MAX_TOP_K, MAX_WIDTH, HipCapabilities,
                        HipMoEExecutor, Q4G32Projection, probe_capabilities, weighted_combine)

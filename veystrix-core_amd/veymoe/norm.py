@@ -4,8 +4,9 @@ MX rows (:class:`MxTensor`) hold e4m3 values with one power-of-two scale (e8m0) 
 least 2^e, e >= -127, that keeps the group's largest magnitude within e4m3's 448, so that no value saturates.  A group
 that holds an infinity or a NaN is NaN.  ``grouped_matmul`` multiplies them on the matrix cores, scales included.
 
-The norm is the reference's hc_norm arithmetic (patch_rmsnorm.py:108-135) in fp32 from end to end, rounded once where a
-value is stored; the reference has no 8-bit output.
+The norm is the reference's hc_norm arithmetic (patch_rmsnorm.py:108-135) in fp32, rounded where a value is stored; fp32
+and MX rows take the row's factor from 64 bits, and MX rows' products keep what fp32 would drop, so that e4m3's is the one
+rounding behind the fp32 sum x + residual.  The reference has no 8-bit output.
 """
 from __future__ import annotations
 

@@ -40,7 +40,7 @@ def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, qua
     multiple of 8) or both :class:`MxTensor` (k a multiple of 32); their rows must be 16-byte aligned.  Returns
     [*inds.shape, n] in bfloat16, or as an MxTensor with ``quantize`` (swiglu only, n a multiple of 32).  The row of an
     id outside 0..experts-1 is zero.  Up to 1024 experts.  ``out`` overlaps no operand.  MX values enter as bfloat16:
-    those below 2^-126 are rounded to multiples of 2^-133.
+    those below 2^-126 are rounded to multiples of 2^-133, those of 2^128 and above are infinite.
     """
     mx = isinstance(x, MxTensor)
     if mx != isinstance(weight, MxTensor):
