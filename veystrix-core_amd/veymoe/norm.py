@@ -6,7 +6,8 @@ that holds an infinity or a NaN is NaN.  ``grouped_matmul`` multiplies them on t
 
 The norm is the reference's hc_norm arithmetic (patch_rmsnorm.py:108-135) in fp32, rounded where a value is stored; fp32
 and MX rows take the row's factor from 64 bits, and MX rows' products keep what fp32 would drop, so that e4m3's is the one
-rounding behind the fp32 sum x + residual.  The reference has no 8-bit output.
+rounding behind the fp32 sum x + residual.  Squares are fp32: a row whose squares pass its range (values of 2^57 and
+above) may come out as zeros.  The reference has no 8-bit output.
 """
 from __future__ import annotations
 
