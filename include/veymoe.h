@@ -361,9 +361,10 @@ typedef struct VmGroupedArgs {
  * 8-byte aligned).  fp32 and MX rows take the row's factor from 64 bits (of
  * sums of eight squares in fp32), and MX rows' products keep what fp32 would
  * drop, so that e4m3's is their one rounding behind h.  Squares are fp32: a row
- * whose squares pass its range (values of 2^57 and above) may come out as zeros.  `sum_out` optionally receives h in act_dtype.  out and
- * sum_out may each be x or residual, row for row; outputs overlap nothing
- * otherwise, each other included.  Strides count elements between rows.
+ * whose squares pass its range (values of 2^57 and above) may come out as
+ * zeros.  `sum_out` optionally receives h in act_dtype.  out and sum_out may
+ * each be x or residual, row for row; outputs overlap nothing otherwise, each
+ * other included.  Strides count elements between rows.
  * width up to VM_NORM_MAX_WIDTH.  No counterpart in the reference's surface
  * beyond its norm (patch_rmsnorm.py:108-135). */
 #define VM_NORM_MAX_WIDTH 16384
