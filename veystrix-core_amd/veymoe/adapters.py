@@ -56,9 +56,9 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         scales_at = scales.data_ptr()
     if out is None:
         out = torch.empty_like(base)
-    elif out.shape != shape:
-        raise ValueError("out must have base's shape")
     out_at, out_stride = row_span("out", out, _BF16, index)
+    if out.shape != shape:
+        raise ValueError("out must have base's shape")
     if rows == 0 or n == 0:
         return out
     lib = _lib.lib()

@@ -44,8 +44,8 @@ def mx_empty(shape, device) -> MxTensor:
 
 
 def require_mx(name: str, t) -> MxTensor:
-    if not isinstance(t, MxTensor):
-        raise TypeError(f"{name} must be an MxTensor")
+    if not isinstance(t, MxTensor) or not all(isinstance(part, torch.Tensor) for part in t):
+        raise TypeError(f"{name} must be an MxTensor of two tensors")
     if t.values.dtype != torch.float8_e4m3fn or t.scales.dtype not in _SCALE_DTYPES:
         raise TypeError(f"{name} must hold float8_e4m3fn values and float8_e8m0fnu (or uint8) scales")
     if t.values.shape[-1] % MX_GROUP or t.scales.shape != (*t.values.shape[:-1], t.values.shape[-1] // MX_GROUP):
@@ -83,14 +83,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     w_at, _ = row_span("weight", weight, weight.dtype, index)
     r_at = r_stride = s_at = s_stride = y_at = y_stride = values_at = scales_at = 0
     if residual is not None:
-        if residual.shape != shape:
-            raise ValueError("residual must have x's shape")
         r_at, r_stride = row_span("residual", residual, dtype, index)
         if residual_out is None:
             residual_out = torch.empty_like(x)
-        elif residual_out.shape != shape:
-            raise ValueError("residual_out must have x's shape")
         s_at, s_stride = row_span("residual_out", residual_out, dtype, index)
+        if residual.shape != shape or residual_out.shape != shape:
+            raise ValueError("residual and residual_out must have x's shape")
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     if quantize:
@@ -102,9 +100,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
         values_at, scales_at = y[0].data_ptr(), y[1].data_ptr()
     else:
         y = torch.empty_like(x) if out is None else out
+        y_at, y_stride = row_span("out", y, dtype, index)
         if y.shape != shape:
             raise ValueError("out must have x's shape")
-        y_at, y_stride = row_span("out", y, dtype, index)
     if count:
         a = _lib.VmNormArgs(x_at, r_at or None, w_at, y_at or None, s_at or None, values_at or None, scales_at or None,
                             x_stride, r_stride, y_stride, s_stride, count // width, width, act, weight_act,

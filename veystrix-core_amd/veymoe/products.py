@@ -82,6 +82,8 @@ def grouped_matmul(x, weight, inds: torch.Tensor, *, activation: str = None, qua
     else:
         if out is None:
             y = torch.empty((*shape, n), dtype=torch.bfloat16, device=xv.device)
+        elif not isinstance(out, torch.Tensor):
+            raise TypeError(f"out must be a torch tensor, got {type(out).__name__}")
         elif out.shape != (*shape, n) or out.dtype != torch.bfloat16 or not out.is_contiguous() \
                 or out.device != xv.device:
             raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {(*shape, n)} on {xv.device}")
