@@ -381,6 +381,43 @@ typedef struct VmNormArgs {
   float eps;
 } VmNormArgs;
 
+/* vm_block_norm: the norms before and after a block's boundary with its gate,
+ * scale and residual, per row:
+ *   n = x / sqrt(mean(x^2) + eps) * post gain        (post_weight NULL: n = x)
+ *   h = residual_scale * residual + scale * gate * n
+ *   y = h / sqrt(mean(h^2) + eps) * gain             (weight NULL: h alone)
+ * gain = weight (one_centered) or 1 + weight.  gate by gate_kind: none (1), one
+ * value per row [rows] (gate_stride apart), per channel [width] or per value
+ * [rows, width], through 1 / (1 + e^-gate) with sigmoid_gate.  `sum_out`
+ * receives h in residual_dtype (optional where a weight is given); y goes to
+ * `out` [rows, width] in act_dtype or to MX rows `values` and `scales` as of
+ * vm_rms_norm (width a multiple of 32, values 8-byte aligned).  Sums of squares
+ * are 64 bits, the rest fp32; to MX everything is 64 bits, so that e4m3's is
+ * the values' one rounding.  The second norm reads the unrounded h.  out and
+ * sum_out may each be x or residual, row for row, where their types are of one
+ * size; outputs overlap nothing otherwise, each other included.  Strides count
+ * elements between rows.  width up to VM_NORM_MAX_WIDTH.  No counterpart in the
+ * reference. */
+#define VM_GATE_NONE 0u
+#define VM_GATE_ROW 1u
+#define VM_GATE_CHANNEL 2u
+#define VM_GATE_VALUE 3u
+typedef struct VmBlockNormArgs {
+  const void* x;                 /* [rows, width] act_dtype */
+  const void* residual;          /* [rows, width] residual_dtype */
+  const void* post_weight;       /* optional [width] post_dtype */
+  const void* gate;              /* by gate_kind, gate_dtype */
+  const void* weight;            /* optional [width] weight_dtype */
+  void* out;
+  void* sum_out;
+  uint8_t* values;
+  uint8_t* scales;
+  uint64_t x_stride, residual_stride, gate_stride, out_stride, sum_stride;
+  double scale, residual_scale, eps;
+  uint32_t rows, width, act_dtype, residual_dtype, post_dtype, gate_dtype, weight_dtype;
+  uint32_t gate_kind, sigmoid_gate, one_centered;
+} VmBlockNormArgs;
+
 /* Element formats of vm_grouped_matmul's operands. */
 #define VM_FORMAT_BF16 0u
 #define VM_FORMAT_MX 1u
@@ -441,6 +478,71 @@ typedef struct VmAdapterArgs {
   uint32_t rows, k, n, rank, adapters;
 } VmAdapterArgs;
 
+/* vm_linear: a matrix product with its epilogue, fp32 sums:
+ *   out = activation(x . weight^T + bias) + residual
+ * VM_ACTIVATION_SWIGLU: weight and bias have 2 n rows, gate then up, and the
+ * activation is silu(gate) * up.  gelu is x Phi(x), gelu_tanh its tanh form.
+ * x and weight are both bf16 or both MX; out and residual are bf16 or fp32, the
+ * epilogue fp32 with one rounding at the end.  MX values enter as bf16: those
+ * below 2^-126 are rounded to multiples of 2^-133, those of 2^128 and above are
+ * infinite.  out may be residual, row for row, where their types are one, and
+ * overlaps nothing otherwise.  k: a multiple of 8 (bf16) or 32 (MX); rows of x
+ * and weight 16-byte aligned.  k and n up to 2^24, rows up to 2^28.  Strides
+ * count elements (of an MX scale array: scales).  A call repeats itself bit for
+ * bit.  No counterpart in the reference. */
+#define VM_ACTIVATION_RELU 2u
+#define VM_ACTIVATION_SILU 3u
+#define VM_ACTIVATION_GELU 4u
+#define VM_ACTIVATION_GELU_TANH 5u
+#define VM_ACTIVATION_SIGMOID 6u
+typedef struct VmLinearArgs {
+  const void* x;                 /* [rows, k] */
+  const uint8_t* x_scales;       /* MX: [rows, k / 32] */
+  const void* weight;            /* [n or 2 n, k] */
+  const uint8_t* weight_scales;  /* MX: [n or 2 n, k / 32] */
+  const void* bias;              /* optional [n or 2 n] bias_dtype */
+  const void* residual;          /* optional [rows, n] residual_dtype */
+  void* out;                     /* [rows, n] out_dtype */
+  uint64_t x_stride, x_scale_stride, weight_stride, weight_scale_stride, residual_stride, out_stride;
+  uint32_t rows, k, n, format, activation, bias_dtype, residual_dtype, out_dtype;
+} VmLinearArgs;
+
+/* vm_select_experts: from a router's logits to experts and weights, per row
+ * (choices in 64 bits):
+ *   score  = VM_SCORES_SOFTMAX: softmax over the open experts (those whose logit
+ *            is above -infinity); VM_SCORES_SIGMOID: 1 / (1 + e^-logit)
+ *   choice = score + bias; without a bias the logit, which orders the experts
+ *            as their scores do even where scores are too small to differ
+ *   groups > 1: the experts are `groups` ranges of neighbours; a group's rank is
+ *            the sum of the choices (without a bias: logit for group_top 1,
+ *            scores for 2) of its group_top best open experts, and only the
+ *            top_groups groups of the largest rank are chosen from
+ *   inds   = the top_k open experts of the largest choice, in that order
+ *   weights = score / sum of the chosen scores (renormalize; 0 where that sum
+ *            is 0) or score, times factor, rounded once
+ * Of equal choices, and of equal groups, the lowest index goes first.  A choice
+ * of -infinity closes an expert, too.  Slots that find no open expert hold -1
+ * and weight 0.  NaN choices go before all others; a row with a NaN or +infinity
+ * has NaN softmax scores.  Strides count elements; inds and weights are
+ * contiguous and overlap nothing.  The reference's router has softmax and top-k
+ * alone (vm_router_topk). */
+#define VM_SCORES_SOFTMAX 0u
+#define VM_SCORES_SIGMOID 1u
+#define VM_SELECT_MAX_EXPERTS 1024
+#define VM_SELECT_MAX_GROUPS 64
+#define VM_SELECT_MAX_TOP_K 64
+typedef struct VmSelectArgs {
+  const void* logits;            /* [rows, experts] logits_dtype */
+  const void* bias;              /* optional [experts] bias_dtype */
+  int32_t* inds;                 /* [rows, top_k] */
+  void* weights;                 /* [rows, top_k] weights_dtype */
+  uint64_t logits_stride;
+  double factor;
+  uint32_t rows, experts, groups, top_groups, group_top, top_k;
+  uint32_t scores, renormalize, logits_dtype, bias_dtype, weights_dtype;
+  uint32_t reserved;
+} VmSelectArgs;
+
 int vm_abi_version(void);
 /* 1 when a gfx950 device is usable by this library, else 0. */
 int vm_available(void);
@@ -491,11 +593,16 @@ int vm_rms_norm(const VmNormArgs* args, void* stream);
 int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* scales, uint32_t rows, uint32_t width,
                    uint32_t act_dtype, void* stream);
 
+int vm_block_norm(const VmBlockNormArgs* args, void* stream);
+
 uint64_t vm_grouped_matmul_workspace(uint32_t rows, uint32_t experts);
 int vm_grouped_matmul(const VmProductArgs* args, void* stream);
 
 uint64_t vm_add_adapters_workspace(uint32_t rows, uint32_t rank, uint32_t adapters);
 int vm_add_adapters(const VmAdapterArgs* args, void* stream);
+
+int vm_linear(const VmLinearArgs* args, void* stream);
+int vm_select_experts(const VmSelectArgs* args, void* stream);
 
 /* out[t, h] = sum_j expert_outputs[t, j, h] * scores[t, j] in fp32, written in
  * act_dtype; the normal form of weighted_combine (metal_runtime.py:145-191). */
@@ -540,7 +647,7 @@ int vm_decode_pipeline(int mode);
  * stream; vm_timing_read returns the summed milliseconds and launch count of
  * the kernel family `name` ("router", "gateup", "down", "experts",
  * "grouped_gateup", "grouped_down", "sort", "combine", "norm", "products",
- * "adapters"). */
+ * "adapters", "route", "linear"). */
 int vm_timing_enable(int enabled);
 int vm_timing_read(const char* name, double* total_ms, uint64_t* launches);
 int vm_timing_reset(void);

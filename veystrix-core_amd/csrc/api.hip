@@ -1617,6 +1617,90 @@ int vm_mx_quantize(const void* x, uint64_t x_stride, uint8_t* values, uint8_t* s
   return run_norm(p, stream);
 }
 
+int vm_block_norm(const VmBlockNormArgs* a, void* stream) {
+  if (a == nullptr) return fail(VM_EINVAL, "null arguments");
+  for (const uint32_t dtype : {a->act_dtype, a->residual_dtype, a->post_dtype, a->gate_dtype, a->weight_dtype})
+    if (dtype > VM_F32) return fail(VM_EINVAL, "dtypes must be bf16 or f32");
+  if (a->gate_kind > VM_GATE_VALUE) return fail(VM_EINVAL, "unknown gate_kind");
+  if (a->width == 0 || a->width > VM_NORM_MAX_WIDTH)
+    return fail(VM_EUNSUPPORTED, "width must be 1..%d", VM_NORM_MAX_WIDTH);
+  if (a->rows > kMaxBlocks) return fail(VM_EUNSUPPORTED, "at most %llu rows per call", (unsigned long long)kMaxBlocks);
+  if (a->rows == 0) return VM_OK;
+  if (a->x == nullptr || a->residual == nullptr) return fail(VM_EINVAL, "x and residual are required");
+  if ((a->gate != nullptr) != (a->gate_kind != VM_GATE_NONE)) return fail(VM_EINVAL, "gate and gate_kind go together");
+  const bool mx = a->values != nullptr || a->scales != nullptr;
+  if (a->weight != nullptr && mx == (a->out != nullptr))
+    return fail(VM_EINVAL, "either out or MX values and scales are required");
+  if (a->weight == nullptr && (mx || a->out != nullptr || a->sum_out == nullptr))
+    return fail(VM_EINVAL, "without a weight sum_out is the one output");
+  if (mx) {
+    const int rc = check_mx_rows(a->values, a->scales, a->rows, a->width);
+    if (rc != VM_OK) return rc;
+  }
+  const uint64_t w = a->width;
+  if (a->rows > 1 && ((a->out != nullptr && a->out_stride < w) || (a->sum_out != nullptr && a->sum_stride < w)))
+    return fail(VM_EINVAL, "the row strides of outputs must be at least the width");
+  const auto size = [](uint32_t dtype) { return dtype == VM_F32 ? uint64_t(4) : uint64_t(2); };
+  const auto span = [&](const void* at, uint64_t rows, uint64_t stride, uint64_t width, uint32_t dtype) {
+    return RowBytes{at, rows, stride * size(dtype), width * size(dtype)};
+  };
+  const RowBytes x = span(a->x, a->rows, a->x_stride, w, a->act_dtype);
+  const RowBytes r = span(a->residual, a->rows, a->residual_stride, w, a->residual_dtype);
+  const RowBytes out = span(a->out, a->rows, a->out_stride, w, a->act_dtype);
+  const RowBytes sum = span(a->sum_out, a->rows, a->sum_stride, w, a->residual_dtype);
+  const RowBytes values{a->values, a->rows, w, w}, scales{a->scales, a->rows, w / VM_MX_GROUP, w / VM_MX_GROUP};
+  RowBytes gate{nullptr, 1, 0, 0};
+  if (a->gate_kind == VM_GATE_ROW) gate = span(a->gate, a->rows, a->gate_stride, 1, a->gate_dtype);
+  if (a->gate_kind == VM_GATE_CHANNEL) gate = span(a->gate, 1, 0, w, a->gate_dtype);
+  if (a->gate_kind == VM_GATE_VALUE) gate = span(a->gate, a->rows, a->gate_stride, w, a->gate_dtype);
+  const auto in_place = [](const RowBytes& o, const RowBytes& in) { return same_rows(o, in) && o.width == in.width; };
+  for (const RowBytes& o : {out, sum}) {
+    for (const RowBytes& in : {x, r})
+      if (!in_place(o, in) && !rows_apart(o, in)) return fail(VM_EINVAL, "outputs overlap each other or an operand");
+    for (const RowBytes& in : {span(a->post_weight, 1, 0, w, a->post_dtype), gate, span(a->weight, 1, 0, w, a->weight_dtype)})
+      if (!rows_apart(o, in)) return fail(VM_EINVAL, "outputs overlap each other or an operand");
+  }
+  if (!rows_apart(out, sum)) return fail(VM_EINVAL, "outputs overlap each other or an operand");
+  for (const RowBytes& in : {x, r, span(a->post_weight, 1, 0, w, a->post_dtype), gate,
+                             span(a->weight, 1, 0, w, a->weight_dtype), sum})
+    if (!rows_apart(values, in) || !rows_apart(scales, in)) return fail(VM_EINVAL, "MX rows overlap an operand");
+  vm::BlockNormLaunch p{};
+  p.x = a->x;
+  p.residual = a->residual;
+  p.post_weight = a->post_weight;
+  p.gate = a->gate;
+  p.weight = a->weight;
+  p.out = a->out;
+  p.values = a->values;
+  p.scales = a->scales;
+  p.sum_out = a->sum_out;
+  p.x_stride = a->x_stride;
+  p.residual_stride = a->residual_stride;
+  p.gate_stride = a->gate_stride;
+  p.out_stride = a->out_stride;
+  p.sum_stride = a->sum_stride;
+  p.scale = a->scale;
+  p.residual_scale = a->residual_scale;
+  p.eps = a->eps;
+  p.rows = a->rows;
+  p.width = a->width;
+  p.gate_kind = a->gate_kind;
+  p.act_dtype = a->act_dtype;
+  p.residual_dtype = a->residual_dtype;
+  p.post_dtype = a->post_dtype;
+  p.gate_dtype = a->gate_dtype;
+  p.weight_dtype = a->weight_dtype;
+  p.sigmoid_gate = a->sigmoid_gate != 0;
+  p.one_centered = a->one_centered != 0;
+  p.vector = p.width % 8 == 0 && rows_aligned(x.at, x.stride, 16) && rows_aligned(r.at, r.stride, 16) &&
+             rows_aligned(out.at, out.stride, 16) && rows_aligned(sum.at, sum.stride, 16) &&
+             rows_aligned(a->post_weight, 0, 16) && rows_aligned(a->weight, 0, 16) &&
+             (a->gate_kind < VM_GATE_CHANNEL || rows_aligned(gate.at, gate.stride, 16));
+  const hipError_t e = vm::launch_block_norm(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "block norm launch");
+  return VM_OK;
+}
+
 // ----------------------------------------------------- sorted row calls ---
 
 // Workspace of a sort of `rows` ids into `groups` groups, laid out for tiles
@@ -1754,6 +1838,125 @@ int vm_grouped_matmul(const VmProductArgs* a, void* stream_ptr) {
   p.out_aligned = aligned16(a->out);
   const hipError_t e = vm::launch_products(p, tile, stream);
   if (e != hipSuccess) return hip_fail(e, "products launch");
+  return VM_OK;
+}
+
+// ------------------------------------------------------------- linear ---
+
+int vm_linear(const VmLinearArgs* a, void* stream) {
+  if (a == nullptr) return fail(VM_EINVAL, "null arguments");
+  if (a->format > VM_FORMAT_MX) return fail(VM_EINVAL, "format must be bf16 or MX");
+  if (a->activation > VM_ACTIVATION_SIGMOID) return fail(VM_EINVAL, "unknown activation");
+  if (a->bias_dtype > VM_F32 || a->residual_dtype > VM_F32 || a->out_dtype > VM_F32)
+    return fail(VM_EINVAL, "dtypes must be bf16 or f32");
+  const bool mx = a->format == VM_FORMAT_MX, swiglu = a->activation == VM_ACTIVATION_SWIGLU;
+  if (a->k == 0 || a->n == 0) return fail(VM_EINVAL, "k and n must be positive");
+  const uint32_t size = mx ? 1 : 2, unit = mx ? VM_MX_GROUP : 8;
+  if (a->k % unit) return fail(VM_EUNSUPPORTED, "k must be a multiple of %u", unit);
+  if (a->k > (1u << 24) || a->n > (1u << 24) || a->rows > (1u << 28))
+    return fail(VM_EUNSUPPORTED, "k and n of at most 2^24 and rows of at most 2^28");
+  if (a->rows == 0) return VM_OK;
+  if (a->x == nullptr || a->weight == nullptr || a->out == nullptr) return fail(VM_EINVAL, "x, weight and out are required");
+  if (mx && (a->x_scales == nullptr || a->weight_scales == nullptr))
+    return fail(VM_EINVAL, "MX operands need x_scales and weight_scales");
+  const uint64_t w_rows = uint64_t(a->n) * (swiglu ? 2 : 1), rows = a->rows;
+  // a stride that leads to no row aligns none
+  if (!rows_aligned(a->x, rows > 1 ? a->x_stride * size : 0, 16) ||
+      !rows_aligned(a->weight, w_rows > 1 ? a->weight_stride * size : 0, 16))
+    return fail(VM_EINVAL, "rows of x and weight must be 16-byte aligned");
+  if (rows > 1 && a->out_stride < a->n) return fail(VM_EINVAL, "the row stride of out must be at least n");
+  if (vm::linear_blocks(a->rows, a->n) > kMaxBlocks)
+    return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
+  const uint64_t out_size = a->out_dtype == VM_F32 ? 4 : 2, res_size = a->residual_dtype == VM_F32 ? 4 : 2;
+  const RowBytes out{a->out, rows, a->out_stride * out_size, a->n * out_size};
+  const RowBytes res{a->residual, rows, a->residual_stride * res_size, a->n * res_size};
+  const RowBytes ins[] = {{a->x, rows, a->x_stride * size, uint64_t(a->k) * size},
+                          {a->weight, w_rows, a->weight_stride * size, uint64_t(a->k) * size},
+                          {mx ? a->x_scales : nullptr, rows, a->x_scale_stride, a->k / VM_MX_GROUP},
+                          {mx ? a->weight_scales : nullptr, w_rows, a->weight_scale_stride, a->k / VM_MX_GROUP},
+                          {a->bias, 1, 0, w_rows * (a->bias_dtype == VM_F32 ? 4 : 2)}};
+  for (const RowBytes& in : ins)
+    if (!rows_apart(out, in)) return fail(VM_EINVAL, "out overlaps an operand");
+  if (!(same_rows(out, res) && out_size == res_size) && !rows_apart(out, res))
+    return fail(VM_EINVAL, "out overlaps residual other than row for row");
+  vm::LinearLaunch p{};
+  p.x = static_cast<const uint8_t*>(a->x);
+  p.x_scales = a->x_scales;
+  p.w = static_cast<const uint8_t*>(a->weight);
+  p.w_scales = a->weight_scales;
+  p.bias = a->bias;
+  p.residual = static_cast<const uint8_t*>(a->residual);
+  p.out = static_cast<uint8_t*>(a->out);
+  p.x_stride = a->x_stride * size;
+  p.x_scale_stride = a->x_scale_stride;
+  p.w_stride = a->weight_stride * size;
+  p.w_scale_stride = a->weight_scale_stride;
+  p.residual_stride = res.stride;
+  p.out_stride = out.stride;
+  p.rows = a->rows;
+  p.k_bytes = a->k * size;
+  p.n = a->n;
+  p.activation = a->activation;
+  p.bias_dtype = a->bias_dtype;
+  p.residual_dtype = a->residual_dtype;
+  p.out_dtype = a->out_dtype;
+  p.mx = mx;
+  p.whole_scales = mx && a->k / VM_MX_GROUP % 4 == 0 && rows_aligned(a->x_scales, rows > 1 ? a->x_scale_stride : 0, 4) &&
+                   rows_aligned(a->weight_scales, w_rows > 1 ? a->weight_scale_stride : 0, 4);
+  p.vector = a->n % 8 == 0 && rows_aligned(a->out, rows > 1 ? out.stride : 0, 16) &&
+             rows_aligned(a->residual, rows > 1 ? res.stride : 0, 16);
+  const hipError_t e = vm::launch_linear(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "linear launch");
+  return VM_OK;
+}
+
+// ------------------------------------------------------------- routing ---
+
+int vm_select_experts(const VmSelectArgs* a, void* stream) {
+  if (a == nullptr) return fail(VM_EINVAL, "null arguments");
+  if (a->logits_dtype > VM_F32 || a->bias_dtype > VM_F32 || a->weights_dtype > VM_F32)
+    return fail(VM_EINVAL, "dtypes must be bf16 or f32");
+  if (a->scores > VM_SCORES_SIGMOID) return fail(VM_EINVAL, "unknown scores");
+  if (a->experts == 0 || a->experts > VM_SELECT_MAX_EXPERTS)
+    return fail(VM_EUNSUPPORTED, "experts must be 1..%d", VM_SELECT_MAX_EXPERTS);
+  if (a->groups == 0 || a->groups > VM_SELECT_MAX_GROUPS || a->experts % a->groups)
+    return fail(VM_EUNSUPPORTED, "groups must be 1..%d and divide the experts", VM_SELECT_MAX_GROUPS);
+  if (a->top_groups == 0 || a->top_groups > a->groups) return fail(VM_EINVAL, "top_groups must be 1..groups");
+  if (a->group_top == 0 || a->group_top > 2) return fail(VM_EUNSUPPORTED, "group_top must be 1 or 2");
+  const uint32_t group_size = a->experts / a->groups;
+  if (a->top_k == 0 || a->top_k > VM_SELECT_MAX_TOP_K) return fail(VM_EUNSUPPORTED, "top_k must be 1..%d", VM_SELECT_MAX_TOP_K);
+  if (a->top_k > a->top_groups * group_size) return fail(VM_EINVAL, "top_k cannot exceed the experts of the kept groups");
+  if (a->rows > (1u << 25)) return fail(VM_EUNSUPPORTED, "at most 2^25 rows per call");
+  if (a->rows == 0) return VM_OK;
+  if (a->logits == nullptr || a->inds == nullptr || a->weights == nullptr)
+    return fail(VM_EINVAL, "logits, inds and weights are required");
+  const uint64_t size = a->logits_dtype == VM_F32 ? 4 : 2, slots = uint64_t(a->rows) * a->top_k;
+  const RowBytes logits{a->logits, a->rows, a->logits_stride * size, a->experts * size};
+  const RowBytes bias{a->bias, 1, 0, uint64_t(a->experts) * (a->bias_dtype == VM_F32 ? 4 : 2)};
+  const RowBytes inds{a->inds, 1, 0, slots * 4}, weights{a->weights, 1, 0, slots * (a->weights_dtype == VM_F32 ? 4 : 2)};
+  for (const RowBytes& out : {inds, weights})
+    if (!rows_apart(out, logits) || !rows_apart(out, bias)) return fail(VM_EINVAL, "outputs overlap an operand");
+  if (!rows_apart(inds, weights)) return fail(VM_EINVAL, "inds and weights overlap");
+  vm::RouteLaunch p{};
+  p.logits = a->logits;
+  p.bias = a->bias;
+  p.inds = a->inds;
+  p.weights = a->weights;
+  p.stride = a->logits_stride;
+  p.rows = a->rows;
+  p.groups = a->groups;
+  p.group_size = group_size;
+  p.top_groups = a->top_groups;
+  p.group_top = a->group_top;
+  p.top_k = a->top_k;
+  p.logits_dtype = a->logits_dtype;
+  p.bias_dtype = a->bias_dtype;
+  p.weights_dtype = a->weights_dtype;
+  p.sigmoid = a->scores == VM_SCORES_SIGMOID;
+  p.renormalize = a->renormalize != 0;
+  p.factor = a->factor;
+  const hipError_t e = vm::launch_route(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "route launch");
   return VM_OK;
 }
 

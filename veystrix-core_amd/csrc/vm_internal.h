@@ -440,6 +440,29 @@ struct NormLaunch {
 
 hipError_t launch_norm(const NormLaunch& p, hipStream_t stream);
 
+enum : uint32_t { kGateNone = 0, kGateRow = 1, kGateChannel = 2, kGateValue = 3 };
+
+// A block's two norms with its gate and residual (block_norm.hip).  Strides in elements.
+struct BlockNormLaunch {
+  const void* x;               // [rows, width] act_dtype
+  const void* residual;        // [rows, width] residual_dtype
+  const void* post_weight;     // optional [width]
+  const void* gate;            // by gate_kind
+  const void* weight;          // optional [width]: without, neither out nor values
+  void* out;                   // [rows, width] act_dtype, or
+  uint8_t* values;             // MX: [rows, width] e4m3 and
+  uint8_t* scales;             // [rows, width / 32] e8m0
+  void* sum_out;               // optional [rows, width] residual_dtype
+  uint64_t x_stride, residual_stride, gate_stride, out_stride, sum_stride;
+  double scale, residual_scale, eps;
+  uint32_t rows, width, gate_kind;
+  uint32_t act_dtype, residual_dtype, post_dtype, gate_dtype, weight_dtype;
+  bool sigmoid_gate, one_centered;
+  bool vector;                 // every row and weight 16-byte aligned, width a multiple of 8
+};
+
+hipError_t launch_block_norm(const BlockNormLaunch& p, hipStream_t stream);
+
 // -------------------------------------------------------------- row sort --
 // Rows sorted by group (row_sort.hip).
 struct RowTile {
@@ -528,5 +551,44 @@ bool adapter_sorted(uint32_t rows);
 // An upper bound of a call's blocks.
 uint64_t adapter_blocks(uint32_t rows, uint32_t adapters, uint32_t n, bool tiled);
 hipError_t launch_adapters(AdapterLaunch p, bool tiled, hipStream_t stream);
+
+// ---------------------------------------------------------------- linear --
+// Matrix products with an epilogue (linear.hip).  Byte strides.
+enum : uint32_t { kActNone = 0, kActSwiglu = 1, kActRelu = 2, kActSilu = 3, kActGelu = 4, kActGeluTanh = 5, kActSigmoid = 6 };
+struct LinearLaunch {
+  const uint8_t* x;            // [rows] rows of k_bytes
+  const uint8_t* x_scales;     // MX: k_bytes / 32 bytes per row
+  const uint8_t* w;            // [n (2 n with SwiGLU)] rows of k_bytes
+  const uint8_t* w_scales;
+  const void* bias;            // optional [n or 2 n]
+  const uint8_t* residual;     // optional [rows, n]
+  uint8_t* out;                // [rows, n]
+  uint64_t x_stride, x_scale_stride, w_stride, w_scale_stride, residual_stride, out_stride;
+  uint32_t rows, k_bytes, n, activation;
+  uint32_t bias_dtype, residual_dtype, out_dtype;
+  bool mx;
+  bool whole_scales;           // every row of scales starts at a multiple of four bytes and has whole words
+  bool vector;                 // rows of out and residual 16-byte aligned, n a multiple of 8
+};
+// An upper bound of a call's blocks.
+uint64_t linear_blocks(uint32_t rows, uint32_t n);
+hipError_t launch_linear(const LinearLaunch& p, hipStream_t stream);
+
+// --------------------------------------------------------------- routing --
+// From logits to experts (routing.hip).
+constexpr uint32_t kRouteMaxExperts = 1024, kRouteMaxGroups = 64, kRouteMaxTopK = 64;
+struct RouteLaunch {
+  const void* logits;          // [rows, groups * group_size], rows `stride` elements apart
+  const void* bias;            // optional [groups * group_size]
+  int32_t* inds;               // [rows, top_k], -1: none left
+  void* weights;               // [rows, top_k]
+  uint64_t stride;
+  uint32_t rows, groups, group_size, top_groups, group_top, top_k;
+  uint32_t lane_bits;          // 2^lane_bits lanes hold a group (set by launch_route)
+  uint32_t logits_dtype, bias_dtype, weights_dtype;
+  bool sigmoid, renormalize;
+  double factor;
+};
+hipError_t launch_route(RouteLaunch p, hipStream_t stream);
 
 }  // namespace vm

@@ -219,6 +219,62 @@ class VmAdapterArgs(ctypes.Structure):
     ]
 
 
+VM_GATE_NONE = 0
+VM_GATE_ROW = 1
+VM_GATE_CHANNEL = 2
+VM_GATE_VALUE = 3
+
+
+class VmBlockNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("post_weight", _vp), ("gate", _vp), ("weight", _vp), ("out", _vp),
+        ("sum_out", _vp), ("values", _vp), ("scales", _vp),
+        ("x_stride", _c_u64), ("residual_stride", _c_u64), ("gate_stride", _c_u64), ("out_stride", _c_u64),
+        ("sum_stride", _c_u64),
+        ("scale", ctypes.c_double), ("residual_scale", ctypes.c_double), ("eps", ctypes.c_double),
+        ("rows", _c_u32), ("width", _c_u32), ("act_dtype", _c_u32), ("residual_dtype", _c_u32), ("post_dtype", _c_u32),
+        ("gate_dtype", _c_u32), ("weight_dtype", _c_u32),
+        ("gate_kind", _c_u32), ("sigmoid_gate", _c_u32), ("one_centered", _c_u32),
+    ]
+
+
+VM_ACTIVATION_RELU = 2
+VM_ACTIVATION_SILU = 3
+VM_ACTIVATION_GELU = 4
+VM_ACTIVATION_GELU_TANH = 5
+VM_ACTIVATION_SIGMOID = 6
+
+
+class VmLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("x_scales", _vp), ("weight", _vp), ("weight_scales", _vp), ("bias", _vp), ("residual", _vp),
+        ("out", _vp),
+        ("x_stride", _c_u64), ("x_scale_stride", _c_u64), ("weight_stride", _c_u64), ("weight_scale_stride", _c_u64),
+        ("residual_stride", _c_u64), ("out_stride", _c_u64),
+        ("rows", _c_u32), ("k", _c_u32), ("n", _c_u32), ("format", _c_u32), ("activation", _c_u32),
+        ("bias_dtype", _c_u32), ("residual_dtype", _c_u32), ("out_dtype", _c_u32),
+    ]
+
+
+VM_SCORES_SOFTMAX = 0
+VM_SCORES_SIGMOID = 1
+VM_SELECT_MAX_EXPERTS = 1024
+VM_SELECT_MAX_GROUPS = 64
+VM_SELECT_MAX_TOP_K = 64
+
+
+class VmSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", _vp), ("bias", _vp), ("inds", _vp), ("weights", _vp),
+        ("logits_stride", _c_u64),
+        ("factor", ctypes.c_double),
+        ("rows", _c_u32), ("experts", _c_u32), ("groups", _c_u32), ("top_groups", _c_u32), ("group_top", _c_u32),
+        ("top_k", _c_u32),
+        ("scores", _c_u32), ("renormalize", _c_u32), ("logits_dtype", _c_u32), ("bias_dtype", _c_u32),
+        ("weights_dtype", _c_u32), ("reserved", _c_u32),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "vm_abi_version": (ctypes.c_int, []),
@@ -243,6 +299,9 @@ SIGNATURES = {
     "vm_grouped_matmul": (ctypes.c_int, [ctypes.POINTER(VmProductArgs), _vp]),
     "vm_add_adapters_workspace": (_c_u64, [_c_u32, _c_u32, _c_u32]),
     "vm_add_adapters": (ctypes.c_int, [ctypes.POINTER(VmAdapterArgs), _vp]),
+    "vm_block_norm": (ctypes.c_int, [ctypes.POINTER(VmBlockNormArgs), _vp]),
+    "vm_linear": (ctypes.c_int, [ctypes.POINTER(VmLinearArgs), _vp]),
+    "vm_select_experts": (ctypes.c_int, [ctypes.POINTER(VmSelectArgs), _vp]),
     "vm_pool_stage": (ctypes.c_int, [_vp, _c_u64, _c_u64, _c_u64, _vp, _c_u64, _c_u64, _c_u64,
                                      ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),
                                      _c_u32, _vp]),

@@ -86,6 +86,8 @@ def row_span(name: str, tensor, dtype, index):
         raise ValueError(f"{name} must have at least one dimension")
     if shape[-1] > 1 and strides[-1] != 1:
         raise ValueError(f"the rows of {name} must be contiguous")
+    if 0 in shape:
+        return tensor.data_ptr(), shape[-1]
     step, span = None, 1        # the leading dimensions as one: each stride the inner one's extent
     for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:

@@ -1,4 +1,5 @@
-"""Root-mean-square norm with the residual's addition in front of it, and rows in MX.
+"""Root-mean-square norm with the residual's addition in front of it, a block's two norms with its gate and residual, and
+rows in MX.
 
 MX rows (:class:`MxTensor`) hold e4m3 values with one power-of-two scale (e8m0) per group of 32 along the row: the
 least 2^e, e >= -127, that keeps the group's largest magnitude within e4m3's 448, so that no value saturates.  A group
@@ -111,6 +112,84 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     return y if residual is None else (y, residual_out)
 
 
+def _weight(name, w, width, index):
+    """(address, dtype code) of a contiguous [width] weight on GPU ``index``; (None, bf16's) of None."""
+    if w is None:
+        return None, _lib.VM_BF16
+    code = _act_dtype(name, w)
+    if w.shape != (width,) or not w.is_contiguous():
+        raise ValueError(f"{name} must be contiguous of shape ({width},)")
+    return row_span(name, w, w.dtype, index)[0], code
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor = None, *, post_weight: torch.Tensor = None,
+               gate: torch.Tensor = None, sigmoid_gate: bool = False, scale: float = 1.0, residual_scale: float = 1.0,
+               eps: float = 1e-6, one_centered: bool = True, quantize: bool = False, out: torch.Tensor = None,
+               residual_out: torch.Tensor = None):
+    """From a block's output x to the next block's input: ``(y, h)`` with
+
+        n = x / sqrt(mean(x^2) + eps) * post_weight          (n = x without a post_weight)
+        h = residual_scale * residual + scale * gate * n
+        y = h / sqrt(mean(h^2) + eps) * weight               (only h is returned without a weight)
+
+    over the last dimension; weights count from zero (1 + weight) unless ``one_centered``.  x [.., width] and residual of
+    its shape, each bfloat16 or float32 with equally spaced rows, width up to 16384; weights [width] in either type.
+    gate: [.., 1], one for each row, [width], one for each channel, or x's shape, in either type, as it is or with
+    ``sigmoid_gate`` through a sigmoid.  h comes in residual's type, y in x's, or as an :class:`MxTensor` with
+    ``quantize`` (width a multiple of 32); the second norm reads the unrounded h.  ``out`` and ``residual_out`` may each
+    be x or residual where the types match, and overlap nothing otherwise.
+    """
+    act, res_act = _act_dtype("x", x), _act_dtype("residual", residual)
+    shape, index = x.shape, x.get_device()
+    x_at, x_stride = row_span("x", x, x.dtype, index)
+    r_at, r_stride = row_span("residual", residual, residual.dtype, index)
+    if residual.shape != shape:
+        raise ValueError("residual must have x's shape")
+    width, count = shape[-1], x.numel()
+    if count:
+        require_32_bits(count // width, width)
+    post_at, post_code = _weight("post_weight", post_weight, width, index)
+    w_at, w_code = _weight("weight", weight, width, index)
+    gate_at, gate_stride, gate_code, kind = None, 0, _lib.VM_BF16, _lib.VM_GATE_NONE
+    if gate is not None:
+        gate_code = _act_dtype("gate", gate)
+        gate_at, gate_stride = row_span("gate", gate, gate.dtype, index)
+        if gate.shape == shape and len(shape) > 1:
+            kind = _lib.VM_GATE_VALUE
+        elif gate.shape == (width,):
+            kind = _lib.VM_GATE_CHANNEL
+        elif gate.shape == (*shape[:-1], 1):
+            kind = _lib.VM_GATE_ROW
+        else:
+            raise ValueError(f"gate {tuple(gate.shape)} is neither one per row, per channel nor per value of x {tuple(shape)}")
+    if weight is None and (quantize or out is not None):
+        raise ValueError("quantize and out need a weight")
+    if quantize and out is not None:
+        raise ValueError("out is not taken with quantize")
+    if quantize and width % MX_GROUP:
+        raise ValueError(f"quantize needs a width that is a multiple of {MX_GROUP}")
+    h = torch.empty_like(residual) if residual_out is None else residual_out
+    h_at, h_stride = row_span("residual_out", h, residual.dtype, index)
+    if h.shape != shape:
+        raise ValueError("residual_out must have x's shape")
+    y = y_at = values_at = scales_at = None
+    y_stride = 0
+    if quantize:
+        y = mx_empty(shape, x.device)
+        values_at, scales_at = y[0].data_ptr(), y[1].data_ptr()
+    elif weight is not None:
+        y = torch.empty_like(x) if out is None else out
+        y_at, y_stride = row_span("out", y, x.dtype, index)
+        if y.shape != shape:
+            raise ValueError("out must have x's shape")
+    if count:
+        a = _lib.VmBlockNormArgs(x_at, r_at, post_at, gate_at, w_at, y_at, h_at, values_at, scales_at, x_stride, r_stride,
+                                 gate_stride, y_stride, h_stride, scale, residual_scale, eps, count // width, width, act,
+                                 res_act, post_code, gate_code, w_code, kind, sigmoid_gate, one_centered)
+        _lib.check(device_call(index, _lib.lib().vm_block_norm, ctypes.byref(a)))
+    return h if weight is None else (y, h)
+
+
 def mx_quantize(x: torch.Tensor) -> MxTensor:
     """x [.., width] bfloat16 or float32 (equally spaced rows, width a multiple of 32 up to 16384) as MX rows."""
     act = _act_dtype("x", x)
@@ -127,4 +206,4 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     return y
 
 
-__all__ = ["MX_GROUP", "MxTensor", "mx_empty", "mx_quantize", "rms_norm"]
+__all__ = ["MX_GROUP", "MxTensor", "block_norm", "mx_empty", "mx_quantize", "rms_norm"]
