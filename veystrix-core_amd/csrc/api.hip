@@ -1903,8 +1903,6 @@ int vm_linear(const VmLinearArgs* a, void* stream) {
   p.mx = mx;
   p.whole_scales = mx && a->k / VM_MX_GROUP % 4 == 0 && rows_aligned(a->x_scales, rows > 1 ? a->x_scale_stride : 0, 4) &&
                    rows_aligned(a->weight_scales, w_rows > 1 ? a->weight_scale_stride : 0, 4);
-  p.vector = a->n % 8 == 0 && rows_aligned(a->out, rows > 1 ? out.stride : 0, 16) &&
-             rows_aligned(a->residual, rows > 1 ? res.stride : 0, 16);
   const hipError_t e = vm::launch_linear(p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "linear launch");
   return VM_OK;

@@ -568,7 +568,6 @@ struct LinearLaunch {
   uint32_t bias_dtype, residual_dtype, out_dtype;
   bool mx;
   bool whole_scales;           // every row of scales starts at a multiple of four bytes and has whole words
-  bool vector;                 // rows of out and residual 16-byte aligned, n a multiple of 8
 };
 // An upper bound of a call's blocks.
 uint64_t linear_blocks(uint32_t rows, uint32_t n);
