@@ -1692,10 +1692,6 @@ int vm_block_norm(const VmBlockNormArgs* a, void* stream) {
   p.weight_dtype = a->weight_dtype;
   p.sigmoid_gate = a->sigmoid_gate != 0;
   p.one_centered = a->one_centered != 0;
-  p.vector = p.width % 8 == 0 && rows_aligned(x.at, x.stride, 16) && rows_aligned(r.at, r.stride, 16) &&
-             rows_aligned(out.at, out.stride, 16) && rows_aligned(sum.at, sum.stride, 16) &&
-             rows_aligned(a->post_weight, 0, 16) && rows_aligned(a->weight, 0, 16) &&
-             (a->gate_kind < VM_GATE_CHANNEL || rows_aligned(gate.at, gate.stride, 16));
   const hipError_t e = vm::launch_block_norm(p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "block norm launch");
   return VM_OK;

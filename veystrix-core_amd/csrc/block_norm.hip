@@ -8,9 +8,9 @@
 // second norm reads h as it was computed, before it is rounded to the residual's type.
 //
 // A row is read once: x and the residual stay in registers from the first sum of squares over the second to the last
-// store, eight consecutive values per thread and step (vm_norm.h).  Squares are summed in 64 bits, which no value
+// store, eight consecutive values per thread and step, at any alignment (vm_any.h).  Squares are summed in 64 bits, which no value
 // overflows and which costs two operations a value.  Rows to MX are computed in 64 bits throughout, so that e4m3's is
-// their one rounding: h is kept as a float and its rest, in the registers that x and the residual leave.
+// their one rounding.
 // Bound by HBM (two rows in, two out), or with few rows by one row's latency, which two sums over the row make up.
 
 #include <hip/hip_ext.h>
@@ -18,6 +18,7 @@
 
 #include <type_traits>
 
+#include "vm_any.h"
 #include "vm_internal.h"
 #include "vm_mx.h"
 #include "vm_norm.h"
@@ -27,19 +28,6 @@ namespace vm {
 namespace {
 
 constexpr int kBlockNormThreads = 256;
-
-template <int LIE>
-__device__ __forceinline__ void load8_any(const void* row, uint32_t dtype, uint32_t at, uint32_t step, uint32_t width,
-                                          float v[8]) {
-  if (dtype == 0) load8<ActBF16, LIE>(row, at, step, width, v);
-  else load8<ActF32, LIE>(row, at, step, width, v);
-}
-template <int LIE>
-__device__ __forceinline__ void store8_any(void* row, uint32_t dtype, uint32_t at, uint32_t step, uint32_t width,
-                                           const float v[8]) {
-  if (dtype == 0) store8<ActBF16, LIE>(row, at, step, width, v);
-  else store8<ActF32, LIE>(row, at, step, width, v);
-}
 
 __device__ __forceinline__ const void* row_at(const void* base, uint64_t row, uint64_t stride, uint32_t dtype) {
   return static_cast<const uint8_t*>(base) + row * stride * (dtype == 0 ? 2u : 4u);
@@ -66,33 +54,33 @@ __device__ __forceinline__ Real gate_sigmoid(float g) {
 }
 
 // TPR threads per row (64 or 256), up to NV steps of eight values per thread.
-template <int TPR, int NV, int LIE, bool MXOUT>
+template <int TPR, int NV, bool MXOUT>
 __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunch p) {
-  static_assert(!MXOUT || LIE != kSpread, "MX rows need a group's values side by side");
   using Real = std::conditional_t<MXOUT, double, float>;
   __shared__ double s_part[2][TPR / 64];
   const uint32_t t = threadIdx.x % TPR;
   const uint32_t row = blockIdx.x * (kBlockNormThreads / TPR) + threadIdx.x / TPR;
   if (row >= p.rows) return;  // TPR 64: whole waves; TPR 256: never
-  constexpr uint32_t kStep = LIE == kSpread ? TPR : 1;
-  const auto at = [&](int i) { return LIE == kSpread ? i * TPR * 8u + t : (i * TPR + t) * 8u; };
-  float h[NV][8], r[NV][8];   // x and the residual, then the sum and, to MX, its rest
-  const void* x = row_at(p.x, row, p.x_stride, p.act_dtype);
-  const void* res = row_at(p.residual, row, p.residual_stride, p.residual_dtype);
-  if (p.act_dtype == 0) {
+  const auto at = [&](int i) { return (i * TPR + t) * 8u; };
+  Real h[NV][8];              // x, then the sum
+  float r[NV][8];
+  // the loads of a row are together on their way: one branch per operand, not per step
+  const auto load_row = [&](const void* from, uint32_t dtype, auto&& keep) {
+    const auto steps = [&](uint32_t type) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8<ActBF16, LIE>(x, at(i), kStep, p.width, h[i]);
-  } else {
+      for (int i = 0; i < NV; ++i) {
+        float v[8];
+        load_run<8>(from, type, at(i), p.width, v);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8<ActF32, LIE>(x, at(i), kStep, p.width, h[i]);
-  }
-  if (p.residual_dtype == 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) load8<ActBF16, LIE>(res, at(i), kStep, p.width, r[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) load8<ActF32, LIE>(res, at(i), kStep, p.width, r[i]);
-  }
+        for (int j = 0; j < 8; ++j) keep(i, j, v[j]);
+      }
+    };
+    if (dtype == 0) steps(0u);
+    else steps(1u);
+  };
+  load_row(row_at(p.x, row, p.x_stride, p.act_dtype), p.act_dtype, [&](int i, int j, float v) { h[i][j] = v; });
+  load_row(row_at(p.residual, row, p.residual_stride, p.residual_dtype), p.residual_dtype,
+           [&](int i, int j, float v) { r[i][j] = v; });
   const double width = p.width;
   Real post = 1;
   if (p.post_weight != nullptr) {
@@ -104,6 +92,7 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
     post = static_cast<Real>(1.0 / sqrt(row_total<TPR>(ss, s_part[0]) / width + p.eps));
   }
   const Real scale = static_cast<Real>(p.scale), residual_scale = static_cast<Real>(p.residual_scale);
+  const Real one = p.one_centered ? 0 : 1;
   const void* gate = p.gate;
   Real row_gate = 1;
   if (p.gate_kind == kGateRow) {
@@ -112,61 +101,62 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
   } else if (p.gate_kind == kGateValue) {
     gate = row_at(p.gate, row, p.gate_stride, p.gate_dtype);
   }
+  void* sum_out = const_cast<void*>(row_at(p.sum_out, row, p.sum_stride, p.residual_dtype));
   double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    Real b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = h[i][j];
     if (p.post_weight != nullptr) {
       float w[8];
-      load8_any<LIE>(p.post_weight, p.post_dtype, at(i), kStep, p.width, w);
+      load_run<8>(p.post_weight, p.post_dtype, at(i), p.width, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = b[j] * post * (p.one_centered ? static_cast<Real>(w[j]) : 1 + static_cast<Real>(w[j]));
+      for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * post * (one + static_cast<Real>(w[j]));
     }
     if (p.gate_kind == kGateChannel || p.gate_kind == kGateValue) {
       float g[8];
-      load8_any<LIE>(gate, p.gate_dtype, at(i), kStep, p.width, g);
+      load_run<8>(gate, p.gate_dtype, at(i), p.width, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] *= p.sigmoid_gate ? gate_sigmoid<Real>(g[j]) : static_cast<Real>(g[j]);
+      for (int j = 0; j < 8; ++j) h[i][j] *= p.sigmoid_gate ? gate_sigmoid<Real>(g[j]) : static_cast<Real>(g[j]);
     }
+    float sum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const Real sum = residual_scale * static_cast<Real>(r[i][j]) + scale * (row_gate * b[j]);
-      // values behind the row's end are zeros, but a gate there may have been anything times them
-      const bool in = at(i) + j * kStep < p.width;
-      h[i][j] = in ? static_cast<float>(sum) : 0.0f;
-      if constexpr (MXOUT) r[i][j] = in ? static_cast<float>(sum - static_cast<Real>(h[i][j])) : 0.0f;
-      const double wide = in ? static_cast<double>(sum) : 0.0;
-      ss = fma(wide, wide, ss);
+      h[i][j] = residual_scale * static_cast<Real>(r[i][j]) + scale * (row_gate * h[i][j]);
+      if (at(i) >= p.width) h[i][j] = 0;   // zeros there, but times a scale that is no number
+      sum[j] = static_cast<float>(h[i][j]);
     }
-  }
-  if (p.sum_out != nullptr) {
-    void* s = const_cast<void*>(row_at(p.sum_out, row, p.sum_stride, p.residual_dtype));
+    if (p.sum_out != nullptr) store_run<8>(sum_out, p.residual_dtype, at(i), p.width, sum);
+    if (at(i) < p.width && at(i) + 8 > p.width) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store8_any<LIE>(s, p.residual_dtype, at(i), kStep, p.width, h[i]);
+      for (int j = 0; j < 8; ++j)
+        if (at(i) + j >= p.width) h[i][j] = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fma(static_cast<double>(h[i][j]), static_cast<double>(h[i][j]), ss);
   }
   if (p.weight == nullptr) return;
   const Real pre = static_cast<Real>(1.0 / sqrt(row_total<TPR>(ss, s_part[1]) / width + p.eps));
+  void* out = const_cast<void*>(row_at(p.out, row, p.out_stride, p.act_dtype));
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float w[8], y[8];
-    load8_any<LIE>(p.weight, p.weight_dtype, at(i), kStep, p.width, w);
+    load_run<8>(p.weight, p.weight_dtype, at(i), p.width, w);
+    uint32_t border = ~0u;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const Real gain = p.one_centered ? static_cast<Real>(w[j]) : 1 + static_cast<Real>(w[j]);
-      if constexpr (MXOUT) {
-        const double v = (static_cast<double>(h[i][j]) + static_cast<double>(r[i][j])) * pre * gain;
-        y[j] = static_cast<float>(v);
-        const double rest = v - static_cast<double>(y[j]);
-        y[j] = off_border(y[j], rest > 0.0 ? 1.0f : rest < 0.0 ? -1.0f : 0.0f);
-      } else {
-        y[j] = h[i][j] * pre * gain;
-      }
+      h[i][j] = h[i][j] * pre * (one + static_cast<Real>(w[j]));
+      y[j] = static_cast<float>(h[i][j]);
+      border = min(border, __float_as_uint(y[j]) & kBorderBits);
     }
     if constexpr (!MXOUT) {
-      store8_any<LIE>(const_cast<void*>(row_at(p.out, row, p.out_stride, p.act_dtype)), p.act_dtype, at(i), kStep, p.width, y);
+      store_run<8>(out, p.act_dtype, at(i), p.width, y);
     } else {
+      if (border == 0) {  // seldom: one of them may lie on a border
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const double rest = h[i][j] - static_cast<double>(y[j]);
+          y[j] = off_border(y[j], rest > 0.0 ? 1.0f : rest < 0.0 ? -1.0f : 0.0f);
+        }
+      }
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(y[j]));
@@ -187,9 +177,7 @@ template <int TPR, int NV>
 hipError_t block_norm_go(const BlockNormLaunch& p, hipStream_t stream) {
   const uint32_t per = kBlockNormThreads / TPR;
   const dim3 grid((p.rows + per - 1) / per);
-  auto kernel = p.values != nullptr
-                    ? (p.vector ? &k_block_norm<TPR, NV, kUnits, true> : &k_block_norm<TPR, NV, kOnes, true>)
-                    : (p.vector ? &k_block_norm<TPR, NV, kUnits, false> : &k_block_norm<TPR, NV, kSpread, false>);
+  auto kernel = p.values != nullptr ? &k_block_norm<TPR, NV, true> : &k_block_norm<TPR, NV, false>;
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("norm", &start, &stop))
     hipExtLaunchKernelGGL(kernel, grid, dim3(kBlockNormThreads), 0, stream, start, stop, 0, p);

@@ -11,6 +11,7 @@
 
 #include <type_traits>
 
+#include "vm_any.h"
 #include "vm_dma.h"
 #include "vm_internal.h"
 #include "vm_mx.h"
@@ -63,60 +64,6 @@ struct SigmoidForm {
   }
 };
 
-// Words at any even address: one load or store of the vector memory unit, which takes any alignment.
-typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t words2 __attribute__((ext_vector_type(2), aligned(2)));
-template <uint32_t N>
-using Words = std::conditional_t<N == 4, words4, words2>;
-
-// N (4 or 8) neighbouring values of one row from column `col`, those at `n` and behind it left out.
-template <uint32_t N>
-__device__ __forceinline__ void load_outputs(const void* row, uint32_t dtype, uint32_t col, uint32_t n, float v[N]) {
-  if (col + N > n) {
-#pragma unroll
-    for (uint32_t j = 0; j < N; ++j) v[j] = load_any(row, min(col + j, n - 1), dtype);
-  } else if (dtype == 0) {
-    const Words<N / 2> a = *(const __attribute__((address_space(1))) Words<N / 2>*)(static_cast<const uint16_t*>(row) + col);
-#pragma unroll
-    for (uint32_t j = 0; j < N / 2; ++j) {
-      v[2 * j] = __uint_as_float(a[j] << 16);
-      v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < N; j += 4) {
-      const Words<4> a = *(const __attribute__((address_space(1))) Words<4>*)(static_cast<const float*>(row) + col + j);
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) v[j + i] = __uint_as_float(a[i]);
-    }
-  }
-}
-
-template <uint32_t N>
-__device__ __forceinline__ void store_outputs(void* row, uint32_t dtype, uint32_t col, uint32_t n, const float v[N]) {
-  if (col + N > n) {
-#pragma unroll
-    for (uint32_t j = 0; j < N; ++j) {
-      if (col + j >= n) continue;
-      if (dtype == 0) ActBF16::store(row, col + j, v[j]);
-      else ActF32::store(row, col + j, v[j]);
-    }
-  } else if (dtype == 0) {
-    Words<N / 2> a;
-#pragma unroll
-    for (uint32_t j = 0; j < N / 2; ++j) a[j] = f32_to_bf16(v[2 * j]) | (f32_to_bf16(v[2 * j + 1]) << 16);
-    *(__attribute__((address_space(1))) Words<N / 2>*)(static_cast<uint16_t*>(row) + col) = a;
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < N; j += 4) {
-      Words<4> a;
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) a[i] = __float_as_uint(v[j + i]);
-      *(__attribute__((address_space(1))) Words<4>*)(static_cast<float*>(row) + col + j) = a;
-    }
-  }
-}
-
 __device__ __forceinline__ void add_bias(const LinearLaunch& p, uint32_t at, uint32_t left, float v[8]) {
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j) v[j] += load_any(p.bias, at + min(j, left - 1), p.bias_dtype);
@@ -153,11 +100,11 @@ __device__ __forceinline__ void finish8(const LinearLaunch& p, uint32_t row, uin
   }
   if (p.residual != nullptr) {
     float r[8];
-    load_outputs<8>(p.residual + row * p.residual_stride, p.residual_dtype, col, p.n, r);
+    load_run<8>(p.residual + row * p.residual_stride, p.residual_dtype, col, p.n, r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += r[j];
   }
-  store_outputs<8>(p.out + row * p.out_stride, p.out_dtype, col, p.n, v);
+  store_run<8>(p.out + row * p.out_stride, p.out_dtype, col, p.n, v);
 }
 
 // ------------------------------------------------------------- few rows ---
@@ -648,7 +595,7 @@ __global__ __launch_bounds__(512, 2) void k_large(LinearLaunch p) {
     if (p.residual != nullptr) {
 #pragma unroll
       for (int i = 0; i < RF; ++i)
-        load_outputs<kOut>(p.residual + min(row + i * 16u, p.rows - 1) * p.residual_stride, p.residual_dtype, col, p.n,
+        load_run<kOut>(p.residual + min(row + i * 16u, p.rows - 1) * p.residual_stride, p.residual_dtype, col, p.n,
                            r[i]);
     }
 #pragma unroll
@@ -665,7 +612,7 @@ __global__ __launch_bounds__(512, 2) void k_large(LinearLaunch p) {
         if (p.residual != nullptr) y[j] += r[i][j];
       }
       if (row + i * 16u < p.rows)
-        store_outputs<kOut>(p.out + (row + i * 16u) * p.out_stride, p.out_dtype, col, p.n, y);
+        store_run<kOut>(p.out + (row + i * 16u) * p.out_stride, p.out_dtype, col, p.n, y);
     }
   }
 }

@@ -458,7 +458,6 @@ struct BlockNormLaunch {
   uint32_t rows, width, gate_kind;
   uint32_t act_dtype, residual_dtype, post_dtype, gate_dtype, weight_dtype;
   bool sigmoid_gate, one_centered;
-  bool vector;                 // every row and weight 16-byte aligned, width a multiple of 8
 };
 
 hipError_t launch_block_norm(const BlockNormLaunch& p, hipStream_t stream);
@@ -586,6 +585,7 @@ struct RouteLaunch {
   uint32_t lane_bits;          // 2^lane_bits lanes hold a group (set by launch_route)
   uint32_t logits_dtype, bias_dtype, weights_dtype;
   bool sigmoid, renormalize;
+  bool wide_logits, wide_bias; // loads of whole aligned units (set by launch_route)
   double factor;
 };
 hipError_t launch_route(RouteLaunch p, hipStream_t stream);
