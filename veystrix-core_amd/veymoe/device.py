@@ -100,6 +100,19 @@ def row_span(name: str, tensor, dtype, index):
     return tensor.data_ptr(), shape[-1] if step is None else step
 
 
+def vector_of(name: str, tensor, size: int, index):
+    """(address, dtype code) of a contiguous bfloat16 or float32 vector of ``size`` values on GPU ``index``."""
+    try:
+        code = ACT_DTYPES[tensor.dtype]
+        if tensor.get_device() != index:
+            raise TypeError(f"{name} must live on GPU {index} (got {tensor.device})")
+    except (AttributeError, KeyError):
+        raise TypeError(f"{name} must be a bfloat16 or float32 tensor") from None
+    if tensor.shape != (size,) or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous of shape ({size},)")
+    return tensor.data_ptr(), code
+
+
 def require_32_bits(*sizes):
     """Sizes that the C ABI takes in 32 bits."""
     if max(sizes) >> 32:

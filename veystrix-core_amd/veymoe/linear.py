@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import ACT_DTYPES, device_call, require_32_bits, row_span
+from .device import ACT_DTYPES, device_call, require_32_bits, row_span, vector_of
 from .norm import MxTensor, require_mx
 
 ACTIVATIONS = {None: _lib.VM_ACTIVATION_NONE, "swiglu": _lib.VM_ACTIVATION_SWIGLU, "relu": _lib.VM_ACTIVATION_RELU,
@@ -61,25 +61,25 @@ def linear(x, weight, bias: torch.Tensor = None, *, activation: str = None, resi
     if dtype not in ACT_DTYPES:
         raise TypeError(f"dtype must be bfloat16 or float32, got {dtype}")
     shape = (*xv.shape[:-1], n)
-    rows = xv.numel() // max(k, 1)
+    rows = xv.numel() // k
     require_32_bits(rows, k, wv.shape[0])
     bias_at = res_at = None
-    bias_code = res_code = _lib.VM_BF16
-    res_stride = 0
+    bias_code = res_code = res_stride = 0
     if bias is not None:
-        bias_code = _code("bias", bias)
-        if bias.shape != (wv.shape[0],) or not bias.is_contiguous():
-            raise ValueError(f"bias must be contiguous of shape ({wv.shape[0]},)")
-        bias_at, _ = row_span("bias", bias, bias.dtype, index)
+        bias_at, bias_code = vector_of("bias", bias, wv.shape[0], index)
     if residual is not None:
         res_code = _code("residual", residual)
         if residual.shape != shape:
             raise ValueError(f"residual must have shape {shape}")
         res_at, res_stride = row_span("residual", residual, residual.dtype, index)
-    y = torch.empty(shape, dtype=dtype, device=xv.device) if out is None else out
-    y_at, y_stride = row_span("out", y, dtype, index)
-    if y.shape != shape:
-        raise ValueError(f"out must have shape {shape}")
+    if out is None:
+        y = xv.new_empty(shape) if xv.dtype == dtype else torch.empty(shape, dtype=dtype, device=xv.device)
+        y_at, y_stride = y.data_ptr(), n
+    else:
+        y = out
+        y_at, y_stride = row_span("out", y, dtype, index)
+        if y.shape != shape:
+            raise ValueError(f"out must have shape {shape}")
     if rows == 0 or n == 0:
         return y
     xs_at = ws_at = None

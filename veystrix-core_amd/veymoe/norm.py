@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .device import ACT_DTYPES, device_call, require_32_bits, row_span
+from .device import ACT_DTYPES, device_call, require_32_bits, row_span, vector_of
 
 MX_GROUP = _lib.VM_MX_GROUP
 _SCALE_DTYPES = (torch.float8_e8m0fnu, torch.uint8)
@@ -112,16 +112,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-6, residu
     return y if residual is None else (y, residual_out)
 
 
-def _weight(name, w, width, index):
-    """(address, dtype code) of a contiguous [width] weight on GPU ``index``; (None, bf16's) of None."""
-    if w is None:
-        return None, _lib.VM_BF16
-    code = _act_dtype(name, w)
-    if w.shape != (width,) or not w.is_contiguous():
-        raise ValueError(f"{name} must be contiguous of shape ({width},)")
-    return row_span(name, w, w.dtype, index)[0], code
-
-
 def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor = None, *, post_weight: torch.Tensor = None,
                gate: torch.Tensor = None, sigmoid_gate: bool = False, scale: float = 1.0, residual_scale: float = 1.0,
                eps: float = 1e-6, one_centered: bool = True, quantize: bool = False, out: torch.Tensor = None,
@@ -146,11 +136,17 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor = N
     if residual.shape != shape:
         raise ValueError("residual must have x's shape")
     width, count = shape[-1], x.numel()
-    if count:
-        require_32_bits(count // width, width)
-    post_at, post_code = _weight("post_weight", post_weight, width, index)
-    w_at, w_code = _weight("weight", weight, width, index)
-    gate_at, gate_stride, gate_code, kind = None, 0, _lib.VM_BF16, _lib.VM_GATE_NONE
+    rows = count // width if count else 0
+    require_32_bits(rows, width)
+    post_at = w_at = gate_at = None
+    post_code = w_code = gate_code = gate_stride = 0
+    kind = _lib.VM_GATE_NONE
+    if post_weight is not None:
+        post_at, post_code = vector_of("post_weight", post_weight, width, index)
+    if weight is not None:
+        w_at, w_code = vector_of("weight", weight, width, index)
+    elif quantize or out is not None:
+        raise ValueError("quantize and out need a weight")
     if gate is not None:
         gate_code = _act_dtype("gate", gate)
         gate_at, gate_stride = row_span("gate", gate, gate.dtype, index)
@@ -162,30 +158,36 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor = N
             kind = _lib.VM_GATE_ROW
         else:
             raise ValueError(f"gate {tuple(gate.shape)} is neither one per row, per channel nor per value of x {tuple(shape)}")
-    if weight is None and (quantize or out is not None):
-        raise ValueError("quantize and out need a weight")
-    if quantize and out is not None:
-        raise ValueError("out is not taken with quantize")
-    if quantize and width % MX_GROUP:
-        raise ValueError(f"quantize needs a width that is a multiple of {MX_GROUP}")
-    h = torch.empty_like(residual) if residual_out is None else residual_out
-    h_at, h_stride = row_span("residual_out", h, residual.dtype, index)
-    if h.shape != shape:
-        raise ValueError("residual_out must have x's shape")
+    if quantize:
+        if out is not None:
+            raise ValueError("out is not taken with quantize")
+        if width % MX_GROUP:
+            raise ValueError(f"quantize needs a width that is a multiple of {MX_GROUP}")
+    if residual_out is None:
+        h = torch.empty_like(residual)
+        h_at, h_stride = (h.data_ptr(), width) if h.is_contiguous() else row_span("residual", h, h.dtype, index)
+    else:
+        h = residual_out
+        h_at, h_stride = row_span("residual_out", h, residual.dtype, index)
+        if h.shape != shape:
+            raise ValueError("residual_out must have x's shape")
     y = y_at = values_at = scales_at = None
     y_stride = 0
     if quantize:
         y = mx_empty(shape, x.device)
         values_at, scales_at = y[0].data_ptr(), y[1].data_ptr()
-    elif weight is not None:
-        y = torch.empty_like(x) if out is None else out
+    elif out is not None:
+        y = out
         y_at, y_stride = row_span("out", y, x.dtype, index)
         if y.shape != shape:
             raise ValueError("out must have x's shape")
-    if count:
+    elif weight is not None:
+        y = torch.empty_like(x)
+        y_at, y_stride = (y.data_ptr(), width) if y.is_contiguous() else row_span("x", y, y.dtype, index)
+    if rows:
         a = _lib.VmBlockNormArgs(x_at, r_at, post_at, gate_at, w_at, y_at, h_at, values_at, scales_at, x_stride, r_stride,
-                                 gate_stride, y_stride, h_stride, scale, residual_scale, eps, count // width, width, act,
-                                 res_act, post_code, gate_code, w_code, kind, sigmoid_gate, one_centered)
+                                 gate_stride, y_stride, h_stride, scale, residual_scale, eps, rows, width, act, res_act,
+                                 post_code, gate_code, w_code, kind, sigmoid_gate, one_centered)
         _lib.check(device_call(index, _lib.lib().vm_block_norm, ctypes.byref(a)))
     return h if weight is None else (y, h)
 

@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .device import ACT_DTYPES, device_call, require_32_bits, row_span
+from .device import ACT_DTYPES, device_call, require_32_bits, row_span, vector_of
 
 _SCORES = {"softmax": _lib.VM_SCORES_SOFTMAX, "sigmoid": _lib.VM_SCORES_SIGMOID}
 
@@ -54,18 +54,11 @@ def select_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax"
     if min(groups, top_groups, group_top) < 1:
         raise ValueError("groups, top_groups and group_top must be positive")
     require_32_bits(rows, experts, groups, top_groups, group_top)
-    bias_at, bias_code = None, code
-    if bias is not None:
-        if not isinstance(bias, torch.Tensor):
-            raise TypeError(f"bias must be a torch tensor on the GPU, got {type(bias).__name__}")
-        bias_code = _dtype_code("bias", bias.dtype)
-        if bias.shape != (experts,) or not bias.is_contiguous():
-            raise ValueError(f"bias must be contiguous of shape ({experts},)")
-        bias_at, _ = row_span("bias", bias, bias.dtype, index)
+    bias_at, bias_code = (None, code) if bias is None else vector_of("bias", bias, experts, index)
     out_code = _dtype_code("dtype", dtype)
-    shape = (*logits.shape[:-1], top_k)
-    inds = torch.empty(shape, dtype=torch.int32, device=logits.device)
-    weights = torch.empty(shape, dtype=dtype, device=logits.device)
+    shape, device = (*logits.shape[:-1], top_k), logits.device
+    inds = torch.empty(shape, dtype=torch.int32, device=device)
+    weights = logits.new_empty(shape) if logits.dtype == dtype else torch.empty(shape, dtype=dtype, device=device)
     a = _lib.VmSelectArgs(at, bias_at, inds.data_ptr(), weights.data_ptr(), stride, scale, rows, experts, groups, top_groups,
                           group_top, top_k, scores, renormalize, code, bias_code, out_code, 0)
     _lib.check(device_call(index, _lib.lib().vm_select_experts, ctypes.byref(a)))
