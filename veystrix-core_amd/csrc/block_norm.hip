@@ -7,8 +7,8 @@
 // gate: none, one per row, per channel or per value, as it is or through a sigmoid; gains are weight or 1 + weight.  The
 // second norm reads h as it was computed, before it is rounded to the residual's type.
 //
-// A row is read once: x and the residual stay in registers from the first sum of squares over the second to the last
-// store, eight consecutive values per thread and step, at any alignment (vm_any.h).  Squares are summed in 64 bits, which no value
+// A row is read once: x and the residual stay in registers, as they lie in memory, until the first sum of squares is
+// known, then h until the second; eight consecutive values per thread and step, at any alignment (vm_any.h).  Squares are summed in 64 bits, which no value
 // overflows and which costs two operations a value.  Rows to MX are computed in 64 bits throughout, so that e4m3's is
 // their one rounding.
 // Bound by HBM (two rows in, two out), or with few rows by one row's latency, which two sums over the row make up.
@@ -53,8 +53,35 @@ __device__ __forceinline__ Real gate_sigmoid(float g) {
   else return 1.0f / (1.0f + expf(-g));
 }
 
-// TPR threads per row (64 or 256), up to NV steps of eight values per thread.
-template <int TPR, int NV, bool MXOUT>
+// Eight values of a row as they lie in memory, so that a row waits for its sums in half of fp32's registers.
+template <class A>
+struct RawRun {
+  uint32_t w[A::kBytes * 2];
+  __device__ __forceinline__ void load(const void* row, uint32_t at, uint32_t width) {
+    const uint8_t* from = static_cast<const uint8_t*>(row) + static_cast<size_t>(at) * A::kBytes;
+    if (at + 8 <= width) {
+#pragma unroll
+      for (int q = 0; q < A::kBytes / 2; ++q) {
+        const words4 a = *(const __attribute__((address_space(1))) words4*)(from + 16 * q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[4 * q + i] = a[i];
+      }
+    } else {
+      uint32_t bits[8];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) bits[j] = at + j < width ? A::load_bits(row, at + j) : 0u;
+#pragma unroll
+      for (int i = 0; i < A::kBytes * 2; ++i) w[i] = A::kBytes == 2 ? bits[2 * i % 8] | (bits[(2 * i + 1) % 8] << 16) : bits[i % 8];
+    }
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (A::kBytes == 2) return __uint_as_float(j % 2 == 0 ? w[j / 2] << 16 : w[j / 2] & 0xffff0000u);
+    else return __uint_as_float(w[j]);
+  }
+};
+
+// Rows of A and residuals of R; TPR threads per row (64 or 256), up to NV steps of eight values per thread.
+template <class A, class R, int TPR, int NV, bool MXOUT>
 __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunch p) {
   using Real = std::conditional_t<MXOUT, double, float>;
   __shared__ double s_part[2][TPR / 64];
@@ -62,25 +89,14 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
   const uint32_t row = blockIdx.x * (kBlockNormThreads / TPR) + threadIdx.x / TPR;
   if (row >= p.rows) return;  // TPR 64: whole waves; TPR 256: never
   const auto at = [&](int i) { return (i * TPR + t) * 8u; };
-  Real h[NV][8];              // x, then the sum
-  float r[NV][8];
-  // the loads of a row are together on their way: one branch per operand, not per step
-  const auto load_row = [&](const void* from, uint32_t dtype, auto&& keep) {
-    const auto steps = [&](uint32_t type) {
+  RawRun<A> x[NV];
+  RawRun<R> r[NV];
+  const void* x_row = row_at(p.x, row, p.x_stride, p.act_dtype);
+  const void* r_row = row_at(p.residual, row, p.residual_stride, p.residual_dtype);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float v[8];
-        load_run<8>(from, type, at(i), p.width, v);
+  for (int i = 0; i < NV; ++i) x[i].load(x_row, at(i), p.width);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) keep(i, j, v[j]);
-      }
-    };
-    if (dtype == 0) steps(0u);
-    else steps(1u);
-  };
-  load_row(row_at(p.x, row, p.x_stride, p.act_dtype), p.act_dtype, [&](int i, int j, float v) { h[i][j] = v; });
-  load_row(row_at(p.residual, row, p.residual_stride, p.residual_dtype), p.residual_dtype,
-           [&](int i, int j, float v) { r[i][j] = v; });
+  for (int i = 0; i < NV; ++i) r[i].load(r_row, at(i), p.width);
   const double width = p.width;
   Real post = 1;
   if (p.post_weight != nullptr) {
@@ -88,7 +104,7 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fma(static_cast<double>(h[i][j]), static_cast<double>(h[i][j]), ss);
+      for (int j = 0; j < 8; ++j) ss = fma(static_cast<double>(x[i][j]), static_cast<double>(x[i][j]), ss);
     post = static_cast<Real>(1.0 / sqrt(row_total<TPR>(ss, s_part[0]) / width + p.eps));
   }
   const Real scale = static_cast<Real>(p.scale), residual_scale = static_cast<Real>(p.residual_scale);
@@ -102,9 +118,12 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
     gate = row_at(p.gate, row, p.gate_stride, p.gate_dtype);
   }
   void* sum_out = const_cast<void*>(row_at(p.sum_out, row, p.sum_stride, p.residual_dtype));
+  Real h[NV][8];
   double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[i][j] = x[i][j];
     if (p.post_weight != nullptr) {
       float w[8];
       load_run<8>(p.post_weight, p.post_dtype, at(i), p.width, w);
@@ -173,11 +192,11 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
   }
 }
 
-template <int TPR, int NV>
+template <class A, class R, int TPR, int NV>
 hipError_t block_norm_go(const BlockNormLaunch& p, hipStream_t stream) {
   const uint32_t per = kBlockNormThreads / TPR;
   const dim3 grid((p.rows + per - 1) / per);
-  auto kernel = p.values != nullptr ? &k_block_norm<TPR, NV, true> : &k_block_norm<TPR, NV, false>;
+  auto kernel = p.values != nullptr ? &k_block_norm<A, R, TPR, NV, true> : &k_block_norm<A, R, TPR, NV, false>;
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("norm", &start, &stop))
     hipExtLaunchKernelGGL(kernel, grid, dim3(kBlockNormThreads), 0, stream, start, stop, 0, p);
@@ -191,25 +210,32 @@ hipError_t block_norm_go(const BlockNormLaunch& p, hipStream_t stream) {
 // a block 26.6; 8192 of 2560 in five steps 34.5 and 40.
 constexpr uint32_t kBlockNormWaveRows = 1024, kBlockNormWaveSteps = 5;
 
+template <class A, class R>
+hipError_t block_norm_rows(const BlockNormLaunch& p, hipStream_t stream) {
+  const uint32_t steps = (p.width + 511) / 512;  // of one wave
+  if (p.rows >= kBlockNormWaveRows && steps <= kBlockNormWaveSteps) {
+    switch (steps) {
+      case 1: return block_norm_go<A, R, 64, 1>(p, stream);
+      case 2: return block_norm_go<A, R, 64, 2>(p, stream);
+      case 3:
+      case 4: return block_norm_go<A, R, 64, 4>(p, stream);
+      default: return block_norm_go<A, R, 64, 5>(p, stream);
+    }
+  }
+  if (steps <= 4) return block_norm_go<A, R, 256, 1>(p, stream);
+  if (steps <= 8) return block_norm_go<A, R, 256, 2>(p, stream);
+  if (steps <= 12) return block_norm_go<A, R, 256, 3>(p, stream);
+  if (steps <= 16) return block_norm_go<A, R, 256, 4>(p, stream);
+  return block_norm_go<A, R, 256, 8>(p, stream);
+}
+
 }  // namespace
 
 hipError_t launch_block_norm(const BlockNormLaunch& p, hipStream_t stream) {
   if (p.rows == 0 || p.width == 0 || p.width > kNormMaxWidth) return hipErrorInvalidValue;
-  const uint32_t steps = (p.width + 511) / 512;  // of one wave
-  if (p.rows >= kBlockNormWaveRows && steps <= kBlockNormWaveSteps) {
-    switch (steps) {
-      case 1: return block_norm_go<64, 1>(p, stream);
-      case 2: return block_norm_go<64, 2>(p, stream);
-      case 3:
-      case 4: return block_norm_go<64, 4>(p, stream);
-      default: return block_norm_go<64, 5>(p, stream);
-    }
-  }
-  if (steps <= 4) return block_norm_go<256, 1>(p, stream);
-  if (steps <= 8) return block_norm_go<256, 2>(p, stream);
-  if (steps <= 12) return block_norm_go<256, 3>(p, stream);
-  if (steps <= 16) return block_norm_go<256, 4>(p, stream);
-  return block_norm_go<256, 8>(p, stream);
+  if (p.act_dtype == 0)
+    return p.residual_dtype == 0 ? block_norm_rows<ActBF16, ActBF16>(p, stream) : block_norm_rows<ActBF16, ActF32>(p, stream);
+  return p.residual_dtype == 0 ? block_norm_rows<ActF32, ActBF16>(p, stream) : block_norm_rows<ActF32, ActF32>(p, stream);
 }
 
 }  // namespace vm

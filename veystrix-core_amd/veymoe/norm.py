@@ -45,11 +45,13 @@ def mx_empty(shape, device) -> MxTensor:
 
 
 def require_mx(name: str, t) -> MxTensor:
-    if not isinstance(t, MxTensor) or not all(isinstance(part, torch.Tensor) for part in t):
+    if not isinstance(t, MxTensor) or not isinstance(t[0], torch.Tensor) or not isinstance(t[1], torch.Tensor):
         raise TypeError(f"{name} must be an MxTensor of two tensors")
-    if t.values.dtype != torch.float8_e4m3fn or t.scales.dtype not in _SCALE_DTYPES:
+    values, scales = t
+    if values.dtype != torch.float8_e4m3fn or scales.dtype not in _SCALE_DTYPES:
         raise TypeError(f"{name} must hold float8_e4m3fn values and float8_e8m0fnu (or uint8) scales")
-    if t.values.shape[-1] % MX_GROUP or t.scales.shape != (*t.values.shape[:-1], t.values.shape[-1] // MX_GROUP):
+    shape, groups = values.shape, scales.shape
+    if not shape or not groups or groups[-1] * MX_GROUP != shape[-1] or groups[:-1] != shape[:-1]:
         raise ValueError(f"{name} needs one scale per {MX_GROUP} values of a row")
     return t
 
