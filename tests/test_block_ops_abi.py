@@ -175,3 +175,12 @@ def test_calls_of_nothing():
                              ("vm_linear", _lib.VmLinearArgs, LINEAR)):
         assert _call(entry, cls, base, {"rows": 0}) == _lib.VM_OK
         assert getattr(_lib.lib(), entry)(None, None) == _lib.VM_EINVAL
+
+
+def test_largest_legal_sizes_pass_the_checks_but_for_their_pointers():
+    """Sizes at the documented limits are not refused for their size."""
+    assert _call("vm_select_experts", _lib.VmSelectArgs, SELECT, {"rows": 1 << 25, "logits": None}) == _lib.VM_EINVAL
+    assert "required" in _lib.last_error()
+    wide = {"rows": 1 << 18, "n": 1 << 13, "out_stride": 1 << 13, "out": (1 << 20) + 64}
+    assert _call("vm_linear", _lib.VmLinearArgs, LINEAR, wide) == _lib.VM_EINVAL
+    assert "overlaps" in _lib.last_error()

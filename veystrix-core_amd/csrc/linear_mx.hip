@@ -1,0 +1,9 @@
+// Matrix products with an epilogue (vm_linear.h): MX operands.
+
+#include "vm_linear.h"
+
+namespace vm {
+
+hipError_t launch_linear_mx(const LinearLaunch& p, hipStream_t stream) { return linear_go<true>(p, stream); }
+
+}  // namespace vm

@@ -69,9 +69,9 @@ def linear(x, weight, bias: torch.Tensor = None, *, activation: str = None, resi
         bias_at, bias_code = vector_of("bias", bias, wv.shape[0], index)
     if residual is not None:
         res_code = _code("residual", residual)
+        res_at, res_stride = row_span("residual", residual, residual.dtype, index)
         if residual.shape != shape:
             raise ValueError(f"residual must have shape {shape}")
-        res_at, res_stride = row_span("residual", residual, residual.dtype, index)
     if out is None:
         y = xv.new_empty(shape) if xv.dtype == dtype else torch.empty(shape, dtype=dtype, device=xv.device)
         y_at, y_stride = y.data_ptr(), n
