@@ -98,22 +98,21 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
 #pragma unroll
   for (int i = 0; i < NV; ++i) r[i].load(r_row, at(i), p.width);
   const double width = p.width;
-  Real post = 1;
+  double factor = p.scale;   // of every value of x: its norm's, the row's gate and the scale
   if (p.post_weight != nullptr) {
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fma(static_cast<double>(x[i][j]), static_cast<double>(x[i][j]), ss);
-    post = static_cast<Real>(1.0 / sqrt(row_total<TPR>(ss, s_part[0]) / width + p.eps));
+    factor /= sqrt(row_total<TPR>(ss, s_part[0]) / width + p.eps);
   }
-  const Real scale = static_cast<Real>(p.scale), residual_scale = static_cast<Real>(p.residual_scale);
+  const Real residual_scale = static_cast<Real>(p.residual_scale);
   const Real one = p.one_centered ? 0 : 1;
   const void* gate = p.gate;
-  Real row_gate = 1;
   if (p.gate_kind == kGateRow) {
     const float g = load_any(row_at(p.gate, row, p.gate_stride, p.gate_dtype), 0, p.gate_dtype);
-    row_gate = p.sigmoid_gate ? gate_sigmoid<Real>(g) : static_cast<Real>(g);
+    factor *= p.sigmoid_gate ? gate_sigmoid<double>(g) : static_cast<double>(g);
   } else if (p.gate_kind == kGateValue) {
     gate = row_at(p.gate, row, p.gate_stride, p.gate_dtype);
   }
@@ -123,12 +122,12 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[i][j] = x[i][j];
+    for (int j = 0; j < 8; ++j) h[i][j] = static_cast<Real>(x[i][j]) * static_cast<Real>(factor);
     if (p.post_weight != nullptr) {
       float w[8];
       load_run<8>(p.post_weight, p.post_dtype, at(i), p.width, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * post * (one + static_cast<Real>(w[j]));
+      for (int j = 0; j < 8; ++j) h[i][j] *= one + static_cast<Real>(w[j]);
     }
     if (p.gate_kind == kGateChannel || p.gate_kind == kGateValue) {
       float g[8];
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
     float sum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      h[i][j] = residual_scale * static_cast<Real>(r[i][j]) + scale * (row_gate * h[i][j]);
+      h[i][j] = fma(residual_scale, static_cast<Real>(r[i][j]), h[i][j]);
       if (at(i) >= p.width) h[i][j] = 0;   // zeros there, but times a scale that is no number
       sum[j] = static_cast<float>(h[i][j]);
     }
