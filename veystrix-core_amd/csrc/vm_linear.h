@@ -254,8 +254,8 @@ __device__ __forceinline__ uint32_t scale_bytes(const uint8_t* row, uint32_t c, 
   return v;
 }
 
-// WM x WN x WK waves; each multiplies 16 RF rows by 16 CF matrix rows, over every WK-th chunk.
-template <bool MX, int RF, int CF, int WM, int WN, int WK>
+// WM x WN x WK waves; each multiplies 16 RF rows by 16 CF matrix rows, over every WK-th chunk; S stages.
+template <bool MX, int RF, int CF, int WM, int WN, int WK, int S>
 __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear(LinearLaunch p) {
   constexpr int kWaves = WM * WN * WK;
   constexpr uint32_t kRows = 16 * RF * WM, kMatrix = 16 * CF * WN;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear(LinearLaunch p) {
   const uint32_t steps = (chunks + WK - 1) / WK;
   const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_linear_zeros);
   VM_KEEP(zeros);
-  uint32_t held_x[2][kXWords], held_w[2][kWWords];   // the scale bytes of the stages
+  uint32_t held_x[S][kXWords], held_w[S][kWWords];   // the scale bytes of the stages
   const auto begin = [&](auto J, uint32_t step) {
     constexpr int j = decltype(J)::value;
     const uint32_t c = step * WK + wk;
@@ -358,17 +358,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear(LinearLaunch p) {
     }
   };
 
-  // Two stages: one is multiplied while the next step's chunks are on their way to the other (behind the last step that
-  // one again, which is not read).
-  begin(std::integral_constant<int, 0>{}, 0);
-  for (uint32_t step = 0; step < steps; step += 2) {
-    unroll<0, 2>([&](auto J) {
+  // One stage is multiplied while the others' steps are on their way (behind the last step zeros, so that every step has
+  // as many loads).
+  unroll<0, S - 1>([&](auto J) { begin(J, decltype(J)::value); });
+  for (uint32_t step = 0; step < steps; step += S) {
+    unroll<0, S>([&](auto J) {
       constexpr int j = decltype(J)::value;
       if (step + j >= steps) return;
-      wait_vm<0>();    // this wave's loads of the stage have landed
-      wait_lgkm0();    // its reads of the other stage are done
+      wait_vm<(S - 2) * kLoads>();   // this wave's loads of the stage have landed
+      wait_lgkm0();                  // its reads of the stage before are done
       bare_barrier();
-      begin(std::integral_constant<int, 1 - j>{}, min(step + j + 1, steps - 1));
+      begin(std::integral_constant<int, (j + S - 1) % S>{}, step + j + S - 1);
       compute(J);
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -687,11 +687,11 @@ hipError_t go(Kernel kernel, uint64_t blocks, uint32_t threads, const LinearLaun
   return hipGetLastError();
 }
 
-template <bool MX, int RF, int CF, int WM, int WN, int WK>
+template <bool MX, int RF, int CF, int WM, int WN, int WK, int S>
 hipError_t tiles_go(const LinearLaunch& p, hipStream_t stream) {
   const uint32_t rows = 16 * RF * WM, cols = 16 * CF * WN / (p.activation == kActSwiglu ? 2 : 1);
   const uint64_t blocks = uint64_t((p.rows + rows - 1) / rows) * ((p.n + cols - 1) / cols);
-  return go(&k_linear<MX, RF, CF, WM, WN, WK>, blocks, 64 * WM * WN * WK, p, stream);
+  return go(&k_linear<MX, RF, CF, WM, WN, WK, S>, blocks, 64 * WM * WN * WK, p, stream);
 }
 
 template <bool MX, int RF, int CF, int WM, int WN>
@@ -720,49 +720,63 @@ hipError_t few_go(const LinearLaunch& p, hipStream_t stream) {
   return go(&k_few<MX, R>, (p.n + cols - 1) / cols, 64 * waves, p, stream);
 }
 
-// Tiles of a form: their rows and matrix rows, how many of them the chip holds at once, and what a round of them takes
-// in us, for each 32 inputs and besides: with every place taken, and with a tile per CU at most.  Measured at 512 to 2560
-// inputs in either format (an MX step of 64 inputs takes what two of bf16 take); the model is within 20 % of the calls
-// that it was not fitted to.
+// Tiles of a form: their rows and matrix rows, how many of them a CU holds at once, and the us in which it computes one
+// alone and all that it holds: a fixed part and one per 32 inputs.  Fitted to calls of 512 to 2560 inputs and one to six
+// rounds of tiles in either format (an MX step of 64 inputs takes about what two of bf16 take); within 20 % of most.
 struct TileForm {
   uint32_t rows, matrix, places;
-  float full, full_step, one, one_step;
+  float one, one_step, full, full_step;
 };
 enum : int { kForm16, kForm32, kForm32x64, kForm64, kForm128, kForm128x320, kForm256, kForm256x320, kForms };
+constexpr uint32_t kCus = 256;
+template <bool MX>
 constexpr TileForm kTileForms[kForms] = {
-    {16, 16, 512, 3.0f, 0.120f, 2.5f, 0.055f},      // 8 waves, each every eighth chunk
-    {32, 32, 512, 4.0f, 0.140f, 3.5f, 0.080f},      // 16 waves, each every fourth
-    {32, 64, 768, 4.0f, 0.220f, 3.5f, 0.160f},      // 8 waves, each every other
-    {64, 64, 768, 8.3f, 0.245f, 8.0f, 0.200f},     // 4 waves
-    {128, 128, 512, 9.0f, 0.450f, 5.9f, 0.277f},    // the large tiles of two groups of waves
-    {128, 320, 256, 14.0f, 0.400f, 14.0f, 0.400f},
-    {256, 256, 256, 12.0f, 0.550f, 12.0f, 0.550f},
-    {256, 320, 256, 18.0f, 0.750f, 18.0f, 0.750f},
+    {16, 16, 2, 2.5f, 0.045f, 2.5f, 0.060f},        // 8 waves, each every eighth chunk
+    {32, 32, 2, 3.5f, 0.058f, 4.0f, 0.090f},        // 16 waves, each every fourth
+    {32, 64, 2, 3.5f, 0.080f, 5.0f, 0.100f},        // 8 waves, each every other
+    {64, 64, 3, 6.0f, 0.100f, 8.0f, 0.220f},        // 4 waves
+    {128, 128, 2, 5.9f, 0.277f, 9.0f, 0.500f},      // the large tiles of two groups of waves
+    {128, 320, 1, 14.0f, 0.450f, 14.0f, 0.450f},
+    {256, 256, 1, 12.0f, 0.580f, 12.0f, 0.580f},
+    {256, 320, 1, 18.0f, 0.820f, 18.0f, 0.820f},
+};
+template <>
+constexpr TileForm kTileForms<true>[kForms] = {
+    {16, 16, 2, 2.5f, 0.042f, 2.5f, 0.050f},
+    {32, 32, 2, 3.5f, 0.058f, 4.0f, 0.080f},
+    {32, 64, 3, 3.8f, 0.085f, 6.0f, 0.165f},
+    {64, 64, 3, 5.0f, 0.137f, 8.0f, 0.235f},
+    {128, 128, 2, 5.9f, 0.240f, 9.0f, 0.400f},
+    {128, 320, 1, 14.0f, 0.450f, 14.0f, 0.450f},
 };
 // Rows up to which a block reads its matrix rows once for all of them, without MFMA: eight rows 7.6 us by 2560 x 2560,
 // in 16 x 16 tiles 6.8; four 5.8.
 constexpr uint32_t kFewRows = 4;
 
-// The form of the least time by the model.
+// The form of the least time by the model, and whether no CU holds two of its tiles.
+struct Choice {
+  int form;
+  bool alone;
+};
 template <bool MX>
-int choose_form(const LinearLaunch& p) {
+Choice choose_form(const LinearLaunch& p) {
   const uint32_t matrix = p.activation == kActSwiglu ? 2 * p.n : p.n;
   const float steps = static_cast<float>(p.k_bytes) / (MX ? 32.0f : 64.0f);
   // the large tiles take scales by the word and row offsets of 32 bits; of MX 256 x 320 would outgrow the LDS, and 256 x 256
   // is slower than 128 x 320 (a full round of the chip 62 us for 52, of a fifth fewer products)
   const int forms = near_rows(p) && (!MX || p.whole_scales) ? (MX ? kForm256 : kForms) : kForm128;
-  int best = kForm16;
+  Choice best{kForm16, false};
   float least = __builtin_huge_valf();
   for (int f = 0; f < forms; ++f) {
-    const TileForm& t = kTileForms[f];
+    const TileForm& t = kTileForms<MX>[f];
     const uint64_t tiles = uint64_t((p.rows + t.rows - 1) / t.rows) * ((matrix + t.matrix - 1) / t.matrix);
-    const uint64_t left = tiles % t.places;
-    float us = static_cast<float>(tiles / t.places) * (t.full + t.full_step * steps);
-    if (left > 256) us += t.full + t.full_step * steps;
-    else if (left > 0) us += t.one + t.one_step * steps;
+    const uint64_t left = tiles % (t.places * kCus), held = (left + kCus - 1) / kCus;   // by a CU, of the last round
+    const float one = t.one + t.one_step * steps, full = t.full + t.full_step * steps;
+    float us = static_cast<float>(tiles / (t.places * kCus)) * full;
+    if (held > 0) us += t.places == 1 ? full : one + (full - one) * static_cast<float>(held - 1) / static_cast<float>(t.places - 1);
     if (us < least) {
       least = us;
-      best = f;
+      best = {f, tiles <= kCus};
     }
   }
   return best;
@@ -775,17 +789,21 @@ hipError_t linear_go(const LinearLaunch& p, hipStream_t stream) {
     if (p.rows == 2) return few_go<MX, 2>(p, stream);
     return few_go<MX, 4>(p, stream);
   }
-  const int choose = choose_form<MX>(p);
-  switch (choose) {
-    case kForm16: return tiles_go<MX, 1, 1, 1, 1, 8>(p, stream);
-    case kForm32: return tiles_go<MX, 1, 1, 2, 2, 4>(p, stream);
-    case kForm32x64: return tiles_go<MX, 1, 2, 2, 2, 2>(p, stream);
-    case kForm64: return tiles_go<MX, 2, 2, 2, 2, 1>(p, stream);
+  // More stages than two keep more loads on their way where a CU's LDS would hold no other tile anyway: 64 rows by
+  // 2560 x 2560 9.9 to 8.1 us in 32 x 32 tiles with four, 128 rows 14.0 to 9.8 in 32 x 64 with three, 2048 rows 49 to 43 in
+  // 64 x 64 with three.  Of MX the scales' registers wait for the loads between: two are the fastest everywhere.
+  constexpr int kDeep = MX ? 2 : 3;
+  const Choice c = choose_form<MX>(p);
+  switch (c.form) {
+    case kForm16: return c.alone ? tiles_go<MX, 1, 1, 1, 1, 8, kDeep>(p, stream) : tiles_go<MX, 1, 1, 1, 1, 8, 2>(p, stream);
+    case kForm32: return c.alone ? tiles_go<MX, 1, 1, 2, 2, 4, MX ? 2 : 4>(p, stream) : tiles_go<MX, 1, 1, 2, 2, 4, 2>(p, stream);
+    case kForm32x64: return tiles_go<MX, 1, 2, 2, 2, 2, kDeep>(p, stream);
+    case kForm64: return tiles_go<MX, 2, 2, 2, 2, 1, kDeep>(p, stream);
     case kForm128: return large_go<MX, 2, 4, 4, 2>(p, stream);
     case kForm128x320: return large_go<MX, 2, 10, 4, 2>(p, stream);
     default: break;
   }
-  if constexpr (!MX) return choose == kForm256 ? large_go<MX, 4, 8, 4, 2>(p, stream) : large_go<MX, 4, 10, 4, 2>(p, stream);
+  if constexpr (!MX) return c.form == kForm256 ? large_go<MX, 4, 8, 4, 2>(p, stream) : large_go<MX, 4, 10, 4, 2>(p, stream);
   return hipErrorInvalidValue;
 }
 
