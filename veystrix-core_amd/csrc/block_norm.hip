@@ -11,7 +11,10 @@
 // known, then h until the second; eight consecutive values per thread and step, at any alignment (vm_any.h).  Squares are summed in 64 bits, which no value
 // overflows and which costs two operations a value.  Rows to MX are computed in 64 bits throughout, so that e4m3's is
 // their one rounding.
-// Bound by HBM (two rows in, two out), or with few rows by one row's latency, which two sums over the row make up.
+// Bound by HBM (two rows in, two out), or with few rows by one row's latency, which two sums over the row make up: 8192 rows
+// of 2560, bf16 32 us (168 MB, 5.3 TB/s), with an fp32 residual 41.5 (252 MB, 6.1), to MX 37.8 (147 MB, 3.9 TB/s; the 64-bit
+// operations, about 18 a value); one row 5.0.  A sigmoid of a gate per channel or value costs a 64-bit exponential each to
+// MX: 8192 rows of 2560 62 us.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>

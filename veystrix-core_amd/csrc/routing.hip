@@ -9,8 +9,15 @@
 // Choices are compared as they are in 64 bits: biases and scores lie so close that in 32 bits every tenth window of 8192
 // tokens would hold a token whose experts, or their order, differ from the formula's.
 //
-// One wave per row.  The groups are dealt to the lanes, a power of two of lanes to each and V neighbouring experts to a
-// lane, so that the order (lane, value) is the experts' order and a group's sums stay within its lanes.
+// One wave per row.  The groups are dealt to the lanes, a power of two of lanes to each and up to 32 neighbouring experts to
+// a lane, so that the order (lane, value) is the experts' order and a group's sums stay within its lanes.
+//
+// 64 bits for all experts would be most of the work (8192 rows of 512 with a sigmoid and a bias, top-10, 31 us).  So choices in
+// 32 bits find the candidates: the top_k-th largest of the lanes' largest choices, less what 32 bits may be off, is a bound
+// that every chosen expert passes and few others do; those, one to a lane, are compared in 64 bits (11.4 us; the logits alone
+// are 17 MB, 3.4 at a copy's rate; bound by a wave's instructions, of which a third are the bound's reductions).  Groups are
+// decided in 32 bits where kept and lost ones lie further apart than 32 bits may be off.  Rows that are not decided so
+// (masses of equal choices, groups that nearly tie) take the whole way in 64 bits.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>

@@ -3,10 +3,17 @@
 // Matrix products with bias, activation and residual in their epilogue (vm_linear):
 //   out = activation(x . W^T + bias) + residual, fp32 sums, bf16 or MX operands (vm_mx.h), out in bf16 or fp32.
 //
-// Both formats move as 128-byte chunks of a row (64 bf16 or 128 e4m3 inputs) made of eight 16-byte units, staged in LDS
-// by DMA (vm_dma.h); an MX unit is converted to two bf16 operands in registers (vm_operand.h), so both formats have the
-// bf16 unit's sums.  The matrix is the first operand, the rows the second, so a lane receives four neighbouring outputs
-// of row lane % 16.  The sums go through LDS to the epilogue, whose threads own eight neighbouring outputs each.
+// Both formats move as runs of a row (64 or 128 bytes: 16-byte units of 8 bf16 or 16 e4m3 inputs), staged in LDS by DMA
+// (vm_dma.h); an MX unit is converted to two bf16 operands in registers (vm_operand.h), so both formats have the bf16
+// unit's sums.  The matrix is the first operand, the rows the second, so a lane receives four neighbouring outputs of row
+// lane % 16.  Four kinds of calls, chosen by choose_form below:
+//   k_few     up to four rows: the matrix read once by plain loads, no MFMA; bound by its bytes (one row 2560 -> 2560, 13 MB,
+//             4.5 us, of which a launch is two).
+//   k_linear  small tiles, whose waves share the inputs where there are few tiles, so that a call of few rows is done in
+//             a few steps: bound by the loads' way from L2 and HBM (32 rows MX 2560 -> 2 x 640 5.5 us, 333 rows 1000 -> 1333
+//             8.2, 2048 rows 2048 -> 512 13.1: 200 MB past the L2s at 15 TB/s).
+//   k_large   large tiles: bound by the products (1100 to 1280 TFLOP/s of 2560 inputs, 1430 of 8192, a library's 8192^3
+//             product 1660) and, all tiles of a round ending together, by the outputs' way to HBM.
 
 #pragma once
 
@@ -431,8 +438,11 @@ __device__ __forceinline__ uint32_t strip_swz(uint32_t r) { return (((r >> 1) ^ 
 // and a slot of MFMAs; the second group runs a slot behind the first, so that one reads while the other multiplies.  Four
 // stages hold the step being read and three on their way.  Every wait for loads is the kernel's own: the compiler's, for
 // loads that it issued, came before every read and cost a third of the time.
-// 8192 x 2560 x 2560 84 us at 256 x 320 (1280 TFLOP/s, MFMA's 62 us at the clock it ran; two stages of 128 bytes 95, half
-// of the matrix rows per slot 90, loads' addresses in 64 bits 87); with bias, SiLU and residual 103.
+// 8192 x 2560 x 2560 84 to 88 us at 256 x 320 (two stages of 128 bytes 95, half of the matrix rows per slot 90, loads'
+// addresses in 64 bits 87), of which the MFMAs take 50 at the 2.0 GHz that it runs at; with bias, SiLU and residual 98, of
+// operands that come from HBM 112.  A library's product of this size, without an epilogue, took 106.  Not kept: loads in
+// the MFMAs' slot, waves' priorities the other way round (within 1 %), lines of later steps (4 to 8 ahead) or of the residual
+// asked for beforehand (8 % and 1 % slower).
 // Fragments of the matrix are dealt in pairs: a lane's eight values of a pair are neighbouring outputs of its row (with
 // SwiGLU four gates and four ups of neighbouring outputs), so that sums go from registers to memory.
 template <bool MX, int EPI, int RF, int CF, int WM, int WN>

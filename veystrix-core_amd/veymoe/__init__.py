@@ -13,6 +13,9 @@ Public surface (reference counterparts in joyboyreturns/Veystrix-Core):
   norm.rms_norm / mx_quantize / MxTensor                    patch_rmsnorm.py (MX rows: none)
   products.grouped_matmul (bf16 and MX experts)             the gather_qmm call of expert_cache.py
   adapters.add_adapters                                     none
+  norm.block_norm (a block's two norms, gate and residual)  patch_rmsnorm.py (the norm alone)
+  linear.linear (bf16 and MX products with an epilogue)     none
+  routing.select_experts (scores, bias, groups, top-k)      adaptive_topk.py (softmax and top-k alone)
 """
 from .executor import (BITS, GROUP_SIZE, MAX_EXPERTS, MAX_TOKENS, MAX_TOP_K, MAX_WIDTH, HipCapabilities,
                        HipMoEExecutor, Q4G32Projection, probe_capabilities, weighted_combine)
