@@ -11,7 +11,7 @@
 //             4.5 us, of which a launch is two).
 //   k_linear  small tiles, whose waves share the inputs where there are few tiles, so that a call of few rows is done in
 //             a few steps: bound by the loads' way from L2 and HBM (32 rows MX 2560 -> 2 x 640 5.5 us, 333 rows 1000 -> 1333
-//             8.2, 2048 rows 2048 -> 512 13.1: 200 MB past the L2s at 15 TB/s).
+//             7.4, 2048 rows 2048 -> 512 10.6: 134 MB past the L2s at 13 TB/s).
 //   k_large   large tiles: bound by the products (1100 to 1280 TFLOP/s of 2560 inputs, 1430 of 8192, a library's 8192^3
 //             product 1660) and, all tiles of a round ending together, by the outputs' way to HBM.
 
@@ -243,7 +243,19 @@ __device__ __forceinline__ f32x4_t unit_product(const Operand<MX>& w, const Oper
   return acc;
 }
 
-// One LDS object per stage, so that the compiler can tell the stage being read from the one being filled.
+// Tile (row tile, column tile) of a block: every XCD (blocks b, b + 8, ..) takes a run of tiles, and runs go down columns
+// of up to eight row tiles, so that the tiles of one L2 share rows and matrix rows (2048 rows 2048 -> 512 in 32 x 64 tiles
+// 11.3 us, row after row 13.1).
+__device__ __forceinline__ void tile_of(uint32_t block, uint32_t row_tiles, uint32_t col_tiles, uint32_t* row, uint32_t* col) {
+  const uint32_t total = row_tiles * col_tiles, xcd = block & 7u, each = total >> 3, over = total & 7u;
+  const uint32_t t = xcd * each + min(xcd, over) + (block >> 3);
+  const uint32_t panel = t / (8u * col_tiles), in = t % (8u * col_tiles);
+  const uint32_t height = min(8u, row_tiles - panel * 8u);
+  *row = panel * 8u + in % height;
+  *col = in / height;
+}
+
+// LDS of stage J.
 template <int J, int BYTES>
 __device__ __forceinline__ uint8_t* linear_stage() {
   __shared__ uint4 buf[BYTES / 16];
@@ -275,8 +287,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear(LinearLaunch p) {
   const uint32_t wk = wave / (WM * WN), wmn = wave % (WM * WN), wm = wmn % WM, wn = wmn / WM;
   const bool pairs = p.activation == kActSwiglu;
   const uint32_t cols = pairs ? kMatrix / 2 : kMatrix;        // outputs per block
-  const uint32_t slices = (p.n + cols - 1) / cols;
-  const uint32_t row0 = blockIdx.x / slices * kRows, col0 = blockIdx.x % slices * cols;
+  uint32_t row_tile, col_tile;
+  tile_of(blockIdx.x, (p.rows + kRows - 1) / kRows, (p.n + cols - 1) / cols, &row_tile, &col_tile);
+  const uint32_t row0 = row_tile * kRows, col0 = col_tile * cols;
   const auto x_row = [&](uint32_t r) { return static_cast<uint64_t>(min(row0 + r, p.rows - 1)); };
   const auto w_row = [&](uint32_t r) {   // with SwiGLU the second half of the block's matrix rows are up rows
     const bool up = pairs && r >= cols;
@@ -417,17 +430,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear(LinearLaunch p) {
 }
 
 // ---------------------------------------------------------- large tiles ---
-
-// Tile (row tile, column tile) of a block: every XCD (blocks b, b + 8, ..) takes a run of tiles, and runs go down columns
-// of up to eight row tiles, so that the tiles of one L2 share rows and matrix rows.
-__device__ __forceinline__ void tile_of(uint32_t block, uint32_t row_tiles, uint32_t col_tiles, uint32_t* row, uint32_t* col) {
-  const uint32_t total = row_tiles * col_tiles, xcd = block & 7u, each = total >> 3, over = total & 7u;
-  const uint32_t t = xcd * each + min(xcd, over) + (block >> 3);
-  const uint32_t panel = t / (8u * col_tiles), in = t % (8u * col_tiles);
-  const uint32_t height = min(8u, row_tiles - panel * 8u);
-  *row = panel * 8u + in % height;
-  *col = in / height;
-}
 
 // Units of a row of 64 bytes lie at unit u ^ strip_swz(row) of it: the four lane groups of a read (lane: row lane % 16,
 // unit lane / 16) then meet all 64 banks each.
@@ -737,7 +739,7 @@ struct TileForm {
   uint32_t rows, matrix, places;
   float one, one_step, full, full_step;
 };
-enum : int { kForm16, kForm32, kForm32x64, kForm64, kForm128, kForm128x320, kForm256, kForm256x320, kForms };
+enum : int { kForm16, kForm32, kForm32x64, kForm64, kForm64Deep, kForm128, kForm128x320, kForm256, kForm256x320, kForms };
 constexpr uint32_t kCus = 256;
 template <bool MX>
 constexpr TileForm kTileForms[kForms] = {
@@ -745,6 +747,7 @@ constexpr TileForm kTileForms[kForms] = {
     {32, 32, 2, 3.5f, 0.058f, 4.0f, 0.090f},        // 16 waves, each every fourth
     {32, 64, 2, 3.5f, 0.080f, 5.0f, 0.100f},        // 8 waves, each every other
     {64, 64, 3, 6.0f, 0.100f, 8.0f, 0.220f},        // 4 waves
+    {64, 64, 1, 5.5f, 0.075f, 5.5f, 0.075f},        // 8 waves, each every other chunk
     {128, 128, 2, 5.9f, 0.277f, 9.0f, 0.500f},      // the large tiles of two groups of waves
     {128, 320, 1, 14.0f, 0.450f, 14.0f, 0.450f},
     {256, 256, 1, 12.0f, 0.580f, 12.0f, 0.580f},
@@ -756,6 +759,7 @@ constexpr TileForm kTileForms<true>[kForms] = {
     {32, 32, 2, 3.5f, 0.058f, 4.0f, 0.080f},
     {32, 64, 3, 3.8f, 0.085f, 6.0f, 0.165f},
     {64, 64, 3, 5.0f, 0.137f, 8.0f, 0.235f},
+    {64, 64, 0, 0.0f, 0.000f, 0.0f, 0.000f},        // no faster than 32 x 64: not built
     {128, 128, 2, 5.9f, 0.240f, 9.0f, 0.400f},
     {128, 320, 1, 14.0f, 0.450f, 14.0f, 0.450f},
 };
@@ -779,6 +783,7 @@ Choice choose_form(const LinearLaunch& p) {
   float least = __builtin_huge_valf();
   for (int f = 0; f < forms; ++f) {
     const TileForm& t = kTileForms<MX>[f];
+    if (t.places == 0) continue;
     const uint64_t tiles = uint64_t((p.rows + t.rows - 1) / t.rows) * ((matrix + t.matrix - 1) / t.matrix);
     const uint64_t left = tiles % (t.places * kCus), held = (left + kCus - 1) / kCus;   // by a CU, of the last round
     const float one = t.one + t.one_step * steps, full = t.full + t.full_step * steps;
@@ -813,6 +818,8 @@ hipError_t linear_go(const LinearLaunch& p, hipStream_t stream) {
     case kForm128x320: return large_go<MX, 2, 10, 4, 2>(p, stream);
     default: break;
   }
+  if constexpr (!MX)
+    if (c.form == kForm64Deep) return tiles_go<MX, 2, 2, 2, 2, 2, kDeep>(p, stream);
   if constexpr (!MX) return c.form == kForm256 ? large_go<MX, 4, 8, 4, 2>(p, stream) : large_go<MX, 4, 10, 4, 2>(p, stream);
   return hipErrorInvalidValue;
 }
