@@ -14,8 +14,8 @@
 //
 // 64 bits for all experts would be most of the work (8192 rows of 512 with a sigmoid and a bias, top-10, 31 us).  So choices in
 // 32 bits find the candidates: the top_k-th largest of the lanes' largest choices, less what 32 bits may be off, is a bound
-// that every chosen expert passes and few others do; those, one to a lane, are compared in 64 bits (11.4 us; the logits alone
-// are 17 MB, 3.4 at a copy's rate; bound by a wave's instructions, of which a third are the bound's reductions).  Groups are
+// that every chosen expert passes and few others do; those, one to a lane, are compared in 64 bits (10.8 us; the logits alone
+// are 17 MB, 3.4 at a copy's rate; bound by a wave's instructions: 470 vector ones, of which the scores are a fourth).  Groups are
 // decided in 32 bits where kept and lost ones lie further apart than 32 bits may be off.  Rows that are not decided so
 // (masses of equal choices, groups that nearly tie) take the whole way in 64 bits.
 
@@ -349,11 +349,12 @@ __device__ bool route_narrow(const RouteLaunch& p, uint32_t row, uint32_t lane, 
   uint32_t best = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) best = max(best, key[j]);
+  // Its first 18 bits are enough: a bound that is 2^-9 low lets few more pass, and takes a comparison a bit.
   uint32_t least = 0;
-  for (uint32_t k = 0; k < p.top_k; ++k) {
-    least = wave_max_u32(best);
-    if (least == 0) break;
-    best = best == least ? 0u : best;
+#pragma unroll
+  for (int bit = 31; bit >= 14; --bit) {
+    const uint32_t more = least | (1u << bit);
+    if (static_cast<uint32_t>(__builtin_popcountll(__ballot(best >= more))) >= p.top_k) least = more;
   }
   if (least == 0) {   // fewer lanes hold open experts: the top_k-th largest itself, or all
     uint32_t left[V];
@@ -406,9 +407,10 @@ __device__ bool route_narrow(const RouteLaunch& p, uint32_t row, uint32_t lane, 
   uint64_t order = 0;
   if (live) order = choice_key(biased ? mass + static_cast<double>(load_any(p.bias, own.x, p.bias_dtype)) : logit);
   uint32_t place = 0;
-  for (uint32_t c = 0; c < count; ++c) {
-    const uint64_t other = readlane_u64(order, c);
-    place += other > order || (other == order && c < lane) ? 1u : 0u;
+  for (uint32_t c = 0; c < count; ++c) {   // candidate c's place: those before it, and of its own choice the earlier ones
+    const uint64_t its = readlane_u64(order, c);
+    const uint64_t before_it = __ballot(order > its) | (__ballot(order == its) & ((1ull << c) - 1ull));
+    place = lane == c ? static_cast<uint32_t>(__builtin_popcountll(before_it)) : place;
   }
   const bool chosen = live && place < p.top_k;
   const double total = p.renormalize ? wave_sum_f64(chosen ? mass : 0.0) : 1.0;
