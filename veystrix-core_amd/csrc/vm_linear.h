@@ -75,15 +75,14 @@ __device__ __forceinline__ float gelu32(float v) {
   return v * (v < 0.0f ? q : 1.0f - q);
 }
 
-// v or 1 times 1 / (1 + e^-(v (a + b v^2))): silu, sigmoid and, since (1 + tanh t) / 2 is the sigmoid of 2 t, gelu_tanh.
+// v or 1 times 1 / (1 + e^-u): silu, sigmoid (u = v) and, since (1 + tanh t) / 2 is the sigmoid of 2 t, gelu_tanh, whose
+// u = v (a + b v^2) alone takes the square, which overflows from 2^64 on: times a b of zero it would be no number.
 struct SigmoidForm {
-  float a, b;
-  bool times;
+  bool cubic, times;
   __device__ __forceinline__ explicit SigmoidForm(uint32_t activation)
-      : a(activation == kActGeluTanh ? 0x1.988454p+0f : 1.0f), b(activation == kActGeluTanh ? 0x1.2444f2p-4f : 0.0f),
-        times(activation != kActSigmoid) {}
+      : cubic(activation == kActGeluTanh), times(activation != kActSigmoid) {}
   __device__ __forceinline__ float operator()(float v) const {
-    const float s = sigmoid32(v * (times ? fmaf(v * v, b, a) : 1.0f));
+    const float s = sigmoid32(cubic ? v * fmaf(v * v, 0x1.2444f2p-4f, 0x1.988454p+0f) : v);
     return times ? v * s : s;
   }
 };
