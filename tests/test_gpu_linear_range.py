@@ -1,5 +1,5 @@
-"""linear's activations of sums at the ends of fp32: sums whose square overflows, infinities; one to four rows, small tiles and
-large ones."""
+"""linear's activations of sums at the ends of fp32: results that are subnormal or just above, sums whose square overflows,
+infinities; one to four rows, small tiles and large ones."""
 import math
 
 import pytest
@@ -41,3 +41,20 @@ def test_sums_of_any_size(device, rows, activation):
     for dtype in (FP32, BF16):
         got = linear(x.to(device), w.to(device), activation=activation, dtype=dtype)
         assert_within(got, want, 4 * F32 * want.abs() + HALF_STEP[dtype] * want.abs() + 2.0 ** -149, activation)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "sigmoid", "swiglu"])
+@pytest.mark.parametrize("rows", ROWS)
+def test_results_down_to_the_least(device, rows, activation):
+    """Sums over which the results fall through the end of fp32's normal range to zero: a relative error, and of subnormal
+    ones half a step of the last rounding."""
+    low, high = {"gelu": (11.0, 14.6), "gelu_tanh": (8.5, 11.4)}.get(activation, (78.0, 110.0))
+    sums = -torch.linspace(low, high, N)
+    b = torch.cat([sums, torch.ones(N)]) if activation == "swiglu" else sums
+    x, w = torch.zeros((rows, K), dtype=BF16), torch.zeros((len(b), K), dtype=BF16)
+    want, steps = _expected(sums.double().expand(rows, N), activation)
+    assert want.abs().min() < 2.0 ** -148 and want.abs().max() > 2.0 ** -120
+    err = want.abs() * F32 * steps + 2.0 ** -150
+    for dtype in (FP32, BF16):
+        got = linear(x.to(device), w.to(device), b.to(device), activation=activation, dtype=dtype)
+        assert_within(got, want, err + ((want.abs() + err) * HALF_STEP[BF16] + 2.0 ** -134 if dtype == BF16 else 0.0), activation)

@@ -52,38 +52,39 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 
 // ------------------------------------------------------------- epilogue ---
 
-// 1 / (1 + e^-v)
-__device__ __forceinline__ float sigmoid32(float v) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -0x1.715476p+0f));
-}
-
 // What an instance's epilogue computes, so that unrolled code holds one activation.
 enum : int { kEpiPlain = 0, kEpiSigmoid = 1, kEpiGelu = 2, kEpiSwiglu = 3 };
 
 // v Phi(v).  For z = |v| / sqrt 2, Phi(-|v|) = erfc(z) / 2 is t e^(-z^2) 2^P(t) with t = 1 / (1 + 0.55 z) and P a
-// polynomial of the ninth degree, fitted for the least largest error over z up to 9.6, behind which fp32 holds nothing
-// (2^-23 in log2; with fp32's roundings 8 + 2 v^2 half steps).  erfcf took 22 us of the 8192 x 2560 outputs of a call of
-// 119, this 4.
+// polynomial of the ninth degree, fitted for the least largest error over z up to 9.6 (2^-23 in log2; with fp32's roundings
+// 8 + 2 v^2 half steps, on to z of 10.1, behind which fp32 holds nothing).  The power of two comes as its root on either
+// factor, since the hardware flushes subnormal ones, from |v| of 13 on.  erfcf took 22 us of the 8192 x 2560 outputs of a
+// call of 119, this 4.
 __device__ __forceinline__ float gelu32(float v) {
   const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(v), 0x1.8e3e18p-2f, 1.0f));
-  constexpr float kP[10] = {-0x1.581160p+1f, 0x1.6ffd0ap+0f,  0x1.1d3eb2p-1f,  -0x1.0b859cp-2f, 0x1.a717ccp-1f,
-                            -0x1.3176e0p+1f, 0x1.304d2cp+1f, -0x1.f55f98p-1f, 0x1.5652f8p-4f,  0x1.0f3ca0p-5f};
+  constexpr float kP[10] = {-0x1.581160p+0f, 0x1.6ffd0ap-1f,  0x1.1d3eb2p-2f,  -0x1.0b859cp-3f, 0x1.a717ccp-2f,   // P / 2
+                            -0x1.3176e0p+0f, 0x1.304d2cp+0f, -0x1.f55f98p-2f, 0x1.5652f8p-5f,  0x1.0f3ca0p-6f};
   float e = kP[9];
 #pragma unroll
   for (int i = 8; i >= 0; --i) e = fmaf(e, t, kP[i]);
-  const float q = t * __builtin_amdgcn_exp2f(fmaf(v * v, -0x1.715476p-1f, e));
-  return v * (v < 0.0f ? q : 1.0f - q);
+  const float root = __builtin_amdgcn_exp2f(fmaf(v * v, -0x1.715476p-2f, e)), q = t * root;
+  return v < 0.0f ? v * q * root : v * fmaf(-q, root, 1.0f);
 }
 
 // v or 1 times 1 / (1 + e^-u): silu, sigmoid (u = v) and, since (1 + tanh t) / 2 is the sigmoid of 2 t, gelu_tanh, whose
-// u = v (a + b v^2) alone takes the square, which overflows from 2^64 on: times a b of zero it would be no number.
+// u = v (a + b v^2) alone takes the square, which overflows from 2^64 on: times a b of zero it would be no number.  A
+// negative u's exponential comes as its root on either factor, as swiglu's, so that results keep their bits down to fp32's
+// least: off by 16 + 2 |u| half steps at most, gelu_tanh by the five more of u's own roundings, |u| times.
 struct SigmoidForm {
   bool cubic, times;
   __device__ __forceinline__ explicit SigmoidForm(uint32_t activation)
       : cubic(activation == kActGeluTanh), times(activation != kActSigmoid) {}
   __device__ __forceinline__ float operator()(float v) const {
-    const float s = sigmoid32(cubic ? v * fmaf(v * v, 0x1.2444f2p-4f, 0x1.988454p+0f) : v);
-    return times ? v * s : s;
+    const float u = cubic ? v * fmaf(v * v, 0x1.2444f2p-4f, 0x1.988454p+0f) : v;
+    const float root = __builtin_amdgcn_exp2f(fabsf(u) * -0x1.715476p-1f);   // e^(-|u| / 2)
+    const float r = __builtin_amdgcn_rcpf(fmaf(root, root, 1.0f));
+    const float w = u < 0.0f ? root : 1.0f;
+    return (times ? v * w : w) * r * w;
   }
 };
 
