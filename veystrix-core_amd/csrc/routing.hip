@@ -97,13 +97,22 @@ __device__ __forceinline__ bool group_kept(const RouteLaunch& p, uint32_t group,
   return better < p.top_groups;
 }
 
+// v to bf16 in one rounding: where fp32 holds the middle of two bf16 values (the last 16 bits 0x8000) and v lies beside it,
+// one step towards v.
+__device__ __forceinline__ uint32_t f64_to_bf16(double v) {
+  float f = static_cast<float>(v);
+  const uint32_t bits = __float_as_uint(f);
+  const double rest = v - static_cast<double>(f);
+  if ((bits & 0xffffu) == 0x8000u && rest != 0.0) f = __uint_as_float((rest > 0.0) == (f > 0.0f) ? bits + 1 : bits - 1);
+  return f32_to_bf16(f);
+}
+
 // Writes slot `slot` of a row; expert ~0: none.
 __device__ __forceinline__ void write_slot(const RouteLaunch& p, uint32_t row, uint32_t slot, uint32_t expert, double weight) {
   const uint64_t at = static_cast<uint64_t>(row) * p.top_k + slot;
   p.inds[at] = static_cast<int32_t>(expert);
-  const float w = static_cast<float>(weight);
-  if (p.weights_dtype == 0) static_cast<uint16_t*>(p.weights)[at] = static_cast<uint16_t>(f32_to_bf16(w));
-  else static_cast<float*>(p.weights)[at] = w;
+  if (p.weights_dtype == 0) static_cast<uint16_t*>(p.weights)[at] = static_cast<uint16_t>(f64_to_bf16(weight));
+  else static_cast<float*>(p.weights)[at] = static_cast<float>(weight);
 }
 
 // score * factor / total of the chosen; scores that are all too small for 64 bits weigh nothing.
