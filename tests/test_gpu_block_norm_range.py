@@ -37,3 +37,15 @@ def test_a_rows_factor_past_fp32(device, rows, width, size, scale):
     _check(x, r, post_weight=w, gate=gate * 1e-20, scale=1e-15, eps=eps)
     if size > 1e30:
         _check(x, r, scale=1e-30, gate=gate * 1e-10)     # no norm: scale times gate
+
+
+@pytest.mark.parametrize("rows,width", [(3, 128), (5, 333), (1100, 96)])
+@pytest.mark.parametrize("size", [1e38, 4e37, 1e-36, 2.0 ** -135])
+def test_a_second_norm_past_fp32(device, rows, width, size):
+    """Rows whose second norm's factor is subnormal or overflows fp32."""
+    gen = torch.Generator().manual_seed(rows)
+    r = (torch.randn((rows, width), generator=gen).clamp(-3, 3) * size).to(device)
+    w = (1 + 0.2 * torch.randn(width, generator=gen)).to(device)
+    x = torch.zeros_like(r)
+    _check(x, r, w, eps=0.0)
+    _check(x.bfloat16(), r, w, eps=0.0)

@@ -185,16 +185,17 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
     for (int j = 0; j < 8; ++j) ss = fma(static_cast<double>(h[i][j]), static_cast<double>(h[i][j]), ss);
   }
   if (p.weight == nullptr) return;
-  const Real pre = static_cast<Real>(1.0 / sqrt(row_total<TPR>(ss, s_part[1]) / width + p.eps));
+  const RowFactor<Real> of_h(1.0 / sqrt(row_total<TPR>(ss, s_part[1]) / width + p.eps));
   void* out = const_cast<void*>(row_at(p.out, row, p.out_stride, p.act_dtype));
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float w[8], y[8];
     load_run<8>(p.weight, p.weight_dtype, at(i), p.width, w);
     uint32_t border = ~0u;
+    of_h.times(h[i], h[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      h[i][j] = h[i][j] * pre * (one + static_cast<Real>(w[j]));
+      h[i][j] *= one + static_cast<Real>(w[j]);
       y[j] = static_cast<float>(h[i][j]);
       border = min(border, __float_as_uint(y[j]) & kBorderBits);
     }
