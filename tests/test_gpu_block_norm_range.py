@@ -1,4 +1,4 @@
-"""block_norm of rows whose factors lie at the ends of fp32 or past them while the results do not."""
+"""block_norm of rows, scales and gates whose factors lie at the ends of fp32 or past them while the results do not."""
 import pytest
 import torch
 
@@ -49,3 +49,15 @@ def test_a_second_norm_past_fp32(device, rows, width, size):
     x = torch.zeros_like(r)
     _check(x, r, w, eps=0.0)
     _check(x.bfloat16(), r, w, eps=0.0)
+
+
+@pytest.mark.parametrize("kind", ["channel", "value"])
+def test_sigmoid_gates_down_to_the_least(device, kind):
+    """Gates whose sigmoid is subnormal: themselves within half a step of those (2^-150) and the sigmoid's own error."""
+    rows, width = 4, 256
+    g = -torch.linspace(80.0, 104.0, width)
+    g = (g if kind == "channel" else g.expand(rows, width).contiguous()).to(device)
+    x = torch.full((rows, width), 2.0 ** 60, device=device)
+    h = block_norm(x, torch.zeros_like(x), gate=g, sigmoid_gate=True)
+    s = torch.sigmoid(g.cpu().double()).expand(rows, width)
+    assert_within(h, s * 2.0 ** 60, (s * 8 * 2.0 ** -24 + 2.0 ** -149) * 2.0 ** 60, kind)

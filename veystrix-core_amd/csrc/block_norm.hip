@@ -80,10 +80,12 @@ struct RowFactor {
   }
 };
 
+// 1 / (1 + e^-g); in fp32 from the exponential of -|g|, which does not overflow where the sigmoid is still a number.
 template <class Real>
 __device__ __forceinline__ Real gate_sigmoid(float g) {
   if constexpr (sizeof(Real) == 8) return 1.0 / (1.0 + exp(-static_cast<double>(g)));
-  else return 1.0f / (1.0f + expf(-g));
+  const float e = expf(-fabsf(g));
+  return (g < 0.0f ? e : 1.0f) / (1.0f + e);
 }
 
 // Eight values of a row as they lie in memory, so that a row waits for its sums in half of fp32's registers.
