@@ -234,15 +234,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(LinearLaunch p) {
 
 // ---------------------------------------------------------------- tiles ---
 
-template <bool MX>
-__device__ __forceinline__ f32x4_t unit_product(const Operand<MX>& w, const Operand<MX>& x, f32x4_t acc) {
-#pragma unroll
-  for (int i = 0; i < (MX ? 2 : 1); ++i)
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w.part[i]),
-                                                  __builtin_bit_cast(bf16x8_t, x.part[i]), acc, 0, 0, 0);
-  return acc;
-}
-
 // Tile (row tile, column tile) of a block: every XCD (blocks b, b + 8, ..) takes a run of tiles, and runs go down columns
 // of up to eight row tiles, so that the tiles of one L2 share rows and matrix rows (2048 rows 2048 -> 512 in 32 x 64 tiles
 // 11.3 us, row after row 13.1).
@@ -373,7 +364,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void k_linear(LinearLaunch p) {
         const Operand<MX> w(wv[f], scale(MX ? ws[f] : 0u, h));
 #pragma unroll
         for (int i = 0; i < RF; ++i)
-          acc[i][f] = unit_product<MX>(w, Operand<MX>(xv[i], scale(MX ? xs[i] : 0u, h)), acc[i][f]);
+          acc[i][f] = unit_mfma<MX>(w, Operand<MX>(xv[i], scale(MX ? xs[i] : 0u, h)), acc[i][f]);
       }
     }
   };
@@ -580,7 +571,7 @@ __global__ __launch_bounds__(512, 2) void k_large(LinearLaunch p) {
     for (int f = 0; f < CF; ++f) {
       const Operand<MX> w(wv[f], ws[f]);
 #pragma unroll
-      for (int i = 0; i < RF; ++i) acc[i][f] = unit_product<MX>(w, Operand<MX>(xv[i], xs[i]), acc[i][f]);
+      for (int i = 0; i < RF; ++i) acc[i][f] = unit_mfma<MX>(w, Operand<MX>(xv[i], xs[i]), acc[i][f]);
     }
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
