@@ -19,6 +19,7 @@
 
 #include "../../include/veymoe.h"
 #include "vm_internal.h"
+#include "vm_linear_form.h"
 
 namespace {
 
@@ -1861,20 +1862,7 @@ int vm_linear(const VmLinearArgs* a, void* stream) {
       !rows_aligned(a->weight, w_rows > 1 ? a->weight_stride * size : 0, 16))
     return fail(VM_EINVAL, "rows of x and weight must be 16-byte aligned");
   if (rows > 1 && a->out_stride < a->n) return fail(VM_EINVAL, "the row stride of out must be at least n");
-  if (vm::linear_blocks(a->rows, a->n) > kMaxBlocks)
-    return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
   const uint64_t out_size = a->out_dtype == VM_F32 ? 4 : 2, res_size = a->residual_dtype == VM_F32 ? 4 : 2;
-  const RowBytes out{a->out, rows, a->out_stride * out_size, a->n * out_size};
-  const RowBytes res{a->residual, rows, a->residual_stride * res_size, a->n * res_size};
-  const RowBytes ins[] = {{a->x, rows, a->x_stride * size, uint64_t(a->k) * size},
-                          {a->weight, w_rows, a->weight_stride * size, uint64_t(a->k) * size},
-                          {mx ? a->x_scales : nullptr, rows, a->x_scale_stride, a->k / VM_MX_GROUP},
-                          {mx ? a->weight_scales : nullptr, w_rows, a->weight_scale_stride, a->k / VM_MX_GROUP},
-                          {a->bias, 1, 0, w_rows * (a->bias_dtype == VM_F32 ? 4 : 2)}};
-  for (const RowBytes& in : ins)
-    if (!rows_apart(out, in)) return fail(VM_EINVAL, "out overlaps an operand");
-  if (!(same_rows(out, res) && out_size == res_size) && !rows_apart(out, res))
-    return fail(VM_EINVAL, "out overlaps residual other than row for row");
   vm::LinearLaunch p{};
   p.x = static_cast<const uint8_t*>(a->x);
   p.x_scales = a->x_scales;
@@ -1887,8 +1875,8 @@ int vm_linear(const VmLinearArgs* a, void* stream) {
   p.x_scale_stride = a->x_scale_stride;
   p.w_stride = a->weight_stride * size;
   p.w_scale_stride = a->weight_scale_stride;
-  p.residual_stride = res.stride;
-  p.out_stride = out.stride;
+  p.residual_stride = a->residual_stride * res_size;
+  p.out_stride = a->out_stride * out_size;
   p.rows = a->rows;
   p.k_bytes = a->k * size;
   p.n = a->n;
@@ -1899,7 +1887,20 @@ int vm_linear(const VmLinearArgs* a, void* stream) {
   p.mx = mx;
   p.whole_scales = mx && a->k / VM_MX_GROUP % 4 == 0 && rows_aligned(a->x_scales, rows > 1 ? a->x_scale_stride : 0, 4) &&
                    rows_aligned(a->weight_scales, w_rows > 1 ? a->weight_scale_stride : 0, 4);
-  const hipError_t e = vm::launch_linear(p, static_cast<hipStream_t>(stream));
+  const vm::LinearForm form = vm::linear_form(p);
+  if (!form.fits()) return fail(VM_EUNSUPPORTED, "a call of %u rows by %u outputs is too large", a->rows, a->n);
+  const RowBytes out{a->out, rows, p.out_stride, a->n * out_size};
+  const RowBytes res{a->residual, rows, p.residual_stride, a->n * res_size};
+  const RowBytes ins[] = {{a->x, rows, a->x_stride * size, uint64_t(a->k) * size},
+                          {a->weight, w_rows, a->weight_stride * size, uint64_t(a->k) * size},
+                          {mx ? a->x_scales : nullptr, rows, a->x_scale_stride, a->k / VM_MX_GROUP},
+                          {mx ? a->weight_scales : nullptr, w_rows, a->weight_scale_stride, a->k / VM_MX_GROUP},
+                          {a->bias, 1, 0, w_rows * (a->bias_dtype == VM_F32 ? 4 : 2)}};
+  for (const RowBytes& in : ins)
+    if (!rows_apart(out, in)) return fail(VM_EINVAL, "out overlaps an operand");
+  if (!(same_rows(out, res) && out_size == res_size) && !rows_apart(out, res))
+    return fail(VM_EINVAL, "out overlaps residual other than row for row");
+  const hipError_t e = vm::launch_linear(p, form, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "linear launch");
   return VM_OK;
 }

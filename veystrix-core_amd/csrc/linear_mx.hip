@@ -4,6 +4,8 @@
 
 namespace vm {
 
-hipError_t launch_linear_mx(const LinearLaunch& p, hipStream_t stream) { return linear_go<true>(p, stream); }
+hipError_t launch_linear_mx(const LinearLaunch& p, const LinearForm& form, hipStream_t stream) {
+  return linear_go<true>(form, p, stream);
+}
 
 }  // namespace vm

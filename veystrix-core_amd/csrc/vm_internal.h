@@ -568,9 +568,9 @@ struct LinearLaunch {
   bool mx;
   bool whole_scales;           // every row of scales starts at a multiple of four bytes and has whole words
 };
-// An upper bound of a call's blocks.
-uint64_t linear_blocks(uint32_t rows, uint32_t n);
-hipError_t launch_linear(const LinearLaunch& p, hipStream_t stream);
+struct LinearForm;               // vm_linear_form.h
+LinearForm linear_form(const LinearLaunch& p);
+hipError_t launch_linear(const LinearLaunch& p, const LinearForm& form, hipStream_t stream);
 
 // --------------------------------------------------------------- routing --
 // From logits to experts (routing.hip).

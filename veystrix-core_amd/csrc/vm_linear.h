@@ -6,7 +6,7 @@
 // Both formats move as runs of a row (64 or 128 bytes: 16-byte units of 8 bf16 or 16 e4m3 inputs), staged in LDS by DMA
 // (vm_dma.h); an MX unit is converted to two bf16 operands in registers (vm_operand.h), so both formats have the bf16
 // unit's sums.  The matrix is the first operand, the rows the second, so a lane receives four neighbouring outputs of row
-// lane % 16.  Four kinds of calls, chosen by choose_form below:
+// lane % 16.  Four kinds of calls, chosen by choose_form (vm_linear_form.h):
 //   k_few     up to four rows: the matrix read once by plain loads, no MFMA; bound by its bytes (one row 2560 -> 2560, 13 MB,
 //             4.5 us, of which a launch is two).
 //   k_linear  small tiles, whose waves share the inputs where there are few tiles, so that a call of few rows is done in
@@ -25,6 +25,7 @@
 #include "vm_any.h"
 #include "vm_dma.h"
 #include "vm_internal.h"
+#include "vm_linear_form.h"
 #include "vm_mx.h"
 #include "vm_operand.h"
 
@@ -132,9 +133,6 @@ __device__ __forceinline__ void finish8(const LinearLaunch& p, uint32_t row, uin
 }
 
 // ------------------------------------------------------------- few rows ---
-
-constexpr int kFewMatrix = 4;             // matrix rows of a block
-constexpr uint32_t kFewWaves = 8;         // at most, each over every so manyth kilobyte of the rows
 
 // The sum of one output through the epilogue.
 __device__ __forceinline__ void finish1(const LinearLaunch& p, uint32_t row, uint32_t col, float v, float up) {
@@ -680,138 +678,67 @@ __global__ __launch_bounds__(512, 2) void k_large(LinearLaunch p) {
 }
 
 template <class Kernel>
-hipError_t go(Kernel kernel, uint64_t blocks, uint32_t threads, const LinearLaunch& p, hipStream_t stream) {
-  if (blocks * threads >> 32) return hipErrorInvalidValue;   // a grid's threads are counted in 32 bits
+hipError_t go(Kernel kernel, const LinearForm& c, const LinearLaunch& p, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(c.blocks)), block(c.threads);
   hipEvent_t start = nullptr, stop = nullptr;
   if (timing_events("linear", &start, &stop))
-    hipExtLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(threads), 0, stream, start, stop, 0, p);
+    hipExtLaunchKernelGGL(kernel, grid, block, 0, stream, start, stop, 0, p);
   else
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(threads), 0, stream, p);
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, p);
   return hipGetLastError();
 }
 
-template <bool MX, int RF, int CF, int WM, int WN, int WK, int S>
-hipError_t tiles_go(const LinearLaunch& p, hipStream_t stream) {
-  const uint32_t rows = 16 * RF * WM, cols = 16 * CF * WN / (p.activation == kActSwiglu ? 2 : 1);
-  const uint64_t blocks = uint64_t((p.rows + rows - 1) / rows) * ((p.n + cols - 1) / cols);
-  return go(&k_linear<MX, RF, CF, WM, WN, WK, S>, blocks, 64 * WM * WN * WK, p, stream);
+// Whether the form's row in the table is an instance's tile and threads.
+template <bool MX, int FORM, int RF, int CF, int WM, int WN, int WK>
+constexpr bool is_form() {
+  constexpr TileForm t = kTileForms<MX>[FORM];
+  return t.rows == 16 * RF * WM && t.matrix == 16 * CF * WN && t.threads == 64 * WM * WN * WK;
 }
 
-template <bool MX, int RF, int CF, int WM, int WN>
-hipError_t large_go(const LinearLaunch& p, hipStream_t stream) {
-  const uint32_t rows = 16 * RF * WM, cols = 16 * CF * WN / (p.activation == kActSwiglu ? 2 : 1);
-  const uint64_t blocks = uint64_t((p.rows + rows - 1) / rows) * ((p.n + cols - 1) / cols);
+template <bool MX, int FORM, int RF, int CF, int WM, int WN, int WK, int S>
+hipError_t tiles_go(const LinearForm& c, const LinearLaunch& p, hipStream_t stream) {
+  static_assert(is_form<MX, FORM, RF, CF, WM, WN, WK>(), "the grid is the form's");
+  return go(&k_linear<MX, RF, CF, WM, WN, WK, S>, c, p, stream);
+}
+
+template <bool MX, int FORM, int RF, int CF, int WM, int WN>
+hipError_t large_go(const LinearForm& c, const LinearLaunch& p, hipStream_t stream) {
+  static_assert(is_form<MX, FORM, RF, CF, WM, WN, 1>(), "the grid is the form's");
   switch (p.activation) {
-    case kActSwiglu: return go(&k_large<MX, kEpiSwiglu, RF, CF, WM, WN>, blocks, 512, p, stream);
-    case kActGelu: return go(&k_large<MX, kEpiGelu, RF, CF, WM, WN>, blocks, 512, p, stream);
+    case kActSwiglu: return go(&k_large<MX, kEpiSwiglu, RF, CF, WM, WN>, c, p, stream);
+    case kActGelu: return go(&k_large<MX, kEpiGelu, RF, CF, WM, WN>, c, p, stream);
     case kActNone:
-    case kActRelu: return go(&k_large<MX, kEpiPlain, RF, CF, WM, WN>, blocks, 512, p, stream);
-    default: return go(&k_large<MX, kEpiSigmoid, RF, CF, WM, WN>, blocks, 512, p, stream);
+    case kActRelu: return go(&k_large<MX, kEpiPlain, RF, CF, WM, WN>, c, p, stream);
+    default: return go(&k_large<MX, kEpiSigmoid, RF, CF, WM, WN>, c, p, stream);
   }
 }
 
-// Whether the rows of a tile lie within 32 bits of its first, the up rows of SwiGLU included.
-bool near_rows(const LinearLaunch& p) {
-  const uint64_t rows = 512, up = p.activation == kActSwiglu ? p.n : 0;
-  return (rows + up) * p.w_stride + p.k_bytes < (1ull << 32) && rows * p.x_stride + p.k_bytes < (1ull << 32);
-}
-
-template <bool MX, int R>
-hipError_t few_go(const LinearLaunch& p, hipStream_t stream) {
-  const uint32_t cols = p.activation == kActSwiglu ? kFewMatrix / 2 : kFewMatrix;
-  const uint32_t waves = min(kFewWaves, (p.k_bytes + 1023) / 1024);
-  return go(&k_few<MX, R>, (p.n + cols - 1) / cols, 64 * waves, p, stream);
-}
-
-// Tiles of a form: their rows and matrix rows, how many of them a CU holds at once, and the us in which it computes one
-// alone and all that it holds: a fixed part and one per 32 inputs.  Fitted to calls of 512 to 2560 inputs and one to six
-// rounds of tiles in either format (an MX step of 64 inputs takes about what two of bf16 take); within 20 % of most.
-struct TileForm {
-  uint32_t rows, matrix, places;
-  float one, one_step, full, full_step;
-};
-enum : int { kForm16, kForm32, kForm32x64, kForm64, kForm64Deep, kForm128, kForm128x320, kForm256, kForm256x320, kForms };
-constexpr uint32_t kCus = 256;
 template <bool MX>
-constexpr TileForm kTileForms[kForms] = {
-    {16, 16, 2, 2.5f, 0.045f, 2.5f, 0.060f},        // 8 waves, each every eighth chunk
-    {32, 32, 2, 3.5f, 0.058f, 4.0f, 0.090f},        // 16 waves, each every fourth
-    {32, 64, 2, 3.5f, 0.080f, 5.0f, 0.100f},        // 8 waves, each every other
-    {64, 64, 3, 6.0f, 0.100f, 8.0f, 0.220f},        // 4 waves
-    {64, 64, 1, 5.5f, 0.075f, 5.5f, 0.075f},        // 8 waves, each every other chunk
-    {128, 128, 2, 5.9f, 0.277f, 9.0f, 0.500f},      // the large tiles of two groups of waves
-    {128, 320, 1, 14.0f, 0.450f, 14.0f, 0.450f},
-    {256, 256, 1, 12.0f, 0.580f, 12.0f, 0.580f},
-    {256, 320, 1, 18.0f, 0.820f, 18.0f, 0.820f},
-};
-template <>
-constexpr TileForm kTileForms<true>[kForms] = {
-    {16, 16, 2, 2.5f, 0.042f, 2.5f, 0.050f},
-    {32, 32, 2, 3.5f, 0.058f, 4.0f, 0.080f},
-    {32, 64, 3, 3.8f, 0.085f, 6.0f, 0.165f},
-    {64, 64, 3, 5.0f, 0.137f, 8.0f, 0.235f},
-    {64, 64, 0, 0.0f, 0.000f, 0.0f, 0.000f},        // no faster than 32 x 64: not built
-    {128, 128, 2, 5.9f, 0.240f, 9.0f, 0.400f},
-    {128, 320, 1, 14.0f, 0.450f, 14.0f, 0.450f},
-};
-// Rows up to which a block reads its matrix rows once for all of them, without MFMA: eight rows 7.6 us by 2560 x 2560,
-// in 16 x 16 tiles 6.8; four 5.8.
-constexpr uint32_t kFewRows = 4;
-
-// The form of the least time by the model, and whether no CU holds two of its tiles.
-struct Choice {
-  int form;
-  bool alone;
-};
-template <bool MX>
-Choice choose_form(const LinearLaunch& p) {
-  const uint32_t matrix = p.activation == kActSwiglu ? 2 * p.n : p.n;
-  const float steps = static_cast<float>(p.k_bytes) / (MX ? 32.0f : 64.0f);
-  // the large tiles take scales by the word and row offsets of 32 bits; of MX 256 x 320 would outgrow the LDS, and 256 x 256
-  // is slower than 128 x 320 (a full round of the chip 62 us for 52, of a fifth fewer products)
-  const int forms = near_rows(p) && (!MX || p.whole_scales) ? (MX ? kForm256 : kForms) : kForm128;
-  Choice best{kForm16, false};
-  float least = __builtin_huge_valf();
-  for (int f = 0; f < forms; ++f) {
-    const TileForm& t = kTileForms<MX>[f];
-    if (t.places == 0) continue;
-    const uint64_t tiles = uint64_t((p.rows + t.rows - 1) / t.rows) * ((matrix + t.matrix - 1) / t.matrix);
-    const uint64_t left = tiles % (t.places * kCus), held = (left + kCus - 1) / kCus;   // by a CU, of the last round
-    const float one = t.one + t.one_step * steps, full = t.full + t.full_step * steps;
-    float us = static_cast<float>(tiles / (t.places * kCus)) * full;
-    if (held > 0) us += t.places == 1 ? full : one + (full - one) * static_cast<float>(held - 1) / static_cast<float>(t.places - 1);
-    if (us < least) {
-      least = us;
-      best = {f, tiles <= kCus};
-    }
-  }
-  return best;
-}
-
-template <bool MX>
-hipError_t linear_go(const LinearLaunch& p, hipStream_t stream) {
-  if (p.rows <= kFewRows) {
-    if (p.rows == 1) return few_go<MX, 1>(p, stream);
-    if (p.rows == 2) return few_go<MX, 2>(p, stream);
-    return few_go<MX, 4>(p, stream);
-  }
+hipError_t linear_go(const LinearForm& c, const LinearLaunch& p, hipStream_t stream) {
   // More stages than two keep more loads on their way where a CU's LDS would hold no other tile anyway: 64 rows by
   // 2560 x 2560 9.9 to 8.1 us in 32 x 32 tiles with four, 128 rows 14.0 to 9.8 in 32 x 64 with three, 2048 rows 49 to 43 in
   // 64 x 64 with three.  Of MX the scales' registers wait for the loads between: two are the fastest everywhere.
-  constexpr int kDeep = MX ? 2 : 3;
-  const Choice c = choose_form<MX>(p);
+  constexpr int kDeep = MX ? 2 : 3, kDeepest = MX ? 2 : 4;
   switch (c.form) {
-    case kForm16: return c.alone ? tiles_go<MX, 1, 1, 1, 1, 8, kDeep>(p, stream) : tiles_go<MX, 1, 1, 1, 1, 8, 2>(p, stream);
-    case kForm32: return c.alone ? tiles_go<MX, 1, 1, 2, 2, 4, MX ? 2 : 4>(p, stream) : tiles_go<MX, 1, 1, 2, 2, 4, 2>(p, stream);
-    case kForm32x64: return tiles_go<MX, 1, 2, 2, 2, 2, kDeep>(p, stream);
-    case kForm64: return tiles_go<MX, 2, 2, 2, 2, 1, kDeep>(p, stream);
-    case kForm128: return large_go<MX, 2, 4, 4, 2>(p, stream);
-    case kForm128x320: return large_go<MX, 2, 10, 4, 2>(p, stream);
+    case kFormFew:
+      if (p.rows == 1) return go(&k_few<MX, 1>, c, p, stream);
+      if (p.rows == 2) return go(&k_few<MX, 2>, c, p, stream);
+      return go(&k_few<MX, 4>, c, p, stream);
+    case kForm16:
+      return c.alone ? tiles_go<MX, kForm16, 1, 1, 1, 1, 8, kDeep>(c, p, stream) : tiles_go<MX, kForm16, 1, 1, 1, 1, 8, 2>(c, p, stream);
+    case kForm32:
+      return c.alone ? tiles_go<MX, kForm32, 1, 1, 2, 2, 4, kDeepest>(c, p, stream) : tiles_go<MX, kForm32, 1, 1, 2, 2, 4, 2>(c, p, stream);
+    case kForm32x64: return tiles_go<MX, kForm32x64, 1, 2, 2, 2, 2, kDeep>(c, p, stream);
+    case kForm64: return tiles_go<MX, kForm64, 2, 2, 2, 2, 1, kDeep>(c, p, stream);
+    case kForm128: return large_go<MX, kForm128, 2, 4, 4, 2>(c, p, stream);
+    case kForm128x320: return large_go<MX, kForm128x320, 2, 10, 4, 2>(c, p, stream);
     default: break;
   }
-  if constexpr (!MX)
-    if (c.form == kForm64Deep) return tiles_go<MX, 2, 2, 2, 2, 2, kDeep>(p, stream);
-  if constexpr (!MX) return c.form == kForm256 ? large_go<MX, 4, 8, 4, 2>(p, stream) : large_go<MX, 4, 10, 4, 2>(p, stream);
+  if constexpr (!MX) {
+    if (c.form == kForm64Deep) return tiles_go<MX, kForm64Deep, 2, 2, 2, 2, 2, kDeep>(c, p, stream);
+    if (c.form == kForm256) return large_go<MX, kForm256, 4, 8, 4, 2>(c, p, stream);
+    return large_go<MX, kForm256x320, 4, 10, 4, 2>(c, p, stream);
+  }
   return hipErrorInvalidValue;
 }
 
