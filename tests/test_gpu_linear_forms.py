@@ -112,3 +112,15 @@ def test_not_numbers_stay_where_they_are(device, form, activation):
     got = linear(_operand(x, mx), _operand(w, mx), b, activation=activation, residual=r, dtype=FP32)
     assert torch.equal(torch.isnan(got), bad)
     assert torch.isfinite(got[~bad]).all()
+
+
+@pytest.mark.parametrize("rows,k,n,activation", [(8192, 40, 2570, None), (7937, 1000, 2559, "silu"), (8191, 72, 1285, "swiglu"),
+                                                 (6001, 2080, 2051, None)])
+def test_large_tiles_of_ragged_sizes_are_numbers(device, rows, k, n, activation):
+    """Every output is a number, which a comparison alone does not show: a difference from NaN is above no bound."""
+    gen = torch.Generator(device=device).manual_seed(rows)
+    make = lambda *shape: torch.randn(shape, generator=gen, device=device).bfloat16()  # noqa: E731
+    x, w = _wide(make(rows, k), 64, 0xff), _wide(make(n * (2 if activation == "swiglu" else 1), k), 64, 0xff)
+    for dtype in (BF16, FP32):
+        for residual in (None, make(rows, n), make(rows, n).float()):
+            assert torch.isfinite(linear(x, w, activation=activation, residual=residual, dtype=dtype)).all()
