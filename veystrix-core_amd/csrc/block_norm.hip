@@ -115,6 +115,25 @@ struct RawRun {
   }
 };
 
+// v as the float that is rounded to e4m3.
+__device__ __forceinline__ float towards(double v) {
+  const float f = static_cast<float>(v);
+  const double rest = v - static_cast<double>(f);
+  return off_border(f, rest > 0.0 ? 1.0f : rest < 0.0 ? -1.0f : 0.0f);
+}
+
+// Magnitude bits of the largest of the 32 values that four neighbouring lanes hold.
+__device__ __forceinline__ uint32_t group_magnitude(const float y[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(y[j]));
+  m = max(m, dpp_u<kDppQuadXor1>(m));
+  return max(m, dpp_u<kDppQuadXor2>(m));
+}
+
+// 2^-80 (off_border knows floats from 2^-101 on, and e4m3 reaches from a group's largest value 2^18 down), zero left out.
+constexpr uint32_t kSmallGroup = 0x17800000u - 1u;
+
 // Rows of A and residuals of R; TPR threads per row (64 or 256), up to NV steps of eight values per thread.
 template <class A, class R, int TPR, int NV, bool MXOUT>
 __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunch p) {
@@ -206,22 +225,21 @@ __global__ __launch_bounds__(kBlockNormThreads) void k_block_norm(BlockNormLaunc
     } else {
       if (border == 0) {  // seldom: one of them may lie on a border
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const double rest = h[i][j] - static_cast<double>(y[j]);
-          y[j] = off_border(y[j], rest > 0.0 ? 1.0f : rest < 0.0 ? -1.0f : 0.0f);
-        }
+        for (int j = 0; j < 8; ++j) y[j] = towards(h[i][j]);
       }
-      uint32_t m = 0;
+      uint32_t m = group_magnitude(y), e = mx_scale(m), up = 0;
+      // Groups whose values may lie where fp32's are not whole or not told from borders: 2^100 times theirs, once more.
+      if (m - 1u < kSmallGroup) {
+        up = 100;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, mx_magnitude(y[j]));
-      m = max(m, dpp_u<kDppQuadXor1>(m));
-      m = max(m, dpp_u<kDppQuadXor2>(m));
-      const uint32_t e = mx_scale(m);
+        for (int j = 0; j < 8; ++j) y[j] = towards(__builtin_amdgcn_ldexp(h[i][j], 100));
+        e = max(mx_scale(group_magnitude(y)), up);   // scales end at 2^-127
+      }
       if (at(i) < p.width) {  // the width is whole groups, so a lane's eight values are all in it
         const uint64_t first = static_cast<uint64_t>(row) * p.width + at(i);
         *reinterpret_cast<uint2*>(p.values + first) =
             make_uint2(mx_pack4(y[0], y[1], y[2], y[3], e), mx_pack4(y[4], y[5], y[6], y[7], e));
-        if (t % 4 == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e);
+        if (t % 4 == 0) p.scales[first / kMxGroup] = static_cast<uint8_t>(e - up);
       }
     }
   }
