@@ -393,10 +393,11 @@ typedef struct VmNormArgs {
  * `out` [rows, width] in act_dtype or to MX rows `values` and `scales` as of
  * vm_rms_norm (width a multiple of 32, values 8-byte aligned).  Sums of squares
  * are 64 bits, the rest fp32; to MX everything is 64 bits, so that e4m3's is
- * the values' one rounding.  The second norm reads the unrounded h.  out and
- * sum_out may each be x or residual, row for row, where their types are of one
- * size; outputs overlap nothing otherwise, each other included.  Strides count
- * elements between rows.  width up to VM_NORM_MAX_WIDTH.  No counterpart in the
+ * the values' one rounding (past fp32's range they are infinite, and their
+ * group NaN).  The second norm reads the unrounded h.  out and sum_out may each
+ * be x or residual, row for row, where their types are of one size; outputs
+ * overlap nothing otherwise, each other included.  Strides count elements
+ * between rows.  width up to VM_NORM_MAX_WIDTH.  No counterpart in the
  * reference. */
 #define VM_GATE_NONE 0u
 #define VM_GATE_ROW 1u
@@ -483,13 +484,17 @@ typedef struct VmAdapterArgs {
  * VM_ACTIVATION_SWIGLU: weight and bias have 2 n rows, gate then up, and the
  * activation is silu(gate) * up.  gelu is x Phi(x), gelu_tanh its tanh form.
  * x and weight are both bf16 or both MX; out and residual are bf16 or fp32, the
- * epilogue fp32 with one rounding at the end.  MX values enter as bf16: those
+ * epilogue fp32 with one rounding at the end.  Its exponentials and reciprocals
+ * are the hardware's: silu, swiglu and sigmoid are off by at most 16 + 2 |x|
+ * half steps of fp32, gelu by 12 + 4 x^2, gelu_tanh by 20 + 7 |u|, u its
+ * sigmoid's argument, down to fp32's least.  MX values enter as bf16: those
  * below 2^-126 are rounded to multiples of 2^-133, those of 2^128 and above are
  * infinite.  out may be residual, row for row, where their types are one, and
  * overlaps nothing otherwise.  k: a multiple of 8 (bf16) or 32 (MX); rows of x
- * and weight 16-byte aligned.  k and n up to 2^24, rows up to 2^28.  Strides
- * count elements (of an MX scale array: scales).  A call repeats itself bit for
- * bit.  No counterpart in the reference. */
+ * and weight 16-byte aligned.  k and n up to 2^24, rows up to 2^28, and no more
+ * tiles than a grid of 2^32 threads holds.  Strides count elements (of an MX
+ * scale array: scales).  A call repeats itself bit for bit.  No counterpart in
+ * the reference. */
 #define VM_ACTIVATION_RELU 2u
 #define VM_ACTIVATION_SILU 3u
 #define VM_ACTIVATION_GELU 4u

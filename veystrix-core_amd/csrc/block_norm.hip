@@ -8,13 +8,14 @@
 // second norm reads h as it was computed, before it is rounded to the residual's type.
 //
 // A row is read once: x and the residual stay in registers, as they lie in memory, until the first sum of squares is
-// known, then h until the second; eight consecutive values per thread and step, at any alignment (vm_any.h).  Squares are summed in 64 bits, which no value
-// overflows and which costs two operations a value.  Rows to MX are computed in 64 bits throughout, so that e4m3's is
-// their one rounding.
+// known, then h until the second; eight consecutive values per thread and step, at any alignment (vm_any.h).  Squares are
+// summed in 64 bits, which no value overflows and which costs two operations a value.  Rows to MX are computed in 64 bits
+// throughout, so that e4m3's is their one rounding.
 // Bound by HBM (two rows in, two out), or with few rows by one row's latency, which two sums over the row make up: 8192 rows
-// of 2560, bf16 32 us (168 MB, 5.3 TB/s), with an fp32 residual 41.5 (252 MB, 6.1), to MX 37.8 (147 MB, 3.9 TB/s; the 64-bit
-// operations, about 18 a value); one row 5.0.  A sigmoid of a gate per channel or value costs a 64-bit exponential each to
-// MX: 8192 rows of 2560 62 us.
+// of 2560, in a graph over three sets of operands, bf16 36 us (168 MB, 4.7 TB/s), with an fp32 residual 47.5 (252 MB, 5.3); one
+// row 5.2.  To MX 39.1 (147 MB, 3.8 TB/s): the vector units are busy half of that time (1582 instructions a row by counter,
+// bf16 rows 1140), and the 128 registers of a lane leave four waves a SIMD, which wait 45 % of theirs.  A sigmoid of a gate
+// per channel or value costs a 64-bit exponential each to MX: 65 and 68 us, in fp32 45.5 and 52.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>

@@ -14,10 +14,12 @@
 //
 // 64 bits for all experts would be most of the work (8192 rows of 512 with a sigmoid and a bias, top-10, 31 us).  So choices in
 // 32 bits find the candidates: the top_k-th largest of the lanes' largest choices, less what 32 bits may be off, is a bound
-// that every chosen expert passes and few others do; those, one to a lane, are compared in 64 bits (10.8 us; the logits alone
-// are 17 MB, 3.4 at a copy's rate; bound by a wave's instructions: 470 vector ones, of which the scores are a fourth).  Groups are
-// decided in 32 bits where kept and lost ones lie further apart than 32 bits may be off.  Rows that are not decided so
-// (masses of equal choices, groups that nearly tie) take the whole way in 64 bits.
+// that every chosen expert passes and few others do; those, one to a lane, are compared in 64 bits (12.1 us in a graph, traced
+// 12.4; the logits alone are 17 MB, 3.4 at a copy's rate; bound by a wave's instructions, 495 vector and 311 scalar ones by
+// counter, a good part of them over a dozen candidates in 64 lanes).  Groups are decided in 32 bits where kept and lost ones
+// lie further apart than 32 bits may be off (four of eight groups 16.1 us).  Softmax scores with a bias, or not
+// renormalised, take the row's sum in 64 bits, an exponential for every expert (16.6 and 14.2 us; without either 10.9).
+// Rows that are not decided so (masses of equal choices, groups that nearly tie) take the whole way in 64 bits.
 
 #include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
@@ -365,8 +367,8 @@ __device__ bool route_narrow(const RouteLaunch& p, uint32_t row, uint32_t lane, 
     const uint32_t more = least | (1u << bit);
     if (static_cast<uint32_t>(__builtin_popcountll(__ballot(best >= more))) >= p.top_k) least = more;
   }
-  // Where fewer lanes hold open experts, the bound of all choices (8192 rows of 512 in 8 groups, one kept, top-16: 17.7 us;
-  // with the top_k-th largest itself, a wave's maximum at a time, 19.4); still 0: every open expert.
+  // Where fewer lanes hold open experts, the bound of all choices (8192 rows of 512 in 8 groups, one kept, top-16, 21.5 us; the
+  // top_k-th largest itself, a wave's maximum at a time, takes a tenth more); still 0: every open expert.
   if (least == 0) {
 #pragma unroll
     for (int bit = 31; bit >= 14; --bit) {

@@ -6,14 +6,15 @@
 // Both formats move as runs of a row (64 or 128 bytes: 16-byte units of 8 bf16 or 16 e4m3 inputs), staged in LDS by DMA
 // (vm_dma.h); an MX unit is converted to two bf16 operands in registers (vm_operand.h), so both formats have the bf16
 // unit's sums.  The matrix is the first operand, the rows the second, so a lane receives four neighbouring outputs of row
-// lane % 16.  Four kinds of calls, chosen by choose_form (vm_linear_form.h):
+// lane % 16.  Three kinds of calls, chosen by choose_form (vm_linear_form.h):
 //   k_few     up to four rows: the matrix read once by plain loads, no MFMA; bound by its bytes (one row 2560 -> 2560, 13 MB,
-//             4.5 us, of which a launch is two).
+//             4.6 us, of which a launch is two; of MX 3.7; four rows 5.6).
 //   k_linear  small tiles, whose waves share the inputs where there are few tiles, so that a call of few rows is done in
-//             a few steps: bound by the loads' way from L2 and HBM (32 rows MX 2560 -> 2 x 640 5.5 us, 333 rows 1000 -> 1333
-//             7.4, 2048 rows 2048 -> 512 10.6: 134 MB past the L2s at 13 TB/s).
-//   k_large   large tiles: bound by the products (1100 to 1280 TFLOP/s of 2560 inputs, 1430 of 8192, a library's 8192^3
-//             product 1660) and, all tiles of a round ending together, by the outputs' way to HBM.
+//             a few steps: bound by the loads' way from L2 and HBM (32 rows MX 2560 -> 2 x 640 6.4 us, 64 rows 2560 -> 2560
+//             7.9, 333 rows 1000 -> 1333 7.8, 2048 rows 2048 -> 512 12.1: 134 MB past the L2s at 11 TB/s).
+//   k_large   large tiles: bound by the products (1240 TFLOP/s of 2560 inputs, 1330 of 8192, a library's 8192^3 product
+//             1610) and, all tiles of a round ending together, by the outputs' way to HBM.
+// Times are a kernel trace's medians.
 
 #pragma once
 
@@ -58,9 +59,9 @@ enum : int { kEpiPlain = 0, kEpiSigmoid = 1, kEpiGelu = 2, kEpiSwiglu = 3 };
 
 // v Phi(v).  For z = |v| / sqrt 2, Phi(-|v|) = erfc(z) / 2 is t e^(-z^2) 2^P(t) with t = 1 / (1 + 0.55 z) and P a
 // polynomial of the ninth degree, fitted for the least largest error over z up to 9.6 (2^-23 in log2; with fp32's roundings
-// 8 + 2 v^2 half steps, on to z of 10.1, behind which fp32 holds nothing).  The power of two comes as its root on either
-// factor, since the hardware flushes subnormal ones, from |v| of 13 on.  erfcf took 22 us of the 8192 x 2560 outputs of a
-// call of 119, this 4.
+// 8 + 2 v^2 half steps over eight million values, on to z of 10.1, behind which fp32 holds nothing).  The power of two comes
+// as its root on either factor, since the hardware flushes subnormal ones, from |v| of 13 on.  erfcf took 22 us of the
+// 8192 x 2560 outputs of a call of 119, this 9.
 __device__ __forceinline__ float gelu32(float v) {
   const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(v), 0x1.8e3e18p-2f, 1.0f));
   constexpr float kP[10] = {-0x1.581160p+0f, 0x1.6ffd0ap-1f,  0x1.1d3eb2p-2f,  -0x1.0b859cp-3f, 0x1.a717ccp-2f,   // P / 2
@@ -75,7 +76,7 @@ __device__ __forceinline__ float gelu32(float v) {
 // v or 1 times 1 / (1 + e^-u): silu, sigmoid (u = v) and, since (1 + tanh t) / 2 is the sigmoid of 2 t, gelu_tanh, whose
 // u = v (a + b v^2) alone takes the square, which overflows from 2^64 on: times a b of zero it would be no number.  A
 // negative u's exponential comes as its root on either factor, as swiglu's, so that results keep their bits down to fp32's
-// least: off by 16 + 2 |u| half steps at most, gelu_tanh by the five more of u's own roundings, |u| times.
+// least: off by 16 + 2 |u| half steps at most, gelu_tanh by up to 20 + 7 |u| with u's own roundings.
 struct SigmoidForm {
   bool cubic, times;
   __device__ __forceinline__ explicit SigmoidForm(uint32_t activation)
@@ -429,9 +430,11 @@ __device__ __forceinline__ uint32_t strip_swz(uint32_t r) { return (((r >> 1) ^ 
 // and a slot of MFMAs; the second group runs a slot behind the first, so that one reads while the other multiplies.  Four
 // stages hold the step being read and three on their way.  Every wait for loads is the kernel's own: the compiler's, for
 // loads that it issued, came before every read and cost a third of the time.
-// 8192 x 2560 x 2560 84 to 88 us at 256 x 320 (two stages of 128 bytes 95, half of the matrix rows per slot 90, loads'
+// 8192 x 2560 x 2560 85 to 86 us at 256 x 320 (two stages of 128 bytes 95, half of the matrix rows per slot 90, loads'
 // addresses in 64 bits 87), of which the MFMAs take 50 at the 2.0 GHz that it runs at; with bias, SiLU and residual 98, of
-// operands that come from HBM 112.  A library's product of this size, without an epilogue, took 106.  Not kept: loads in
+// operands that come from HBM 112 in a graph and 115 to 120 traced.  A library's product of this size, without an epilogue,
+// took 106.  Of MX 2560 -> 2 x 640 with SwiGLU 54: the MFMAs take 51,200 cycles of a SIMD, 40 % of that at 2.4 GHz, beside 3.4
+// other vector instructions to one of them, most of them conversions.  Not kept: loads in
 // the MFMAs' slot, waves' priorities the other way round (within 1 %), lines of later steps (4 to 8 ahead) or of the residual
 // asked for beforehand (8 % and 1 % slower).
 // Fragments of the matrix are dealt in pairs: a lane's eight values of a pair are neighbouring outputs of its row (with

@@ -36,6 +36,9 @@ def linear(x, weight, bias: torch.Tensor = None, *, activation: str = None, resi
     residual [.., n] in bfloat16 or float32; ``dtype`` bfloat16 or float32.  Returns [.., n].  ``out`` [.., n] (of
     ``dtype``, rows equally spaced) may be residual where the types match, and overlaps nothing otherwise.  MX values
     enter as bfloat16: those below 2^-126 are rounded to multiples of 2^-133, those of 2^128 and above are infinite.
+    silu, swiglu and sigmoid are off by at most 16 + 2 |x| half steps of fp32, gelu by 12 + 4 x^2, gelu_tanh by 20 + 7 |u|, u
+    its sigmoid's argument; where the formula is infinity times zero (silu, gelu, gelu_tanh and swiglu at -infinity) they are
+    NaN.
     """
     mx = isinstance(x, MxTensor)
     if mx != isinstance(weight, MxTensor):
